@@ -418,6 +418,84 @@ MTC_API int mtc_rd_search(const float* W, int32_t K, int32_t N, int32_t block_si
                           int32_t mode, const float* alphas, int32_t n_alpha, int32_t bf16_scales,
                           double* out_dist, float* out_scale, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit floating point (e4m3) matrices, and experts built of them.  No
+ * counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+
+/* Element types of activations and outputs. */
+enum { MTC_F32 = 0, MTC_BF16 = 1, MTC_F16 = 2 };
+
+/* E stacked K x N weights (in_features x out_features) in e4m3: codes as
+ * [E][N][ldk] (one row of K codes per output feature, ldk a multiple of 16,
+ * 16-byte aligned), scales as [E][ceil(N/128)][ceil(K/128)], one fp32 scale
+ * per 128 x 128 block.  W[e][k][n] = code[e][n][k] * scale[e][n/128][k/128].
+ * A NaN code makes the outputs of its feature NaN. */
+typedef struct mtc_fp8_matrix {
+  const uint8_t* codes;
+  const float* scales;
+  int64_t ldk;
+  int32_t E, K, N;
+  int32_t pad_;
+} mtc_fp8_matrix;
+
+/* W (K x N fp32, row stride ldw) to codes and scales of one matrix: per block
+ * amax = max(max|w|, 2^-100), scale = amax / 448, code = e4m3(w * (448 /
+ * amax)), each step rounded to nearest even in fp32.  A block holding an
+ * infinity or a NaN gets a NaN scale and zero codes. */
+MTC_API int mtc_fp8_pack(const float* W, int32_t K, int32_t N, int64_t ldw, uint8_t* codes, int64_t ldk,
+                         float* scales, void* stream);
+
+/* Matrix e of w as fp32: out[k][n] = code * scale (one rounding), row stride ldo. */
+MTC_API int mtc_fp8_unpack(const mtc_fp8_matrix* w, int32_t e, float* out, int64_t ldo, void* stream);
+
+/* Activations X (M x K, type MTC_F32 / BF16 / F16, row stride ldx) to codes
+ * (M rows of ldq bytes, ldq a multiple of 16; bytes from K to ldq are
+ * written as zero) and scales (scales[b * lds + m] for inputs 128 b .. 128 b
+ * + 127 of row m), by the rule of mtc_fp8_pack per row and 128 inputs. */
+MTC_API int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_t K, int64_t ldx, uint8_t* codes,
+                             int64_t ldq, float* scales, int64_t lds, void* stream);
+
+/* Y = act(Xq @ W + bias) for one matrix (E = 1): X is quantized as by
+ * mtc_fp8_quantize, products of codes are exact, sums are fp32 (128 inputs on
+ * the tensor cores, the scaled sums of the blocks in order), Y is rounded
+ * once to its type.  Up to 16 rows need no workspace (the kernel quantizes
+ * them itself); `ws` is 256-byte aligned, its size from
+ * mtc_fp8_gemm_workspace_bytes on the same device.  Same inputs, same bits. */
+MTC_API size_t mtc_fp8_gemm_workspace_bytes(const mtc_fp8_matrix* w, int32_t M);
+MTC_API int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type, int32_t M, int64_t ldx, void* Y,
+                         int32_t y_type, int64_t ldy, void* ws, size_t ws_bytes, uint32_t* status,
+                         const mtc_epilogue* ep, void* stream);
+
+/* Routing of T tokens to k of E experts (E <= 1024, k <= 32) from router
+ * logits (T x E, row stride ld).  Scores: softmax over the experts, or
+ * sigmoid.  The choice goes by score + bias (bias: E finite floats, or NULL)
+ * in 64 bits.  With groups > 1 (at most 32, dividing E) only the experts of
+ * the top_groups groups with the largest sum of their two best choices
+ * compete.  ids: the k best, best first, ties to the lowest index; weights:
+ * their scores (without bias), divided by their sum if renormalize, times
+ * scale.  A logit of -inf or NaN is a masked expert: score 0, chosen only
+ * when no other is left; +inf counts as the largest finite number.  A row
+ * with masked experts only has weights 0. */
+enum { MTC_SCORE_SOFTMAX = 0, MTC_SCORE_SIGMOID = 1 };
+MTC_API int mtc_route_experts(const void* logits, int32_t type, int32_t T, int32_t E, int64_t ld, int32_t k,
+                              int32_t score, const float* bias, int32_t groups, int32_t top_groups,
+                              int32_t renormalize, float scale, int32_t* ids, float* weights, void* stream);
+
+/* Gated feed-forward of the chosen experts: Y[t] = sum_j weights[t][j] *
+ * (act(x_t Wg) * (x_t Wu)) Wd with the matrices of expert ids[t][j]; gate and
+ * up are E x (K = D, N = I), down is E x (K = I, N = D).  x_t and the gated
+ * values are quantized as by mtc_fp8_quantize; the gated values are fp32
+ * before that, the experts' outputs are rounded to Y's type, weighted and
+ * added in fp32 in the order of j, and rounded once more.  An id outside
+ * 0..E-1 is no expert and adds nothing.  `ws` is 256-byte aligned, its size
+ * from mtc_experts_workspace_bytes.  Y must not overlap X. */
+MTC_API size_t mtc_experts_workspace_bytes(const mtc_fp8_matrix* gate, int32_t T, int32_t k, int32_t y_type);
+MTC_API int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_matrix* up, const mtc_fp8_matrix* down,
+                                const void* X, int32_t x_type, int32_t T, int64_t ldx, const int32_t* ids,
+                                const float* weights, int32_t k, int32_t act, void* Y, int32_t y_type, int64_t ldy,
+                                void* ws, size_t ws_bytes, uint32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -76,6 +76,19 @@ ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_TANH = 0, 1, 2, 3
 ACTIVATIONS = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "gelu_tanh": ACT_GELU_TANH}
 _EP = ctypes.POINTER(Epilogue)
 
+
+class FP8Desc(ctypes.Structure):
+    """struct mtc_fp8_matrix: E stacked K x N matrices of e4m3 codes."""
+
+    _fields_ = [("codes", c_p), ("scales", c_p), ("ldk", c_i64), ("E", c_i32), ("K", c_i32), ("N", c_i32),
+                ("pad_", c_i32)]
+
+
+assert ctypes.sizeof(FP8Desc) == 40
+_FP8 = ctypes.POINTER(FP8Desc)
+F32, BF16, F16 = 0, 1, 2
+SCORES = {"softmax": 0, "sigmoid": 1}
+
 # name -> (restype, argtypes); every symbol declared in include/mtc_b200.h.
 SIGNATURES = {
     "mtc_abi_version": (c_i32, []),
@@ -112,6 +125,16 @@ SIGNATURES = {
     "mtc_prefill_gemm": (c_i32, [ctypes.POINTER(StreamDesc), c_i32, c_p, c_i64, c_i32, c_p, c_size, c_p, _EP,
                                  c_p]),
     "mtc_prefill_scatter": (c_i32, [ctypes.POINTER(StreamDesc), c_i32, c_p, c_p, c_i64, c_p, c_size, _EP, c_p]),
+    "mtc_fp8_pack": (c_i32, [c_p, c_i32, c_i32, c_i64, c_p, c_i64, c_p, c_p]),
+    "mtc_fp8_unpack": (c_i32, [_FP8, c_i32, c_p, c_i64, c_p]),
+    "mtc_fp8_quantize": (c_i32, [c_p, c_i32, c_i32, c_i32, c_i64, c_p, c_i64, c_p, c_i64, c_p]),
+    "mtc_fp8_gemm_workspace_bytes": (c_size, [_FP8, c_i32]),
+    "mtc_fp8_gemm": (c_i32, [_FP8, c_p, c_i32, c_i32, c_i64, c_p, c_i32, c_i64, c_p, c_size, c_p, _EP, c_p]),
+    "mtc_route_experts": (c_i32, [c_p, c_i32, c_i32, c_i32, c_i64, c_i32, c_i32, c_p, c_i32, c_i32, c_i32,
+                                  ctypes.c_float, c_p, c_p, c_p]),
+    "mtc_experts_workspace_bytes": (c_size, [_FP8, c_i32, c_i32, c_i32]),
+    "mtc_experts_forward": (c_i32, [_FP8, _FP8, _FP8, c_p, c_i32, c_i32, c_i64, c_p, c_p, c_i32, c_i32, c_p, c_i32,
+                                    c_i64, c_p, c_size, c_p, c_p]),
     "mtc_permute_rows": (c_i32, [c_p, c_i64, c_i64, c_i32, c_i32, c_p, c_i32, c_i32, c_p, c_i64, _EP, c_p]),
 }
 

@@ -1,0 +1,562 @@
+// Mixture-of-experts operators: routing (scores, group limit, top-k), the
+// plan that sorts token rows by expert, the weighted sum of the experts'
+// outputs, and the gated feed-forward that runs them with the 8-bit products.
+#include "mtc_fp8.cuh"
+#include "mtc_fp8_internal.h"
+
+namespace mtc {
+namespace fp8 {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 32;
+constexpr int kMaxGroups = 32;
+
+// ---------------------------------------------------------------------------
+// Routing: one warp per token
+// ---------------------------------------------------------------------------
+struct RouteParams {
+  const void* logits;
+  long long ld;
+  int T, E, k, sigmoid;
+  const float* bias;
+  int groups, gsize, top_groups, renorm;
+  double scale;
+  int32_t* ids;
+  float* weights;
+};
+
+// A score that decides: 64-bit order, so that experts whose scores agree in
+// 32 bits are still told apart.  The unsigned order of the key is the order
+// of the value; key 1 is a masked (-inf or NaN) expert, key 0 one that may
+// not be chosen.
+__device__ __forceinline__ unsigned long long order_key(double c) {
+  if (!(c > -INFINITY)) return 1ull;  // -inf, NaN
+  const long long b = __double_as_longlong(c);
+  return (unsigned long long)b ^ (b < 0 ? ~0ull : 0x8000000000000000ull);
+}
+
+template <typename T, int NPL>
+__global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
+  extern __shared__ double route_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * (blockDim.x >> 5) + warp;
+  if (t >= p.T) return;
+  const T* z = reinterpret_cast<const T*>(p.logits) + t * p.ld;
+  float v[NPL];
+  float zmax = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) {
+    const int e = 32 * i + lane;
+    float x = -INFINITY;
+    if (e < p.E) {
+      x = to_f32(z[e]);
+      if (x != x) x = -INFINITY;
+      x = fminf(x, 3.402823466e38f);
+    }
+    v[i] = x;
+    zmax = fmaxf(zmax, x);
+  }
+  for (int d = 16; d; d >>= 1) zmax = fmaxf(zmax, __shfl_xor_sync(0xffffffffu, zmax, d));
+  // score of a logit: exp(z - max) / total, or 1 / (1 + exp(-z)); a masked one has score 0
+  auto raw_score = [&](float x) -> double {
+    if (x == -INFINITY) return 0.0;
+    return p.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : exp((double)x - (double)zmax);
+  };
+  double total = 1.0;
+  unsigned long long key[NPL];
+  {
+    double c[NPL];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      c[i] = raw_score(v[i]);
+      sum += c[i];
+    }
+    if (!p.sigmoid) {
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      total = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const int e = 32 * i + lane;
+      if (!p.sigmoid) c[i] = c[i] / total;
+      if (p.bias && e < p.E) c[i] += (double)p.bias[e];
+      if (v[i] == -INFINITY) c[i] = -INFINITY;
+    }
+    uint32_t keep = ~0u;
+    if (p.groups > 1) {
+      double* cs = route_smem + warp * p.E;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i)
+        if (32 * i + lane < p.E) cs[32 * i + lane] = c[i];
+      __syncwarp();
+      double g1 = -INFINITY, g2 = -INFINITY;
+      if (lane < p.groups)
+        for (int i = 0; i < p.gsize; ++i) {
+          const double x = cs[lane * p.gsize + i];
+          if (x > g1) {
+            g2 = g1;
+            g1 = x;
+          } else if (x > g2) {
+            g2 = x;
+          }
+        }
+      const double gv = p.gsize > 1 ? g1 + g2 : g1;
+      int rank = 0;
+      for (int g = 0; g < p.groups; ++g) {
+        const double o = __shfl_sync(0xffffffffu, gv, g);
+        rank += o > gv || (o == gv && g < lane);
+      }
+      keep = __ballot_sync(0xffffffffu, lane < p.groups && rank < p.top_groups);
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const int e = 32 * i + lane;
+      key[i] = 0ull;
+      if (e < p.E && (p.groups == 1 || (keep >> (e / p.gsize) & 1u))) key[i] = order_key(c[i]);
+    }
+  }
+  int my_id = 0;
+  for (int j = 0; j < p.k; ++j) {
+    unsigned long long best = 0ull;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    const uint32_t hi = (uint32_t)(best >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t lo = hi == mh ? (uint32_t)best : 0u, ml = __reduce_max_sync(0xffffffffu, lo);
+    const uint32_t mine = (hi == mh && lo == ml) ? (uint32_t)(32 * at + lane) : ~0u;
+    const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
+    if (mine == id) {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i)
+        if (i == at) key[i] = 0ull;
+    }
+    if (lane == j) my_id = (int)id;
+  }
+  double w = 0.0;
+  if (lane < p.k) {
+    float x = to_f32(z[my_id]);
+    if (x != x) x = -INFINITY;
+    w = raw_score(fminf(x, 3.402823466e38f));
+  }
+  double div = total;
+  if (p.renorm) {
+    div = w;
+    for (int d = 16; d; d >>= 1) div += __shfl_xor_sync(0xffffffffu, div, d);
+  }
+  if (lane < p.k) {
+    p.ids[(long long)t * p.k + lane] = my_id;
+    p.weights[(long long)t * p.k + lane] = (float)(div > 0.0 ? w / div * p.scale : 0.0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Plan: rows (t, j) sorted by expert, stable, by one CTA
+// ---------------------------------------------------------------------------
+struct PlanParams {
+  const int32_t* ids;
+  int R, E, size;        // rows T * k, experts, rows per slot
+  int32_t* order;        // [R] row (t * k + j) at each sorted place
+  int32_t* pos;          // [R] sorted place of each row, -1 for an id outside 0..E-1
+  int32_t* slots;        // slot list
+  int32_t* n_rows;       // rows that have an expert
+};
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive scan of one value per thread over the CTA.
+__device__ __forceinline__ int block_scan(int x, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int s = x;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += o;
+  }
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    int v = warp_sums[lane], q = v;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, q, d);
+      if (lane >= d) q += o;
+    }
+    warp_sums[lane] = q - v;
+    if (lane == 31) warp_sums[32] = q;
+  }
+  __syncthreads();
+  const int r = warp_sums[warp] + s - x;
+  *total = warp_sums[32];
+  __syncthreads();
+  return r;
+}
+
+// Each warp owns a contiguous piece of the rows: it counts its experts, the
+// counts become places (experts in order, inside an expert the pieces in
+// order), and a second pass hands out the places in row order.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
+  extern __shared__ int32_t hist[];  // [32][E]
+  __shared__ int warp_sums[33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < 32 * p.E; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  const int piece = (((p.R + 31) >> 5) + 31) & ~31;
+  const int r0 = min((long long)warp * piece, (long long)p.R), r1 = min(r0 + piece, p.R);
+  int32_t* mine = hist + warp * p.E;
+  for (int r = r0 + lane; r < r1; r += 32) {
+    const int e = p.ids[r];
+    if ((unsigned)e < (unsigned)p.E) atomicAdd(&mine[e], 1);
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  int count = 0;
+  if (e < p.E)
+    for (int w = 0; w < 32; ++w) {
+      const int c = hist[w * p.E + e];
+      hist[w * p.E + e] = count;
+      count += c;
+    }
+  int total, n_slots;
+  const int off = block_scan(count, warp_sums, &total);
+  const int ns = (count + p.size - 1) / p.size;
+  const int sl = block_scan(ns, warp_sums, &n_slots);
+  if (e < p.E) {
+    for (int w = 0; w < 32; ++w) hist[w * p.E + e] += off;
+    for (int i = 0; i < ns; ++i)
+      *reinterpret_cast<int4*>(p.slots + 4 + 4 * (sl + i)) = make_int4(e, off + i * p.size, off + count, 0);
+  }
+  if (threadIdx.x == 0) {
+    p.slots[0] = n_slots;
+    *p.n_rows = total;
+  }
+  __syncthreads();
+  for (int rb = r0; rb < r1; rb += 32) {
+    const int r = rb + lane;
+    const int id = r < r1 ? p.ids[r] : -1;
+    const bool ok = (unsigned)id < (unsigned)p.E;
+    const uint32_t same = __match_any_sync(0xffffffffu, ok ? id : -1);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    int at = -1;
+    if (ok) at = mine[id] + rank;
+    __syncwarp();
+    if (ok && rank == 0) mine[id] += __popc(same);
+    __syncwarp();
+    if (r < r1) {
+      p.pos[r] = at;
+      if (ok) p.order[at] = r;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Y[t] = sum_j weights[t][j] * rows[pos[t][j]], j in order, fp32
+// ---------------------------------------------------------------------------
+struct CombineParams {
+  const void* rows;
+  long long ldr;
+  const int32_t* pos;
+  const float* weights;
+  int T, k, D;
+  void* Y;
+  long long ldy;
+  int ydt, vec;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+  const int t = blockIdx.x;
+  __shared__ int at[kMaxTopK];
+  __shared__ float w[kMaxTopK];
+  if (threadIdx.x < p.k) {
+    at[threadIdx.x] = p.pos[(long long)t * p.k + threadIdx.x];
+    w[threadIdx.x] = p.weights[(long long)t * p.k + threadIdx.x];
+  }
+  __syncthreads();
+  for (int d = 8 * threadIdx.x; d < p.D; d += 8 * 256) {
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = 0.0f;
+    for (int j = 0; j < p.k; ++j) {
+      if (at[j] < 0) continue;
+      float v[8];
+      load8(reinterpret_cast<const T*>(p.rows) + at[j] * p.ldr + d, p.D - d, true, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = fmaf(w[j], v[i], a[i]);
+    }
+    const long long y = t * p.ldy + d;
+    if (p.vec && d + 8 <= p.D) {
+      if (p.ydt == MTC_F32) {
+        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + y);
+        o[0] = make_float4(a[0], a[1], a[2], a[3]);
+        o[1] = make_float4(a[4], a[5], a[6], a[7]);
+      } else {
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.Y) + y) =
+            make_uint4(pack2(p.ydt, a[0], a[1]), pack2(p.ydt, a[2], a[3]), pack2(p.ydt, a[4], a[5]),
+                       pack2(p.ydt, a[6], a[7]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (d + i < p.D) store1(p.Y, p.ydt, y + i, a[i]);
+    }
+  }
+}
+
+bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16; }
+size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// How the experts' products run, from the mean number of rows of an expert:
+// up to 8, 16-row tiles whose tokens the products quantize themselves; up to
+// 96, wider tiles of codes; above, the 128-token kernel.
+struct ExpertsPlan {
+  int R, tile, slot_bound, slot_expect;
+  bool raw, many;
+  long long ldx, ldh, ldg, lds, ldo;
+  size_t order, pos, slots, n_rows, xq, xs, gu, hq, hs, out, bytes;
+};
+bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
+  const long long R = (long long)T * k;
+  if (R > 0x7fff0000ll) return false;
+  pl->R = (int)R;
+  const double mean = (double)R / E;
+  pl->raw = mean <= 8.0;
+  pl->many = mean > 96.0;
+  pl->tile = pl->raw ? 16 : mean <= 20.0 ? 32 : mean <= 40.0 ? 64 : 128;
+  const long long used = R < E ? R : E;
+  long long bound = R / pl->tile + used;
+  if (bound > R) bound = R;
+  pl->slot_bound = (int)bound;
+  const long long expect = used + (long long)(mean / pl->tile) * E;
+  pl->slot_expect = (int)(expect < bound ? expect : bound);
+  pl->ldx = (D + 15) & ~15ll;
+  pl->ldh = (I + 15) & ~15ll;
+  pl->ldg = (I + 3) & ~3ll;
+  pl->lds = (R + 3) & ~3ll;
+  pl->ldo = (D + 7) & ~7ll;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t here = at;
+    at += round256(n);
+    return here;
+  };
+  pl->order = take(4 * (size_t)R);
+  pl->pos = take(4 * (size_t)R);
+  pl->slots = take(16 * (size_t)(pl->slot_bound + 1));
+  pl->n_rows = take(4);
+  pl->xq = pl->xs = pl->gu = pl->hq = pl->hs = 0;
+  if (!pl->raw) {
+    pl->xq = take((size_t)R * pl->ldx);
+    pl->xs = take((size_t)((D + 127) / 128) * pl->lds * 4);
+    pl->hq = take((size_t)R * pl->ldh);
+    pl->hs = take((size_t)((I + 127) / 128) * pl->lds * 4);
+  }
+  if (!pl->many) pl->gu = take((size_t)R * 2 * pl->ldg * 4);
+  pl->out = take((size_t)R * pl->ldo * (ydt == MTC_F32 ? 4 : 2));
+  pl->bytes = at;
+  return true;
+}
+
+template <typename T>
+int launch_route(const RouteParams& p, cudaStream_t st) {
+  const int warps = p.groups > 1 && p.E > 512 ? 4 : 8;
+  const size_t smem = p.groups > 1 ? (size_t)warps * p.E * 8 : 0;
+  auto go = [&](auto kernel) -> int {
+    if (smem > 48 * 1024)
+      MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                     "mtc_route_experts");
+    kernel<<<(p.T + warps - 1) / warps, 32 * warps, smem, st>>>(p);
+    MTC_CHECK_LAUNCH("mtc_route_experts");
+    return MTC_OK;
+  };
+  if (p.E <= 32) return go(route_kernel<T, 1>);
+  if (p.E <= 64) return go(route_kernel<T, 2>);
+  if (p.E <= 128) return go(route_kernel<T, 4>);
+  if (p.E <= 256) return go(route_kernel<T, 8>);
+  if (p.E <= 512) return go(route_kernel<T, 16>);
+  return go(route_kernel<T, 32>);
+}
+
+}  // namespace
+}  // namespace fp8
+}  // namespace mtc
+
+using namespace mtc;
+using namespace mtc::fp8;
+
+extern "C" int mtc_route_experts(const void* logits, int32_t type, int32_t T, int32_t E, int64_t ld, int32_t k,
+                                 int32_t score, const float* bias, int32_t groups, int32_t top_groups,
+                                 int32_t renormalize, float scale, int32_t* ids, float* weights, void* stream) {
+  clear_error();
+  MTC_REQUIRE(logits && ids && weights, "mtc_route_experts: null pointer");
+  MTC_REQUIRE(dtype_ok(type), "mtc_route_experts: unknown element type %d", type);
+  MTC_REQUIRE(score == MTC_SCORE_SOFTMAX || score == MTC_SCORE_SIGMOID, "mtc_route_experts: unknown score %d", score);
+  MTC_REQUIRE(T >= 0 && E >= 1 && E <= kMaxExperts && ld >= E, "mtc_route_experts: bad shape (T=%d, E=%d, ld=%lld)", T,
+              E, (long long)ld);
+  MTC_REQUIRE(groups >= 1 && groups <= kMaxGroups && E % groups == 0 && top_groups >= 1 && top_groups <= groups,
+              "mtc_route_experts: %d experts in %d groups, %d of them kept", E, groups, top_groups);
+  MTC_REQUIRE(k >= 1 && k <= kMaxTopK && k <= top_groups * (E / groups),
+              "mtc_route_experts: k=%d outside 1..%d", k, top_groups * (E / groups) < kMaxTopK ? top_groups * (E / groups) : kMaxTopK);
+  if (T == 0) return MTC_OK;
+  RouteParams p = {};
+  p.logits = logits;
+  p.ld = ld;
+  p.T = T;
+  p.E = E;
+  p.k = k;
+  p.sigmoid = score == MTC_SCORE_SIGMOID;
+  p.bias = bias;
+  p.groups = groups == top_groups ? 1 : groups;  // every group kept: no limit
+  p.gsize = E / groups;
+  p.top_groups = top_groups;
+  p.renorm = renormalize != 0;
+  p.scale = (double)scale;
+  p.ids = ids;
+  p.weights = weights;
+  if (type == MTC_F32) return launch_route<float>(p, as_stream(stream));
+  if (type == MTC_BF16) return launch_route<__nv_bfloat16>(p, as_stream(stream));
+  return launch_route<__half>(p, as_stream(stream));
+}
+
+extern "C" size_t mtc_experts_workspace_bytes(const mtc_fp8_matrix* gate, int32_t T, int32_t k, int32_t y_type) {
+  ExpertsPlan pl;
+  if (!gate || T < 1 || k < 1 || !experts_plan(T, k, gate->E, gate->K, gate->N, y_type, &pl)) return 0;
+  return pl.bytes;
+}
+
+extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_matrix* up, const mtc_fp8_matrix* down,
+                                   const void* X, int32_t x_type, int32_t T, int64_t ldx, const int32_t* ids,
+                                   const float* weights, int32_t k, int32_t act, void* Y, int32_t y_type, int64_t ldy,
+                                   void* ws, size_t ws_bytes, uint32_t* status, void* stream) {
+  const char* who = "mtc_experts_forward";
+  clear_error();
+  int rc = check_matrix(gate, who);
+  if (rc == MTC_OK) rc = check_matrix(up, who);
+  if (rc == MTC_OK) rc = check_matrix(down, who);
+  if (rc != MTC_OK) return rc;
+  MTC_REQUIRE(up->E == gate->E && up->K == gate->K && up->N == gate->N, "%s: gate and up differ in shape", who);
+  MTC_REQUIRE(down->E == gate->E && down->K == gate->N && down->N == gate->K, "%s: down is not the transpose shape of gate",
+              who);
+  MTC_REQUIRE(gate->E <= kMaxExperts, "%s: %d experts, at most %d", who, gate->E, kMaxExperts);
+  MTC_REQUIRE(X && ids && weights && Y, "%s: null pointer", who);
+  MTC_REQUIRE(dtype_ok(x_type) && dtype_ok(y_type), "%s: unknown element type", who);
+  MTC_REQUIRE(act >= MTC_ACT_NONE && act <= MTC_ACT_GELU_TANH, "%s: unknown activation %d", who, act);
+  MTC_REQUIRE(T >= 1 && k >= 1 && k <= kMaxTopK && ldx >= gate->K && ldy >= gate->K,
+              "%s: bad shape (T=%d, k=%d, ldx=%lld, ldy=%lld)", who, T, k, (long long)ldx, (long long)ldy);
+  const int E = gate->E, D = gate->K, I = gate->N;
+  ExpertsPlan pl;
+  MTC_REQUIRE(experts_plan(T, k, E, D, I, y_type, &pl), "%s: too many rows (%d x %d)", who, T, k);
+  if (ws_bytes < pl.bytes || !ws || (reinterpret_cast<uintptr_t>(ws) & 255)) {
+    set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, pl.bytes, ws_bytes);
+    return MTC_ERR_WORKSPACE;
+  }
+  const cudaStream_t st = as_stream(stream);
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  int32_t* order = reinterpret_cast<int32_t*>(base + pl.order);
+  int32_t* pos = reinterpret_cast<int32_t*>(base + pl.pos);
+  int32_t* slots = reinterpret_cast<int32_t*>(base + pl.slots);
+  int32_t* n_rows = reinterpret_cast<int32_t*>(base + pl.n_rows);
+  float* gu = reinterpret_cast<float*>(base + pl.gu);
+  {
+    PlanParams p = {ids, pl.R, E, pl.tile, order, pos, slots, n_rows};
+    const size_t smem = (size_t)32 * E * 4;
+    if (smem > 48 * 1024)
+      MTC_CHECK_CUDA(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+    plan_kernel<<<1, kPlanThreads, smem, st>>>(p);
+    MTC_CHECK_LAUNCH(who);
+  }
+  Product a;
+  a.w[0] = gate;
+  a.w[1] = up;
+  a.slots = slots;
+  a.slot_bound = pl.slot_bound;
+  a.slot_expect = pl.slot_expect;
+  a.rows = pl.R;
+  a.tile = pl.tile;
+  a.many = pl.many;
+  a.gate_act = act;
+  a.status = status;
+  Product b = a;
+  b.w[0] = down;
+  b.w[1] = nullptr;
+  if (!pl.raw) {
+    QuantRows q;
+    q.X = X;
+    q.dt = x_type;
+    q.M = T;
+    q.K = D;
+    q.ldx = ldx;
+    q.pos = pos;
+    q.copies = k;
+    q.q = base + pl.xq;
+    q.ldq = pl.ldx;
+    q.s = reinterpret_cast<float*>(base + pl.xs);
+    q.lds = pl.lds;
+    rc = launch_quantize(q, st, who);
+    if (rc != MTC_OK) return rc;
+    a.xq = q.q;
+    a.ldq = q.ldq;
+    a.sx = q.s;
+    a.lds = q.lds;
+    b.xq = base + pl.hq;
+    b.ldq = pl.ldh;
+    b.sx = reinterpret_cast<float*>(base + pl.hs);
+    b.lds = pl.lds;
+  } else {
+    a.X = X;
+    a.xdt = x_type;
+    a.ldx = ldx;
+    a.order = order;
+    a.kdiv = k;
+    b.gated_src = true;
+    b.X = gu;
+    b.ldx = 2 * pl.ldg;
+    b.src_off = pl.ldg;
+  }
+  if (pl.many) {
+    a.hq = base + pl.hq;
+    a.ldh = pl.ldh;
+    a.hs = reinterpret_cast<float*>(base + pl.hs);
+    a.hs_ld = pl.lds;
+  } else {
+    a.Y = gu;
+    a.ydt = MTC_F32;
+    a.ldy = 2 * pl.ldg;
+    a.mat_off = pl.ldg;
+  }
+  rc = launch_product(a, st, who);
+  if (rc != MTC_OK) return rc;
+  if (!pl.raw && !pl.many) {
+    QuantRows q;
+    q.X = gu;
+    q.dt = MTC_F32;
+    q.M = pl.R;
+    q.K = I;
+    q.ldx = 2 * pl.ldg;
+    q.gated = true;
+    q.src_off = pl.ldg;
+    q.gate_act = act;
+    q.n_rows = n_rows;
+    q.q = base + pl.hq;
+    q.ldq = pl.ldh;
+    q.s = reinterpret_cast<float*>(base + pl.hs);
+    q.lds = pl.lds;
+    rc = launch_quantize(q, st, who);
+    if (rc != MTC_OK) return rc;
+  }
+  b.Y = base + pl.out;
+  b.ydt = y_type;
+  b.ldy = pl.ldo;
+  rc = launch_product(b, st, who);
+  if (rc != MTC_OK) return rc;
+  CombineParams c = {base + pl.out, pl.ldo, pos, weights, T, k, D, Y, ldy, y_type, 0};
+  c.vec = (reinterpret_cast<uintptr_t>(Y) & 15) == 0 && ldy % (y_type == MTC_F32 ? 4 : 8) == 0;
+  if (y_type == MTC_F32) combine_kernel<float><<<T, 256, 0, st>>>(c);
+  else if (y_type == MTC_BF16) combine_kernel<__nv_bfloat16><<<T, 256, 0, st>>>(c);
+  else combine_kernel<__half><<<T, 256, 0, st>>>(c);
+  MTC_CHECK_LAUNCH(who);
+  return MTC_OK;
+}

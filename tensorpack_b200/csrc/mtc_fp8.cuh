@@ -1,0 +1,214 @@
+// Device helpers of the 8-bit (e4m3) kernels: the quantization of one group
+// of 128 values, tcgen05 kind::f8f6f4 with fp32 accumulators in TMEM, TMEM
+// loads that are waited for separately, and the token tiles ("slots") that
+// dense and grouped products share.
+//
+// Format.  A weight matrix of K inputs and N outputs is stored as N rows of
+// K codes (one row per output feature) with one fp32 scale per 128 x 128
+// block; activations are rows of K codes with one fp32 scale per row and 128
+// inputs.  A product is a sum over blocks of 128 inputs,
+//   Y[m][n] = sum_b sx[m][b] sw[n / 128][b] sum_{k in block b} qx[m][k] qw[n][k],
+// whose inner sum the tensor cores leave in TMEM; CUDA cores multiply it by
+// the two scales and add it up in fp32 registers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "mtc_common.cuh"
+#include "mtc_tc.cuh"
+
+namespace mtc {
+namespace fp8 {
+
+constexpr int kBlock = 128;                   // inputs (and outputs) per scale
+constexpr float kMax = 448.0f;                // largest e4m3 value
+constexpr uint32_t kFloorBits = 27u << 23;    // 2^-100: amax below this is raised to it
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// The scale of a group and the factor its values are multiplied by, from the
+// bits of its largest |x| (unsigned order of the bits is the order of the
+// values, with infinity and NaN above every number).  amax / 448 and
+// 448 / amax are both rounded once; a group holding an infinity or a NaN gets
+// a NaN scale and zero codes, so that its row of every product is NaN.
+struct GroupScale {
+  float scale, mul;
+};
+__device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
+  GroupScale g;
+  if (amax_bits >= kInfBits) {
+    g.scale = __uint_as_float(0x7fffffffu);
+    g.mul = 0.0f;
+  } else {
+    const float a = __uint_as_float(amax_bits < kFloorBits ? kFloorBits : amax_bits);
+    g.scale = __fdiv_rn(a, kMax);
+    g.mul = __fdiv_rn(kMax, a);
+  }
+  return g;
+}
+
+// Two codes e4m3(a * mul), e4m3(b * mul): round to nearest even, saturating
+// at 448 (a * mul can exceed it by one rounding).  mul = 0 marks a group that
+// is not finite.
+__device__ __forceinline__ uint32_t codes2(float a, float b, float mul) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(a, mul), __fmul_rn(b, mul)), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float mul) {
+  if (mul == 0.0f) return make_uint2(0u, 0u);
+  uint2 r;
+  r.x = codes2(v[0], v[1], mul) | codes2(v[2], v[3], mul) << 16;
+  r.y = codes2(v[4], v[5], mul) | codes2(v[6], v[7], mul) << 16;
+  return r;
+}
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
+  uint32_t m = abs_bits(v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = max(m, abs_bits(v[i]));
+  return m;
+}
+// Largest over the 16 lanes of a half warp.
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {
+#pragma unroll
+  for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  return m;
+}
+
+// Element types of activations and outputs (mtc_dtype of the C ABI).
+template <int DT>
+struct Elem;
+template <>
+struct Elem<MTC_F32> {
+  typedef float T;
+};
+template <>
+struct Elem<MTC_BF16> {
+  typedef __nv_bfloat16 T;
+};
+template <>
+struct Elem<MTC_F16> {
+  typedef __half T;
+};
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+
+// Eight consecutive values at p as fp32; `n` of them exist (the others read
+// as zero).  `vec`: p is 16-byte aligned and n >= 8 may be read as vectors.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        T lo, hi;
+        *reinterpret_cast<uint16_t*>(&lo) = (uint16_t)(w[i] & 0xffffu);
+        *reinterpret_cast<uint16_t*>(&hi) = (uint16_t)(w[i] >> 16);
+        v[2 * i] = to_f32(lo);
+        v[2 * i + 1] = to_f32(hi);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+  }
+}
+
+// One output value in the output's type (fp32, or rounded once to nearest).
+__device__ __forceinline__ void store1(void* y, int dt, long long i, float v) {
+  if (dt == MTC_F32) reinterpret_cast<float*>(y)[i] = v;
+  else if (dt == MTC_BF16) reinterpret_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(y)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ uint32_t pack2(int dt, float a, float b) {
+  if (dt == MTC_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---------------------------------------------------------------------------
+// tcgen05, 8-bit operands
+// ---------------------------------------------------------------------------
+// Instruction descriptor for kind::f8f6f4: e4m3 A and B, fp32 D, both K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// D (TMEM) = or += A B^T for 32 inputs; operands by shared-memory descriptor.
+__device__ __forceinline__ void mma_e4m3_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 16 consecutive fp32 columns, not waited for: thread i gets lane
+// (base + i).  tmem_wait16 completes it and ties the registers to the wait.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                 "+r"(v[15])
+               :
+               : "memory");
+}
+
+// acc[0..1] += v[0..1] * s (two fp32 products in one instruction).
+__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t v1, float s) {
+  unsigned long long a, v, m;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(m) : "f"(s));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(v), "l"(m));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
+}
+
+// ---------------------------------------------------------------------------
+// Token tiles
+// ---------------------------------------------------------------------------
+// Slot list written by the plan kernel for a grouped product: word 0 is the
+// number of slots, slot i is {expert, first row, end row of the expert, 0} at
+// words 4 + 4 i.  A dense product has no list: slot i covers rows from
+// i * size of the single matrix.
+struct Slot {
+  int e, row0, end;
+};
+__device__ __forceinline__ int slot_count(const int32_t* slots, int M, int size) {
+  return slots ? __ldg(slots) : (M + size - 1) / size;
+}
+__device__ __forceinline__ Slot slot_at(const int32_t* slots, int M, int size, int i) {
+  Slot s;
+  if (slots) {
+    const int4 v = *reinterpret_cast<const int4*>(slots + 4 + 4 * i);
+    s.e = v.x;
+    s.row0 = v.y;
+    s.end = v.z;
+  } else {
+    s.e = 0;
+    s.row0 = i * size;
+    s.end = M;
+  }
+  return s;
+}
+
+}  // namespace fp8
+}  // namespace mtc

@@ -1,0 +1,807 @@
+// Products with 8-bit (e4m3) weights and activations, dense and grouped by
+// expert: Y[m][n] = act(sum_b sx[m][b] sw[n/128][b] (qx[m] . qw[n])_b + bias[n])
+// with the sums of 128 inputs on the tensor cores and the scaled sums in fp32
+// registers (mtc_fp8.cuh).
+//
+// Two kernels, by the number of rows that share a weight tile:
+//
+//  * few_kernel<BN, SRC>: 128 output features x BN <= 128 tokens.  The
+//    features are the M side of the MMA (TMEM lane = feature), so one token
+//    costs 16 columns instead of 128 rows, and a warp's stores are
+//    consecutive features.  Bound by the weight bytes: each CTA streams its
+//    features' codes once through a TMA ring.  A cluster of up to 8 CTAs
+//    splits the inputs and adds its partial sums through distributed shared
+//    memory in rank order: no workspace, no atomics, the same result every
+//    time.
+//  * many_kernel<GATED>: 128 tokens x 256 features (TMEM lane = token), one
+//    persistent CTA per SM, two 256-column accumulators that alternate
+//    between the MMA and eight warps that scale and add.  Bound by the
+//    tensor cores.  GATED: the 256 features are 128 of the gate matrix and
+//    the same 128 of the up matrix; the output is act(gate) * up, quantized.
+#include "mtc_fp8.cuh"
+#include "mtc_internal.h"
+#include "mtc_fp8_internal.h"
+
+namespace mtc {
+namespace fp8 {
+namespace {
+
+constexpr uint32_t kATile = 128 * 128;  // bytes of one 128-row x 128-input tile of codes
+
+__device__ __forceinline__ void flag(uint32_t* st, uint32_t bits) {
+  if (st) atomicOr(st, bits);
+}
+
+// ---------------------------------------------------------------------------
+// few_kernel
+// ---------------------------------------------------------------------------
+enum { SRC_CODES = 0, SRC_ROWS = 1, SRC_GATED = 2 };
+
+template <int BN>
+struct FewCfg {
+  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
+  static constexpr int kAcc = BN <= 64 ? 4 : 2;        // TMEM accumulators
+  static constexpr uint32_t kBTile = BN * 128;
+  static constexpr uint32_t kStage = kATile + kBTile;
+  static constexpr int kRing = kStages + kAcc;          // slots of in-kernel token scales
+  static constexpr uint32_t kBars = kStages * kStage;
+  static constexpr size_t kSmem = 1024 + kBars + 512 + (BN == 16 ? kRing * BN * 4 : 0);
+};
+constexpr int kFewThreads = 192;      // 4 scaling warps, TMA warp, MMA warp
+constexpr int kQuantWarps = 4;        // more when the kernel quantizes its tokens itself
+
+struct FewParams {
+  int K, nkb, N, Nb, n_tiles;         // n_tiles: 128-feature tiles of one matrix
+  const float* sw[2];                 // scales of the matrix (or of gate and up)
+  const int32_t* slots;
+  int M;
+  const float* sx;                    // SRC_CODES: token scales [nkb][lds]
+  long long lds;
+  const void* X;                      // SRC_ROWS: activations; SRC_GATED: fp32 {gate, up} rows
+  int xdt, vec;
+  long long ldx;
+  const int32_t* order;               // SRC_ROWS, grouped: row r is token order[r] / kdiv
+  int kdiv;
+  int gate_act;
+  void* Y;
+  int ydt;
+  long long ldy, mat_off;             // matrix i writes at column i * mat_off
+  const float* bias;
+  int act;
+  int split;                          // CTAs of a cluster
+  uint32_t* status;
+  unsigned long long timeout_ns;
+};
+
+// One group of 128 inputs of one row by a half warp: 8 values per lane.
+template <int SRC>
+__device__ __forceinline__ void load_group(const FewParams& p, long long row, int k, float (&v)[8]) {
+  const int n = p.K - k;
+  if constexpr (SRC == SRC_GATED) {
+    const float* g = reinterpret_cast<const float*>(p.X) + row * p.ldx;
+    float u[8];
+    load8(g + k, n, p.vec, v);
+    load8(g + p.mat_off + k, n, p.vec, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = epi_act(v[i], p.gate_act) * u[i];
+  } else {
+    if (p.xdt == MTC_F32) load8(reinterpret_cast<const float*>(p.X) + row * p.ldx + k, n, p.vec, v);
+    else if (p.xdt == MTC_BF16) load8(reinterpret_cast<const __nv_bfloat16*>(p.X) + row * p.ldx + k, n, p.vec, v);
+    else load8(reinterpret_cast<const __half*>(p.X) + row * p.ldx + k, n, p.vec, v);
+  }
+}
+
+template <int BN, int SRC>
+__global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps, 2)
+    few_kernel(const __grid_constant__ CUtensorMap tw0, const __grid_constant__ CUtensorMap tw1,
+               const __grid_constant__ CUtensorMap tx, const FewParams p) {
+  using C = FewCfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + C::kAcc;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(acc_empty + C::kAcc);
+  uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
+  float* sring = reinterpret_cast<float*>(smem + C::kBars + 512);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = p.split, rank = split > 1 ? (int)tc::cluster_rank() : 0;
+  // every CTA of a cluster has the same blockIdx.y, so a cluster leaves together
+  if ((int)blockIdx.y >= slot_count(p.slots, p.M, BN)) return;
+  const Slot slot = slot_at(p.slots, p.M, BN, blockIdx.y);
+  const int ntok = min(BN, slot.end - slot.row0);
+  const int t = blockIdx.x / split, mat = t / p.n_tiles, f0 = (t - mat * p.n_tiles) * 128;
+  const int kb0 = (int)((long long)rank * p.nkb / split), kb1 = (int)((long long)(rank + 1) * p.nkb / split);
+  const int n_it = kb1 - kb0;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], SRC == SRC_CODES ? 1 : 2);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < C::kAcc; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    abort_flag[0] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) tc::tmem_alloc(tmem_slot, C::kAcc * BN);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  float acc[BN];
+  if (warp == 4) {
+    // ------------------------------------------------------------ weights (and codes of the tokens) by TMA
+    if (lane == 0) {
+      int i = 0;
+      for (; i < n_it && !abort_flag[0]; ++i) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !mbar_wait(&empty[s], ((i / C::kStages) & 1) ^ 1, p.timeout_ns)) {
+          abort_flag[0] = 1;
+          break;
+        }
+        uint8_t* st = smem + s * C::kStage;
+        mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : kATile);
+        tc::tma_load_2d(st, mat ? &tw1 : &tw0, (kb0 + i) * 128, slot.e * p.N + f0, &full[s]);
+        if constexpr (SRC == SRC_CODES) tc::tma_load_2d(st + kATile, &tx, (kb0 + i) * 128, slot.row0, &full[s]);
+      }
+      if (abort_flag[0]) {
+        // this CTA's copies in flight must land before it leaves
+        for (int j = i > C::kStages ? i - C::kStages : 0; j < i; ++j)
+          (void)mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, 10000000ull);
+        flag(p.status, MTC_STATUS_TIMEOUT);
+      }
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(128, BN);
+      for (int i = 0; i < n_it && !abort_flag[0]; ++i) {
+        const int s = i % C::kStages, b = i % C::kAcc;
+        if (!mbar_wait(&full[s], (i / C::kStages) & 1, p.timeout_ns) ||
+            (i >= C::kAcc && !mbar_wait(&acc_empty[b], ((i / C::kAcc) & 1) ^ 1, p.timeout_ns))) {
+          abort_flag[0] = 1;
+          break;
+        }
+        tc::fence_after();
+        const uint32_t a0 = smem_u32(smem + s * C::kStage), b0 = a0 + kATile;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma_e4m3_ss(tmem + b * BN, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
+                      j > 0);
+        tc::commit(&empty[s]);
+        tc::commit(&acc_full[b]);
+      }
+    }
+  } else if (warp < 4) {
+    // ------------------------------------------------------------ scale and add
+    const float* swp = p.sw[mat] + ((long long)slot.e * p.Nb + (f0 >> 7)) * p.nkb + kb0;
+    constexpr int kCols = (BN + 31) / 32;
+#pragma unroll
+    for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+    float sn[kCols];  // the next block's scales, columns lane, lane + 32, ...
+    auto load_scales = [&](int i) {
+      const float w = __ldg(swp + i);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        const int m = 32 * c + lane;
+        if constexpr (SRC == SRC_CODES) sn[c] = m < ntok ? p.sx[(long long)(kb0 + i) * p.lds + slot.row0 + m] * w : 0.0f;
+        else sn[c] = w;
+      }
+    };
+    load_scales(0);
+    for (int i = 0; i < n_it; ++i) {
+      const int b = i % C::kAcc;
+      float sc[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) sc[c] = sn[c];
+      if (i + 1 < n_it) load_scales(i + 1);
+      if (!__all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(&acc_full[b], (i / C::kAcc) & 1, p.timeout_ns))) {
+        abort_flag[0] = 1;
+        break;
+      }
+      tc::fence_after();
+      // the quantizing warps wrote this block's token scales before its MMA ran
+      if constexpr (SRC != SRC_CODES) sc[0] *= sring[(i % C::kRing) * BN + (lane & (BN - 1))];
+      uint32_t v[2][16];
+      const uint32_t ta = tmem + b * BN + ((uint32_t)(32 * warp) << 16);
+      tmem_ld16(ta, v[0]);
+#pragma unroll
+      for (int c = 0; c < BN / 16; ++c) {
+        tmem_wait16(v[c & 1]);
+        if (c + 1 < BN / 16) {
+          tmem_ld16(ta + 16 * (c + 1), v[(c + 1) & 1]);
+        } else {
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[b]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float s = __shfl_sync(0xffffffffu, sc[(16 * c + j) / 32], (16 * c + j) & 31);
+          acc[16 * c + j] = fmaf(__uint_as_float(v[c & 1][j]), s, acc[16 * c + j]);
+        }
+      }
+    }
+  } else if constexpr (SRC != SRC_CODES) {
+    // ------------------------------------------------------------ quantize the tokens: warp w takes blocks w, w + 4, ...
+    static_assert(SRC == SRC_CODES || BN == 16, "in-kernel quantization serves 16 tokens");
+    const int qw = warp - 6, half = lane >> 4, l = lane & 15;
+    const int rounds = (ntok + 1) >> 1;
+    for (int i = qw; i < n_it; i += kQuantWarps) {
+      const int s = i % C::kStages;
+      const int k = (kb0 + i) * 128 + 8 * l;
+      bool waited = false;
+      for (int r0 = 0; r0 < rounds; r0 += 4) {
+        float v[4][8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = 2 * (r0 + r) + half;
+          if (m < ntok) {
+            long long row = slot.row0 + m;
+            if (SRC == SRC_ROWS && p.order) row = p.order[row] / p.kdiv;
+            load_group<SRC>(p, row, k, v[r]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[r][q] = 0.0f;
+          }
+        }
+        if (!waited) {
+          waited = true;
+          if (i >= C::kStages &&
+              !__all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / C::kStages) & 1) ^ 1, p.timeout_ns)))
+            abort_flag[0] = 1;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = 2 * (r0 + r) + half;
+          const GroupScale g = group_scale(half_warp_max(amax8(v[r])));
+          const uint2 c = codes8(v[r], g.mul);
+          if (m < BN) {
+            // row m of the K-major SWIZZLE_128B tile: 16-byte chunk j sits at chunk j ^ (m % 8)
+            uint8_t* dst = smem + s * C::kStage + kATile + m * 128 + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8;
+            *reinterpret_cast<uint2*>(dst) = c;
+            if (l == 0) sring[(i % C::kRing) * BN + m] = g.scale;
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, abort_flag[0])) break;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+    }
+  }
+  __syncwarp();
+
+  // ------------------------------------------------------------ sum over the cluster, epilogue, store
+  const int feat = 32 * warp + lane;  // warps 0..3
+  const int n = f0 + feat;
+  const bool live = warp < 4 && n < p.N && !abort_flag[0];
+  const long long col = (long long)mat * p.mat_off + n;
+  const float bias = (live && p.bias) ? __ldg(p.bias + n) : 0.0f;
+  if (split == 1) {
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < BN; ++j)
+        if (j < ntok) {
+          const float a = acc[j] + bias;
+          store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + col, p.act ? epi_act(a, p.act) : a);
+        }
+    }
+  } else {
+    // all stages have been consumed: their memory takes the partial sums, [token][feature]
+    float* red = reinterpret_cast<float*>(smem);
+    if (warp < 4) {
+#pragma unroll
+      for (int j = 0; j < BN; ++j)
+        if (j < ntok) red[j * 128 + feat] = acc[j];
+    }
+    __syncthreads();
+    tc::cluster_sync();
+    if (live) {
+      for (int j = rank; j < ntok; j += split) {
+        float a = 0.0f;
+        for (int q = 0; q < split; ++q) {
+          float x;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::mapa(red + j * 128 + feat, q)) : "memory");
+          a += x;
+        }
+        a += bias;
+        store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + col, p.act ? epi_act(a, p.act) : a);
+      }
+    }
+    tc::cluster_sync();  // no CTA leaves while another reads its partial sums
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc::fence_after();
+    tc::tmem_dealloc(tmem, C::kAcc * BN);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// many_kernel
+// ---------------------------------------------------------------------------
+constexpr int kManyStages = 4;
+constexpr uint32_t kManyStage = 3 * kATile;
+constexpr int kManyWarps = 8;                         // scaling warps
+constexpr int kManyThreads = 32 * (kManyWarps + 2);   // + TMA warp, MMA warp
+constexpr int kStageLd = 20;                          // floats per row of the store staging: 16-byte accesses, no bank conflict
+constexpr uint32_t kStaging = 32 * kStageLd * 4;      // per warp
+constexpr uint32_t kManyBars = kManyStages * kManyStage + kManyWarps * kStaging;
+constexpr size_t kManySmem = 1024 + kManyBars + 256;
+
+struct ManyParams {
+  int nkb, N, Nb, n_tiles;            // n_tiles: feature tiles (256 wide, or 128 of gate and up)
+  const float* sw[2];
+  const int32_t* slots;
+  int M;
+  const float* sx;
+  long long lds;
+  void* Y;
+  int ydt, vec;
+  long long ldy;
+  const float* bias;
+  int act;
+  uint8_t* hq;                        // GATED: codes [row][ldh] and scales [n / 128][hs_ld]
+  long long ldh;
+  float* hs;
+  long long hs_ld;
+  uint32_t* status;
+  unsigned long long timeout_ns;
+};
+
+// Barrier of two warps; the second form also tells both whether either of
+// them passed true.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_sync_or(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    many_kernel(const __grid_constant__ CUtensorMap tw0, const __grid_constant__ CUtensorMap tw1,
+                const __grid_constant__ CUtensorMap tx, const ManyParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* staging = reinterpret_cast<float*>(smem + kManyStages * kManyStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kManyBars);
+  uint64_t* empty = full + kManyStages;
+  uint64_t* acc_full = empty + kManyStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;        // [2]
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(acc_empty + 2);
+  uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n_slots = slot_count(p.slots, p.M, 128);
+  const int n_work = n_slots * p.n_tiles;
+  if ((int)blockIdx.x >= n_work) return;
+
+  if (tid == 0) {
+    for (int i = 0; i < kManyStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], kManyWarps);
+    }
+    abort_flag[0] = 0;
+    fence_barrier_init();
+  }
+  if (warp == kManyWarps + 1) tc::tmem_alloc(tmem_slot, 512);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == kManyWarps) {
+    // ------------------------------------------------------------ TMA
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
+        const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
+        const int nt = t / n_slots;
+        const int f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
+        for (int kb = 0; kb < p.nkb; ++kb, ++it) {
+          const int s = it % kManyStages;
+          if (it >= kManyStages && !mbar_wait(&empty[s], ((it / kManyStages) & 1) ^ 1, p.timeout_ns)) {
+            abort_flag[0] = 1;
+            break;
+          }
+          uint8_t* st = smem + s * kManyStage;
+          mbar_expect_tx(&full[s], kManyStage);
+          tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
+          tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
+          tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
+        }
+      }
+      if (abort_flag[0]) {
+        for (uint32_t j = it > kManyStages ? it - kManyStages : 0; j < it; ++j)
+          (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
+        flag(p.status, MTC_STATUS_TIMEOUT);
+      }
+    }
+  } else if (warp == kManyWarps + 1) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(128, 256);
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
+        for (int kb = 0; kb < p.nkb; ++kb, ++it) {
+          const int s = it % kManyStages, b = it & 1;
+          if (!mbar_wait(&full[s], (it / kManyStages) & 1, p.timeout_ns) ||
+              (it >= 2 && !mbar_wait(&acc_empty[b], ((it >> 1) & 1) ^ 1, p.timeout_ns))) {
+            abort_flag[0] = 1;
+            break;
+          }
+          tc::fence_after();
+          const uint32_t a0 = smem_u32(smem + s * kManyStage), b0 = a0 + kATile;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_e4m3_ss(tmem + b * 256, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
+                        j > 0);
+          tc::commit(&empty[s]);
+          tc::commit(&acc_full[b]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ scale and add, then store
+    const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
+    float* stg = staging + warp * (kStaging / 4);
+    uint32_t it = 0;
+    bool stop = false;
+    for (int t = blockIdx.x; t < n_work && !stop; t += gridDim.x) {
+      const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
+      const int nt = t / n_slots;
+      const int row = slot.row0 + 32 * quad + lane;
+      const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
+      const bool row_ok = row < slot.end;
+      const int nb = min(n0 >> 7, p.Nb - 1);
+      const float* swp = p.sw[GATED ? hf : 0] + ((long long)slot.e * p.Nb + nb) * p.nkb;
+      const float* sxp = p.sx + row;
+      auto scale_at = [&](int kb) {
+        return (row_ok && kb < p.nkb) ? sxp[(long long)kb * p.lds] * __ldg(swp + kb) : 0.0f;
+      };
+      float s0 = scale_at(0), s1 = scale_at(1);
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      bool ok = true;
+      for (int kb = 0; kb < p.nkb; ++kb, ++it) {
+        const int b = it & 1;
+        const float sc = s0;
+        s0 = s1;
+        s1 = scale_at(kb + 2);
+        if (!__all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(&acc_full[b], (it >> 1) & 1, p.timeout_ns))) {
+          abort_flag[0] = 1;
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+        uint32_t v[2][16];
+        const uint32_t ta = tmem + b * 256 + 128 * hf + ((uint32_t)(32 * quad) << 16);
+        tmem_ld16(ta, v[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tmem_wait16(v[c & 1]);
+          if (c < 7) {
+            tmem_ld16(ta + 16 * (c + 1), v[(c + 1) & 1]);
+          } else {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) fma2(acc[16 * c + j], acc[16 * c + j + 1], v[c & 1][j], v[c & 1][j + 1], sc);
+        }
+      }
+      if constexpr (GATED) {
+        // warps 4..7 hand their up values, 16 columns at a time, to the gate
+        // warps of the same rows through two of the staging areas
+        float* ex[2] = {staging + quad * (kStaging / 4), staging + (4 + quad) * (kStaging / 4)};
+        if (hf == 1) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float* d = ex[c & 1] + lane * kStageLd;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(d + j) =
+                  make_float4(acc[16 * c + j], acc[16 * c + j + 1], acc[16 * c + j + 2], acc[16 * c + j + 3]);
+            pair_sync(1 + quad);
+          }
+        } else {
+          uint32_t am = 0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            pair_sync(1 + quad);
+            const float* u = ex[c & 1] + lane * kStageLd;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int q = 16 * c + j;
+              acc[q] = n0 + q < p.N ? epi_act(acc[q], p.act) * u[j] : 0.0f;
+              am = max(am, abs_bits(acc[q]));
+            }
+          }
+          if (row_ok && ok) {
+            const GroupScale g = group_scale(am);
+            p.hs[(long long)nt * p.hs_ld + row] = g.scale;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              if (n0 + 16 * c < p.ldh) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int q = 16 * c + 4 * j;
+                  w[j] = g.mul == 0.0f ? 0u
+                                       : codes2(acc[q], acc[q + 1], g.mul) | codes2(acc[q + 2], acc[q + 3], g.mul) << 16;
+                }
+                *reinterpret_cast<uint4*>(p.hq + (long long)row * p.ldh + n0 + 16 * c) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+              }
+          }
+        }
+        // the areas are free for the next tile; both warps of the pair stop at the same one
+        stop = pair_sync_or(1 + quad, !ok);
+      } else if (!ok) {
+        stop = true;
+      } else {
+        // 16 columns at a time through the warp's staging area: rows in, row pieces out
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int nc = n0 + 16 * c;
+          float* d = stg + lane * kStageLd;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            float o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float a = acc[16 * c + j + q];
+              const int n = nc + j + q;
+              if (p.bias) a += n < p.N ? __ldg(p.bias + n) : 0.0f;
+              o[q] = p.act ? epi_act(a, p.act) : a;
+            }
+            *reinterpret_cast<float4*>(d + j) = make_float4(o[0], o[1], o[2], o[3]);
+          }
+          __syncwarp();
+          // lane: 4 columns of row 8 r + lane / 4
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int rr = 8 * r + (lane >> 2), n = nc + 4 * (lane & 3);
+            const long long m = slot.row0 + 32 * quad + rr;
+            if (m >= slot.end) continue;
+            const float4 o = *reinterpret_cast<const float4*>(stg + rr * kStageLd + 4 * (lane & 3));
+            const long long at = m * p.ldy + n;
+            if (p.vec && n + 3 < p.N) {
+              if (p.ydt == MTC_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + at) = o;
+              else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.Y) + at) =
+                       make_uint2(pack2(p.ydt, o.x, o.y), pack2(p.ydt, o.z, o.w));
+            } else {
+              const float e[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (n + q < p.N) store1(p.Y, p.ydt, at + q, e[q]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (warp == kManyWarps + 1) {
+    tc::fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+template <int BN, int SRC>
+int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid_x,
+               int grid_y, cudaStream_t st, const char* who) {
+  auto kernel = few_kernel<BN, SRC>;
+  constexpr size_t smem = FewCfg<BN>::kSmem;
+  MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(grid_x, grid_y, 1);
+  cfg.blockDim = dim3(SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  MTC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw0, tw1, tx, p), who);
+  return MTC_OK;
+}
+
+}  // namespace
+
+namespace {
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(p);
+    return nullptr;
+  }();
+  return fn;
+}
+}  // namespace
+
+// TMA map of rows of codes: boxes of 128 inputs x box_rows in the K-major
+// 128-byte swizzle; inputs past K and rows past `rows` read as zero.
+int encode_codes_map(CUtensorMap* map, const uint8_t* codes, long long ld, long long K, long long rows, int box_rows,
+                     const char* who) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) {
+    set_error("%s: cuTensorMapEncodeTiled unavailable from the driver", who);
+    return MTC_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("%s: cuTensorMapEncodeTiled failed (%d)", who, (int)r);
+    return MTC_ERR_CUDA;
+  }
+  return MTC_OK;
+}
+
+int check_matrix(const mtc_fp8_matrix* w, const char* who) {
+  MTC_REQUIRE(w && w->codes && w->scales, "%s: null matrix", who);
+  MTC_REQUIRE(w->K >= 1 && w->N >= 1 && w->E >= 1, "%s: bad matrix shape %d x (%d, %d)", who, w->E, w->K, w->N);
+  MTC_REQUIRE(w->ldk >= w->K && (w->ldk & 15) == 0, "%s: row stride %lld of the codes is not a multiple of 16 >= K",
+              who, (long long)w->ldk);
+  MTC_REQUIRE((reinterpret_cast<uintptr_t>(w->codes) & 15) == 0, "%s: codes not 16-byte aligned", who);
+  MTC_REQUIRE((long long)w->E * w->N <= 0x7fffff00ll, "%s: more than 2^31 weight rows", who);
+  return MTC_OK;
+}
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return sms;
+}
+
+int launch_product(const Product& a, cudaStream_t st, const char* who) {
+  const mtc_fp8_matrix* w = a.w[0];
+  const int nkb = (w->K + kBlock - 1) / kBlock, Nb = (w->N + kBlock - 1) / kBlock;
+  const int n_mats = a.w[1] ? 2 : 1;
+  const int sms = sm_count();
+  MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
+  if (a.slot_bound <= 0) return MTC_OK;
+  CUtensorMap tw[2], tx;
+  for (int i = 0; i < 2; ++i) {
+    const mtc_fp8_matrix* m = a.w[i] ? a.w[i] : w;
+    const int rc = encode_codes_map(&tw[i], m->codes, m->ldk, m->K, (long long)m->E * m->N, 128, who);
+    if (rc != MTC_OK) return rc;
+  }
+  tx = tw[0];
+  if (a.xq) {
+    const int rc = encode_codes_map(&tx, a.xq, a.ldq, w->K, a.rows, a.tile, who);
+    if (rc != MTC_OK) return rc;
+  }
+  if (a.many) {
+    ManyParams p = {};
+    p.nkb = nkb;
+    p.N = w->N;
+    p.Nb = Nb;
+    p.n_tiles = n_mats == 2 ? Nb : (w->N + 255) / 256;
+    p.sw[0] = w->scales;
+    p.sw[1] = a.w[1] ? a.w[1]->scales : w->scales;
+    p.slots = a.slots;
+    p.M = a.rows;
+    p.sx = a.sx;
+    p.lds = a.lds;
+    p.Y = a.Y;
+    p.ydt = a.ydt;
+    p.ldy = a.ldy;
+    const uintptr_t align = a.ydt == MTC_F32 ? 16 : 8;
+    p.vec = (reinterpret_cast<uintptr_t>(a.Y) & (align - 1)) == 0 && (a.ldy & 3) == 0;
+    p.bias = a.bias;
+    p.act = n_mats == 2 ? a.gate_act : a.act;
+    p.hq = a.hq;
+    p.ldh = a.ldh;
+    p.hs = a.hs;
+    p.hs_ld = a.hs_ld;
+    p.status = a.status;
+    p.timeout_ns = wait_limit_ns();
+    auto kernel = n_mats == 2 ? many_kernel<true> : many_kernel<false>;
+    MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kManySmem), who);
+    const long long work = (long long)a.slot_bound * p.n_tiles;
+    kernel<<<(int)(work < sms ? work : sms), kManyThreads, kManySmem, st>>>(tw[0], tw[1], tx, p);
+    MTC_CHECK_LAUNCH(who);
+    return MTC_OK;
+  }
+  FewParams p = {};
+  p.K = w->K;
+  p.nkb = nkb;
+  p.N = w->N;
+  p.Nb = Nb;
+  p.n_tiles = Nb;
+  p.sw[0] = w->scales;
+  p.sw[1] = a.w[1] ? a.w[1]->scales : w->scales;
+  p.slots = a.slots;
+  p.M = a.rows;
+  p.sx = a.sx;
+  p.lds = a.lds;
+  p.order = a.order;
+  p.kdiv = a.kdiv;
+  p.gate_act = a.gate_act;
+  p.Y = a.Y;
+  p.ydt = a.ydt;
+  p.ldy = a.ldy;
+  p.mat_off = a.mat_off;
+  p.bias = a.bias;
+  p.act = a.act;
+  p.status = a.status;
+  p.timeout_ns = wait_limit_ns();
+  // Split the inputs over a cluster while the CTAs of the expected slots
+  // leave SMs idle (two CTAs are resident per SM) and every CTA keeps at
+  // least two blocks of 128 inputs.
+  const long long tiles = (long long)Nb * n_mats * a.slot_expect;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * sms && nkb >= 4 * split) split *= 2;
+  p.split = split;
+  const int gx = Nb * n_mats * split;
+  MTC_REQUIRE(a.slot_bound <= 65535, "%s: %d token tiles in one launch", who, a.slot_bound);
+  if (a.xq) {
+    switch (a.tile) {
+      case 16: return launch_few<16, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+      case 32: return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+      case 64: return launch_few<64, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+      default: return launch_few<128, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+    }
+  }
+  p.X = a.X;
+  p.xdt = a.xdt;
+  p.ldx = a.ldx;
+  const int per16 = a.gated_src || a.xdt == MTC_F32 ? 4 : 8;
+  p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % per16 == 0 && (!a.gated_src || a.src_off % 4 == 0);
+  if (a.gated_src) {
+    p.mat_off = a.src_off;
+    return launch_few<16, SRC_GATED>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+  }
+  return launch_few<16, SRC_ROWS>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+}
+
+}  // namespace fp8
+}  // namespace mtc

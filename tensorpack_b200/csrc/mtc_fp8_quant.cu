@@ -1,0 +1,290 @@
+// Activations and weights to e4m3 codes, weights back to fp32, and the dense
+// product entry point.
+#include "mtc_fp8.cuh"
+#include "mtc_fp8_internal.h"
+
+namespace mtc {
+namespace fp8 {
+namespace {
+
+struct QuantParams {
+  const void* X;
+  int M, K, Kb, vec;
+  long long ldx, src_off;
+  int gate_act;
+  const int32_t* n_rows;
+  const int32_t* pos;
+  int copies;
+  uint8_t* q;
+  long long ldq;
+  float* s;
+  long long lds;
+};
+
+// One half warp per group of 128 inputs, 8 values per lane.
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
+  const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int rows = p.n_rows ? min(p.M, *p.n_rows) : p.M;
+  const long long groups = (long long)rows * p.Kb;
+  const long long step = (long long)gridDim.x * 16;
+  const long long last = (groups + 15) & ~15ll;  // whole warps take part in the shuffles
+  for (long long g = (long long)blockIdx.x * 16 + half; g < last; g += step) {
+    const bool on = g < groups;
+    const int m = on ? (int)(g / p.Kb) : 0, b = on ? (int)(g - (long long)m * p.Kb) : 0;
+    const int k = b * kBlock + 8 * l, n = on ? p.K - k : 0;
+    float v[8];
+    const T* x = reinterpret_cast<const T*>(p.X) + m * p.ldx + k;
+    load8(x, n, p.vec, v);
+    if constexpr (GATED) {
+      float u[8];
+      load8(x + p.src_off, n, p.vec, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = epi_act(v[i], p.gate_act) * u[i];
+    }
+    const GroupScale gs = group_scale(half_warp_max(amax8(v)));
+    const uint2 c = codes8(v, gs.mul);
+    if (!on) continue;
+    // (k is a multiple of 8 and ldq of 16, so a lane's 8 codes stay inside the row)
+    if (p.pos) {
+      for (int j = 0; j < p.copies; ++j) {
+        const int r = p.pos[(long long)m * p.copies + j];
+        if (r < 0) continue;
+        if (k < p.ldq) *reinterpret_cast<uint2*>(p.q + (long long)r * p.ldq + k) = c;
+        if (l == 0) p.s[(long long)b * p.lds + r] = gs.scale;
+      }
+    } else {
+      if (k < p.ldq) *reinterpret_cast<uint2*>(p.q + (long long)m * p.ldq + k) = c;
+      if (l == 0) p.s[(long long)b * p.lds + m] = gs.scale;
+    }
+  }
+}
+
+// One 128 x 128 block of W (K x N fp32, row-major) to codes (N rows of K) and its scale.
+__global__ void __launch_bounds__(256) pack_kernel(const float* __restrict__ W, int K, int N, long long ldw,
+                                                   uint8_t* __restrict__ codes, long long ldk,
+                                                   float* __restrict__ scales, int Kb) {
+  __shared__ uint32_t red[8];
+  __shared__ uint8_t tile[128][132];
+  const int k0 = blockIdx.x * 128, n0 = blockIdx.y * 128;
+  const int tn = threadIdx.x & 127, tk = threadIdx.x >> 7;
+  uint32_t m = 0;
+  for (int k = tk; k < 128; k += 2)
+    if (k0 + k < K && n0 + tn < N) m = max(m, abs_bits(W[(long long)(k0 + k) * ldw + n0 + tn]));
+  for (int d = 16; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+  const GroupScale g = group_scale(m);
+  if (threadIdx.x == 0) scales[(long long)blockIdx.y * Kb + blockIdx.x] = g.scale;
+  for (int k = tk; k < 128; k += 2) {
+    float v = 0.0f;
+    if (k0 + k < K && n0 + tn < N) v = W[(long long)(k0 + k) * ldw + n0 + tn];
+    tile[tn][k] = g.mul == 0.0f ? 0 : (uint8_t)(codes2(v, 0.0f, g.mul) & 0xffu);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+    const int n = i >> 7, k = i & 127;
+    if (n0 + n < N && k0 + k < ldk) codes[(long long)(n0 + n) * ldk + k0 + k] = tile[n][k];
+  }
+}
+
+// out[k][n] = code * scale, fp32 (one rounding).
+__global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__ codes, long long ldk,
+                                                     const float* __restrict__ scales, int K, int N, int Kb,
+                                                     float* __restrict__ out, long long ldo) {
+  __shared__ uint8_t tile[128][132];
+  const int k0 = blockIdx.x * 128, n0 = blockIdx.y * 128;
+  for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+    const int n = i >> 7, k = i & 127;
+    tile[n][k] = (n0 + n < N && k0 + k < K) ? codes[(long long)(n0 + n) * ldk + k0 + k] : 0;
+  }
+  __syncthreads();
+  const float s = scales[(long long)blockIdx.y * Kb + blockIdx.x];
+  for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+    const int k = i >> 7, n = i & 127;
+    if (n0 + n < N && k0 + k < K) {
+      __nv_fp8_e4m3 c;
+      c.__x = tile[n][k];
+      out[(long long)(k0 + k) * ldo + n0 + n] = __fmul_rn((float)c, s);
+    }
+  }
+}
+
+}  // namespace
+
+int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
+  if (a.M == 0) return MTC_OK;
+  QuantParams p = {};
+  p.X = a.X;
+  p.M = a.M;
+  p.K = a.K;
+  p.Kb = (a.K + kBlock - 1) / kBlock;
+  p.ldx = a.ldx;
+  p.src_off = a.src_off;
+  p.gate_act = a.gate_act;
+  p.n_rows = a.n_rows;
+  p.pos = a.pos;
+  p.copies = a.copies;
+  p.q = a.q;
+  p.ldq = a.ldq;
+  p.s = a.s;
+  p.lds = a.lds;
+  const int per16 = a.dt == MTC_F32 ? 4 : 8;
+  p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % per16 == 0 && (!a.gated || a.src_off % per16 == 0);
+  const long long blocks = ((long long)a.M * p.Kb + 15) / 16;
+  const int sms = sm_count();
+  MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
+  const int grid = (int)(blocks < 8ll * sms ? blocks : 8ll * sms);
+  if (a.gated) quantize_kernel<float, true><<<grid, 256, 0, st>>>(p);
+  else if (a.dt == MTC_F32) quantize_kernel<float, false><<<grid, 256, 0, st>>>(p);
+  else if (a.dt == MTC_BF16) quantize_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(p);
+  else quantize_kernel<__half, false><<<grid, 256, 0, st>>>(p);
+  MTC_CHECK_LAUNCH(who);
+  return MTC_OK;
+}
+
+namespace {
+bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16; }
+
+// Rows of one token tile of a dense product: the kernel for few rows up to
+// 128 of them, in tiles that waste at most half of the MMA; above, the
+// 128 x 256 tiles, once there are enough of them to occupy the SMs.
+struct DensePlan {
+  int tile;
+  bool many, raw;
+  long long ldq, lds;
+  size_t q_bytes, bytes;
+};
+DensePlan dense_plan(int M, int K, int N, int sms) {
+  DensePlan d;
+  const long long many_tiles = (long long)((M + 127) / 128) * ((N + 255) / 256);
+  d.many = M > 128 && many_tiles >= sms;
+  d.tile = d.many || M > 64 ? 128 : M > 32 ? 64 : M > 16 ? 32 : 16;
+  d.raw = M <= 16;
+  d.ldq = (K + 15) & ~15ll;
+  d.lds = (M + 3) & ~3ll;
+  d.q_bytes = d.raw ? 0 : (((size_t)M * d.ldq + 255) & ~(size_t)255);
+  d.bytes = d.raw ? 0 : d.q_bytes + (size_t)((K + 127) / 128) * d.lds * 4;
+  return d;
+}
+}  // namespace
+
+}  // namespace fp8
+}  // namespace mtc
+
+using namespace mtc;
+using namespace mtc::fp8;
+
+extern "C" int mtc_fp8_pack(const float* W, int32_t K, int32_t N, int64_t ldw, uint8_t* codes, int64_t ldk,
+                            float* scales, void* stream) {
+  clear_error();
+  MTC_REQUIRE(W && codes && scales, "mtc_fp8_pack: null pointer");
+  MTC_REQUIRE(K >= 1 && N >= 1 && ldw >= N && ldk >= K && (ldk & 15) == 0, "mtc_fp8_pack: bad shape or strides");
+  const dim3 grid((K + 127) / 128, (N + 127) / 128);
+  MTC_REQUIRE(grid.y <= 65535, "mtc_fp8_pack: N=%d too large", N);
+  pack_kernel<<<grid, 256, 0, as_stream(stream)>>>(W, K, N, ldw, codes, ldk, scales, grid.x);
+  MTC_CHECK_LAUNCH("mtc_fp8_pack");
+  return MTC_OK;
+}
+
+extern "C" int mtc_fp8_unpack(const mtc_fp8_matrix* w, int32_t e, float* out, int64_t ldo, void* stream) {
+  clear_error();
+  const int rc = check_matrix(w, "mtc_fp8_unpack");
+  if (rc != MTC_OK) return rc;
+  MTC_REQUIRE(out && ldo >= w->N && e >= 0 && e < w->E, "mtc_fp8_unpack: bad argument");
+  const dim3 grid((w->K + 127) / 128, (w->N + 127) / 128);
+  MTC_REQUIRE(grid.y <= 65535, "mtc_fp8_unpack: N=%d too large", w->N);
+  unpack_kernel<<<grid, 256, 0, as_stream(stream)>>>(w->codes + (long long)e * w->N * w->ldk, w->ldk,
+                                                     w->scales + (long long)e * grid.x * grid.y, w->K, w->N, grid.x,
+                                                     out, ldo);
+  MTC_CHECK_LAUNCH("mtc_fp8_unpack");
+  return MTC_OK;
+}
+
+extern "C" int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_t K, int64_t ldx, uint8_t* codes,
+                                int64_t ldq, float* scales, int64_t lds, void* stream) {
+  clear_error();
+  MTC_REQUIRE(X && codes && scales, "mtc_fp8_quantize: null pointer");
+  MTC_REQUIRE(dtype_ok(x_type), "mtc_fp8_quantize: unknown element type %d", x_type);
+  MTC_REQUIRE(M >= 0 && K >= 1 && ldx >= K, "mtc_fp8_quantize: bad shape (M=%d, K=%d, ldx=%lld)", M, K,
+              (long long)ldx);
+  MTC_REQUIRE(ldq >= K && (ldq & 15) == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && lds >= M,
+              "mtc_fp8_quantize: codes need rows of a multiple of 16 bytes >= K and 16-byte alignment");
+  QuantRows a;
+  a.X = X;
+  a.dt = x_type;
+  a.M = M;
+  a.K = K;
+  a.ldx = ldx;
+  a.q = codes;
+  a.ldq = ldq;
+  a.s = scales;
+  a.lds = lds;
+  return launch_quantize(a, as_stream(stream), "mtc_fp8_quantize");
+}
+
+extern "C" size_t mtc_fp8_gemm_workspace_bytes(const mtc_fp8_matrix* w, int32_t M) {
+  if (!w || M < 1 || w->K < 1) return 0;
+  const int sms = sm_count();
+  return dense_plan(M, w->K, w->N, sms > 0 ? sms : 1).bytes;
+}
+
+extern "C" int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type, int32_t M, int64_t ldx, void* Y,
+                            int32_t y_type, int64_t ldy, void* ws, size_t ws_bytes, uint32_t* status,
+                            const mtc_epilogue* ep, void* stream) {
+  clear_error();
+  int rc = check_matrix(w, "mtc_fp8_gemm");
+  if (rc != MTC_OK) return rc;
+  MTC_REQUIRE(w->E == 1, "mtc_fp8_gemm: %d stacked matrices", w->E);
+  MTC_REQUIRE(X && Y, "mtc_fp8_gemm: null pointer");
+  MTC_REQUIRE(dtype_ok(x_type) && dtype_ok(y_type), "mtc_fp8_gemm: unknown element type");
+  MTC_REQUIRE(M >= 1 && ldx >= w->K && ldy >= w->N, "mtc_fp8_gemm: bad shape (M=%d, ldx=%lld, ldy=%lld)", M,
+              (long long)ldx, (long long)ldy);
+  EpiArg epa;
+  rc = read_epilogue(ep, &epa, "mtc_fp8_gemm");
+  if (rc != MTC_OK) return rc;
+  const int sms = sm_count();
+  MTC_REQUIRE(sms > 0, "mtc_fp8_gemm: no CUDA device");
+  const DensePlan d = dense_plan(M, w->K, w->N, sms);
+  if (ws_bytes < d.bytes || (d.bytes && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255)))) {
+    set_error("mtc_fp8_gemm: workspace of %zu bytes (256-byte aligned) needed, %zu given", d.bytes, ws_bytes);
+    return MTC_ERR_WORKSPACE;
+  }
+  const cudaStream_t st = as_stream(stream);
+  Product a;
+  a.w[0] = w;
+  a.rows = M;
+  a.tile = d.tile;
+  a.many = d.many;
+  a.slot_bound = a.slot_expect = (M + d.tile - 1) / d.tile;
+  a.Y = Y;
+  a.ydt = y_type;
+  a.ldy = ldy;
+  a.bias = epa.bias;
+  a.act = epa.act;
+  a.status = status;
+  if (d.raw) {
+    a.X = X;
+    a.xdt = x_type;
+    a.ldx = ldx;
+  } else {
+    QuantRows q;
+    q.X = X;
+    q.dt = x_type;
+    q.M = M;
+    q.K = w->K;
+    q.ldx = ldx;
+    q.q = reinterpret_cast<uint8_t*>(ws);
+    q.ldq = d.ldq;
+    q.s = reinterpret_cast<float*>(q.q + d.q_bytes);
+    q.lds = d.lds;
+    rc = launch_quantize(q, st, "mtc_fp8_gemm");
+    if (rc != MTC_OK) return rc;
+    a.xq = q.q;
+    a.ldq = q.ldq;
+    a.sx = q.s;
+    a.lds = q.lds;
+  }
+  return launch_product(a, st, "mtc_fp8_gemm");
+}

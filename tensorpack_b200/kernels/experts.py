@@ -1,0 +1,118 @@
+"""Mixture-of-experts operators: routing and the experts' gated feed-forward.
+
+``route_experts`` turns router logits into the chosen experts and their
+weights; ``experts_forward`` runs the chosen experts, whose matrices are
+``FP8Experts`` stacks, on every token:
+
+    y_t = sum_j weights[t, j] * (act(x_t @ gate_e) * (x_t @ up_e)) @ down_e,   e = ids[t, j]
+
+Both enqueue their kernels on the current stream and do not synchronise.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import _lib
+from .fp8 import _TYPES, FP8Experts, _ld, _on, _output, _rows, _stream
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 32
+MAX_GROUPS = 32
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias=None, n_groups: int = 1,
+                  top_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """(ids (T, top_k) int32, weights (T, top_k) float32) from router logits (T, E).
+
+    Scores are the softmax over the experts or the sigmoid of the logits.
+    The experts are chosen by score + ``bias`` (E finite floats, to balance
+    their load), compared in 64 bits, best first, ties to the lowest index.
+    With ``n_groups`` > 1 only the experts of the ``top_groups`` groups (equal
+    consecutive parts of the E experts) with the largest sum of their two best
+    choices compete.  The weights are the scores without the bias, divided by
+    their sum if ``renormalize``, times ``scale``.
+
+    A logit of -inf or NaN masks its expert: score 0, chosen only when no
+    other is left; a row of masked experts gets weights 0.  +inf counts as the
+    largest finite number."""
+    logits = _rows(logits, "route_experts")
+    T, E = logits.shape
+    if score not in _lib.SCORES:
+        raise ValueError(f"route_experts: unknown score {score!r} (softmax or sigmoid)")
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"route_experts: {E} experts (1..{MAX_EXPERTS})")
+    if not 1 <= n_groups <= MAX_GROUPS or E % n_groups or not 1 <= top_groups <= n_groups:
+        raise ValueError(f"route_experts: {E} experts in {n_groups} groups, {top_groups} of them kept")
+    if not 1 <= top_k <= min(MAX_TOP_K, top_groups * (E // n_groups)):
+        raise ValueError(f"route_experts: top_k={top_k} outside 1..{min(MAX_TOP_K, top_groups * (E // n_groups))}")
+    dev = logits.device
+    if bias is not None:
+        bias = torch.as_tensor(bias, dtype=torch.float32, device=dev).reshape(-1).contiguous()
+        if bias.numel() != E:
+            raise ValueError(f"route_experts: bias has {bias.numel()} values, there are {E} experts")
+    ids = torch.empty(T, top_k, dtype=torch.int32, device=dev)
+    weights = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    if T:
+        with _on(dev):
+            _lib.check(_lib.load().mtc_route_experts(
+                logits.data_ptr(), _TYPES[logits.dtype], T, E, _ld(logits), top_k, _lib.SCORES[score],
+                None if bias is None else bias.data_ptr(), n_groups, top_groups, int(bool(renormalize)), scale,
+                ids.data_ptr(), weights.data_ptr(), _stream(dev)), "route experts")
+    return ids, weights
+
+
+def experts_forward(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: FP8Experts, up: FP8Experts,
+                    down: FP8Experts, *, activation: Optional[str] = "silu", Y=None, out_dtype=None) -> torch.Tensor:
+    """The weighted sum of the chosen experts' gated feed-forward for every token.
+
+    X: (T, D) CUDA tensor (fp32, bf16, fp16); ids (T, k) integers, weights
+    (T, k) floats, as ``route_experts`` gives them; gate and up (E, D, I),
+    down (E, I, D).  An id outside 0..E-1 is no expert and adds nothing (a
+    padded token, or an expert of another rank).  The activations and the
+    gated values act(gate) * up (fp32 until then) are quantized as in
+    ``fp8_quantize``; an expert's output is rounded to the result's type, the
+    weighted sum is fp32 in the order of j.  The result is fp32, or
+    ``out_dtype``; ``Y`` takes it if given (it must not overlap an input)."""
+    X = _rows(X, "experts_forward")
+    for m in (gate, up, down):
+        if not isinstance(m, FP8Experts) or len(m.shape) != 3:
+            raise TypeError("experts_forward: gate, up and down must be FP8Experts")
+    T, D = X.shape
+    E, K, I = gate.shape
+    dev = X.device
+    assert D == K, f"Shape mismatch: {tuple(X.shape)} vs {gate.shape}"
+    if up.shape != (E, D, I) or down.shape != (E, I, D):
+        raise ValueError(f"experts_forward: gate {gate.shape}, up {up.shape} and down {down.shape} do not fit")
+    if E > MAX_EXPERTS:
+        raise ValueError(f"experts_forward: {E} experts, at most {MAX_EXPERTS}")
+    if any(m.device != dev for m in (gate, up, down)) or ids.device != dev or weights.device != dev:
+        raise ValueError(f"experts_forward: all operands must be on {dev}")
+    if ids.dim() != 2 or ids.shape[0] != T or ids.shape != weights.shape or not 1 <= ids.shape[1] <= MAX_TOP_K:
+        raise ValueError(f"experts_forward: ids {tuple(ids.shape)} and weights {tuple(weights.shape)} for {T} tokens "
+                         f"(1..{MAX_TOP_K} experts each)")
+    if ids.dtype != torch.int32:
+        if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+            raise ValueError(f"experts_forward: ids of type {ids.dtype}")
+        # (an id that does not fit 32 bits is no expert either)
+        ids = torch.where((ids >= 0) & (ids < E), ids, torch.full_like(ids, -1) if ids.dtype.is_signed else E).to(
+            torch.int32)
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r} (one of relu, silu, gelu_tanh)")
+    ids, weights = ids.contiguous(), weights.to(torch.float32).contiguous()
+    k = ids.shape[1]
+    Y = _output(Y, (T, D), out_dtype, dev, (X, ids, weights), "experts_forward")
+    if T:
+        lib = _lib.load()
+        with _on(dev):
+            need = lib.mtc_experts_workspace_bytes(gate._ref, T, k, _TYPES[Y.dtype])
+            if not need:
+                raise ValueError(f"experts_forward: too many rows ({T} x {k})")
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            _lib.check(lib.mtc_experts_forward(
+                gate._ref, up._ref, down._ref, X.data_ptr(), _TYPES[X.dtype], T, _ld(X), ids.data_ptr(),
+                weights.data_ptr(), k, _lib.ACTIVATIONS[activation], Y.data_ptr(), _TYPES[Y.dtype],
+                Y.stride(0) if T > 1 else D, ws.data_ptr(), need, gate.status.data_ptr(), _stream(dev)), "experts")
+    return Y

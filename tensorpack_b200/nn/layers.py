@@ -16,6 +16,8 @@ import numpy as np
 import torch
 
 from ..core.arena import MemoryArena
+from ..kernels.experts import experts_forward, route_experts
+from ..kernels.fp8 import FP8Experts, FP8Matrix, fp8_gemm
 from ..kernels.gemm import MTCMatrix, gemm_fused, mtc_gemm
 
 _NP_ACT = {
@@ -111,3 +113,73 @@ def fold_layers(a: LinearMTCAdaptive, b: LinearMTCAdaptive):
     pc = a.W_mtc.col_perm
     bias_a = a.b if pc is None else a.b[np.asarray(pc)]
     return (LinearMTCAdaptive.from_mtc(wa, bias_a, a.activation), LinearMTCAdaptive.from_mtc(wb, b.b, b.activation))
+
+
+class LinearFP8(torch.nn.Module):
+    """Linear layer on an ``FP8Matrix`` (e4m3 weights, one scale per 128 x 128
+    block): ``act(X @ W + b)`` with the activations quantized on the way.  The
+    8-bit counterpart of ``LinearMTCAdaptive``, used the same way: numpy in,
+    numpy out, or a CUDA tensor in and out (fp32 unless ``out_dtype`` says
+    otherwise)."""
+
+    def __init__(self, W_fp8: FP8Matrix, bias: Optional[np.ndarray] = None, activation: Optional[str] = None,
+                 out_dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        if activation not in _NP_ACT:
+            raise ValueError(f"unknown activation {activation!r}")
+        self.in_features, self.out_features = W_fp8.shape
+        self.W_fp8 = W_fp8
+        self.activation = activation
+        self.out_dtype = out_dtype
+        self.b = np.zeros(self.out_features, dtype=np.float32) if bias is None else np.asarray(bias, np.float32)
+        if self.b.shape != (self.out_features,):
+            raise ValueError(f"bias has shape {self.b.shape}, the layer {self.out_features} outputs")
+        self._bias_dev = None if bias is None else torch.from_numpy(self.b).to(W_fp8.device)
+
+    @classmethod
+    def from_mtc(cls, layer: LinearMTCAdaptive, device=None) -> "LinearFP8":
+        """The 8-bit form of a packed layer: its weights requantized, its bias and activation kept."""
+        return cls(FP8Matrix.from_mtc(layer.W_mtc, device), layer.b, layer.activation)
+
+    @property
+    def weight_bytes(self) -> int:
+        return self.W_fp8.weight_bytes + self.b.nbytes
+
+    def forward(self, X):
+        out = None if isinstance(X, np.ndarray) else self.out_dtype
+        return fp8_gemm(X, self.W_fp8, self._bias_dev, self.activation, out_dtype=out)
+
+
+class ExpertsFP8(torch.nn.Module):
+    """Mixture-of-experts feed-forward: ``router`` (any layer of this module,
+    or a callable) gives logits (T, E) for tokens (T, D), ``route_experts``
+    chooses ``top_k`` of the experts, and ``experts_forward`` runs their gated
+    feed-forward on 8-bit weights (gate and up (E, D, I), down (E, I, D))."""
+
+    def __init__(self, router, gate: FP8Experts, up: FP8Experts, down: FP8Experts, top_k: int, *,
+                 score: str = "softmax", bias=None, n_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+                 scale: float = 1.0, activation: Optional[str] = "silu"):
+        super().__init__()
+        if up.shape != gate.shape or down.shape != (gate.shape[0], gate.shape[2], gate.shape[1]):
+            raise ValueError(f"gate {gate.shape}, up {up.shape} and down {down.shape} do not fit")
+        if activation not in _NP_ACT:
+            raise ValueError(f"unknown activation {activation!r}")
+        self.router, self.gate, self.up, self.down = router, gate, up, down
+        self.top_k, self.activation = top_k, activation
+        self.routing = dict(score=score, n_groups=n_groups, top_groups=top_groups, renormalize=renormalize, scale=scale)
+        self.bias = None if bias is None else torch.as_tensor(bias, dtype=torch.float32, device=gate.device)
+
+    @property
+    def weight_bytes(self) -> int:
+        return self.gate.weight_bytes + self.up.weight_bytes + self.down.weight_bytes
+
+    def forward(self, X, out_dtype=None):
+        if not isinstance(X, torch.Tensor) or X.device.type != "cuda":
+            raise ValueError("ExpertsFP8: activations must be a CUDA tensor (no CPU path)")
+        logits = self.router(X)
+        if logits.shape != (X.shape[0], self.gate.shape[0]):
+            raise ValueError(f"the router gave logits {tuple(logits.shape)} for {X.shape[0]} tokens and "
+                             f"{self.gate.shape[0]} experts")
+        ids, weights = route_experts(logits, self.top_k, bias=self.bias, **self.routing)
+        return experts_forward(X, ids, weights, self.gate, self.up, self.down, activation=self.activation,
+                               out_dtype=out_dtype)
