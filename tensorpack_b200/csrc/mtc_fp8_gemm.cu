@@ -184,14 +184,15 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     constexpr int kCols = (BN + 31) / 32;
 #pragma unroll
     for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
-    float sn[kCols];  // the next block's scales, columns lane, lane + 32, ...
+    // The next block's scales, columns lane, lane + 32, ...; multiplied where
+    // they are used, so that nothing waits for the loads before that.
+    float sn[kCols], wn;
     auto load_scales = [&](int i) {
-      const float w = __ldg(swp + i);
+      wn = __ldg(swp + i);
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         const int m = 32 * c + lane;
-        if constexpr (SRC == SRC_CODES) sn[c] = m < ntok ? p.sx[(long long)(kb0 + i) * p.lds + slot.row0 + m] * w : 0.0f;
-        else sn[c] = w;
+        if constexpr (SRC == SRC_CODES) sn[c] = m < ntok ? p.sx[(long long)(kb0 + i) * p.lds + slot.row0 + m] : 0.0f;
       }
     };
     load_scales(0);
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
       const int b = i % C::kAcc;
       float sc[kCols];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) sc[c] = sn[c];
+      for (int c = 0; c < kCols; ++c) sc[c] = SRC == SRC_CODES ? sn[c] * wn : wn;
       if (i + 1 < n_it) load_scales(i + 1);
       if (!__all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(&acc_full[b], (i / C::kAcc) & 1, p.timeout_ns))) {
         abort_flag[0] = 1;
@@ -284,39 +285,38 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
   const bool live = warp < 4 && n < p.N && !abort_flag[0];
   const long long col = (long long)mat * p.mat_off + n;
   const float bias = (live && p.bias) ? __ldg(p.bias + n) : 0.0f;
-  if (split == 1) {
-    if (live) {
+  // All stages have been consumed: their memory takes the sums, [token]
+  // [feature].  The loops over tokens stay loops (the epilogue's code once,
+  // not once per token: unrolled, its instruction fetches took longer than
+  // the product).
+  float* red = reinterpret_cast<float*>(smem);
+  if (warp < 4) {
 #pragma unroll
-      for (int j = 0; j < BN; ++j)
-        if (j < ntok) {
-          const float a = acc[j] + bias;
-          store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + col, p.act ? epi_act(a, p.act) : a);
-        }
-    }
-  } else {
-    // all stages have been consumed: their memory takes the partial sums, [token][feature]
-    float* red = reinterpret_cast<float*>(smem);
-    if (warp < 4) {
-#pragma unroll
-      for (int j = 0; j < BN; ++j)
-        if (j < ntok) red[j * 128 + feat] = acc[j];
-    }
+    for (int j = 0; j < BN; ++j)
+      if (j < ntok) red[j * 128 + feat] = acc[j];
+  }
+  if (split > 1) {
     __syncthreads();
     tc::cluster_sync();
-    if (live) {
-      for (int j = rank; j < ntok; j += split) {
-        float a = 0.0f;
+  }
+  if (live) {
+#pragma unroll 1
+    for (int j = rank; j < ntok; j += split) {
+      float a = 0.0f;
+      if (split == 1) {
+        a = red[j * 128 + feat];
+      } else {
         for (int q = 0; q < split; ++q) {
           float x;
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::mapa(red + j * 128 + feat, q)) : "memory");
           a += x;
         }
-        a += bias;
-        store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + col, p.act ? epi_act(a, p.act) : a);
       }
+      a += bias;
+      store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + col, p.act ? epi_act(a, p.act) : a);
     }
-    tc::cluster_sync();  // no CTA leaves while another reads its partial sums
   }
+  if (split > 1) tc::cluster_sync();  // no CTA leaves while another reads its partial sums
   tc::fence_before();
   __syncthreads();
   if (warp == 5) {
@@ -371,6 +371,21 @@ __device__ __forceinline__ bool pair_sync_or(int id, bool x) {
       : "r"(id), "r"((uint32_t)x)
       : "memory");
   return r != 0;
+}
+
+// 16 accumulators of chunk c (0..7): a uniform branch to the one copy of the
+// moves, so that loops over chunks can stay loops and hold their body once.
+template <bool TO_ACC>
+__device__ __forceinline__ void move_chunk(int c, float (&acc)[128], float (&t)[16]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (c == q) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (TO_ACC) acc[16 * q + j] = t[j];
+        else t[j] = acc[16 * q + j];
+      }
+    }
 }
 
 template <bool GATED>
@@ -476,19 +491,22 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int nb = min(n0 >> 7, p.Nb - 1);
       const float* swp = p.sw[GATED ? hf : 0] + ((long long)slot.e * p.Nb + nb) * p.nkb;
       const float* sxp = p.sx + row;
-      auto scale_at = [&](int kb) {
-        return (row_ok && kb < p.nkb) ? sxp[(long long)kb * p.lds] * __ldg(swp + kb) : 0.0f;
-      };
-      float s0 = scale_at(0), s1 = scale_at(1);
+      // scales of the blocks kb and kb + 1, multiplied where they are used so
+      // that nothing waits for the loads before that
+      auto sx_at = [&](int kb) { return (row_ok && kb < p.nkb) ? sxp[(long long)kb * p.lds] : 0.0f; };
+      auto sw_at = [&](int kb) { return kb < p.nkb ? __ldg(swp + kb) : 0.0f; };
+      float x0 = sx_at(0), x1 = sx_at(1), w0 = sw_at(0), w1 = sw_at(1);
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
       bool ok = true;
       for (int kb = 0; kb < p.nkb; ++kb, ++it) {
         const int b = it & 1;
-        const float sc = s0;
-        s0 = s1;
-        s1 = scale_at(kb + 2);
+        const float sc = x0 * w0;
+        x0 = x1;
+        w0 = w1;
+        x1 = sx_at(kb + 2);
+        w1 = sw_at(kb + 2);
         if (!__all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(&acc_full[b], (it >> 1) & 1, p.timeout_ns))) {
           abort_flag[0] = 1;
           ok = false;
@@ -528,16 +546,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         } else {
           uint32_t am = 0;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 8; ++c) {
             pair_sync(1 + quad);
             const float* u = ex[c & 1] + lane * kStageLd;
+            float g[16];
+            move_chunk<false>(c, acc, g);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int q = 16 * c + j;
-              acc[q] = n0 + q < p.N ? epi_act(acc[q], p.act) * u[j] : 0.0f;
-              am = max(am, abs_bits(acc[q]));
+            for (int j = 0; j < 16; j += 4) {
+              const float4 u4 = *reinterpret_cast<const float4*>(u + j);
+              const float uu[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                g[j + q] = n0 + 16 * c + j + q < p.N ? epi_act(g[j + q], p.act) * uu[q] : 0.0f;
+                am = max(am, abs_bits(g[j + q]));
+              }
             }
+            move_chunk<true>(c, acc, g);
           }
           if (row_ok && ok) {
             const GroupScale g = group_scale(am);
@@ -562,41 +587,44 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       } else if (!ok) {
         stop = true;
       } else {
-        // 16 columns at a time through the warp's staging area: rows in, row pieces out
-#pragma unroll
+        // 16 columns at a time through the warp's staging area: rows in, row
+        // pieces out (a loop, so that the epilogue's code stands once)
+#pragma unroll 1
         for (int c = 0; c < 8; ++c) {
           const int nc = n0 + 16 * c;
           float* d = stg + lane * kStageLd;
+          float t16[16];
+          move_chunk<false>(c, acc, t16);
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            float o[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float a = acc[16 * c + j + q];
-              const int n = nc + j + q;
-              if (p.bias) a += n < p.N ? __ldg(p.bias + n) : 0.0f;
-              o[q] = p.act ? epi_act(a, p.act) : a;
-            }
-            *reinterpret_cast<float4*>(d + j) = make_float4(o[0], o[1], o[2], o[3]);
-          }
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<float4*>(d + j) = make_float4(t16[j], t16[j + 1], t16[j + 2], t16[j + 3]);
           __syncwarp();
           // lane: 4 columns of row 8 r + lane / 4
-#pragma unroll
+#pragma unroll 1
           for (int r = 0; r < 4; ++r) {
             const int rr = 8 * r + (lane >> 2), n = nc + 4 * (lane & 3);
             const long long m = slot.row0 + 32 * quad + rr;
             if (m >= slot.end) continue;
-            const float4 o = *reinterpret_cast<const float4*>(stg + rr * kStageLd + 4 * (lane & 3));
+            const float4 o4 = *reinterpret_cast<const float4*>(stg + rr * kStageLd + 4 * (lane & 3));
+            float o[4] = {o4.x, o4.y, o4.z, o4.w};
+            if (p.bias || p.act) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if (p.bias && n + q < p.N) o[q] += __ldg(p.bias + n + q);
+                if (p.act) o[q] = epi_act(o[q], p.act);
+              }
+            }
             const long long at = m * p.ldy + n;
             if (p.vec && n + 3 < p.N) {
-              if (p.ydt == MTC_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + at) = o;
-              else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.Y) + at) =
-                       make_uint2(pack2(p.ydt, o.x, o.y), pack2(p.ydt, o.z, o.w));
+              if (p.ydt == MTC_F32)
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + at) = make_float4(o[0], o[1], o[2], o[3]);
+              else
+                *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.Y) + at) =
+                    make_uint2(pack2(p.ydt, o[0], o[1]), pack2(p.ydt, o[2], o[3]));
             } else {
-              const float e[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
               for (int q = 0; q < 4; ++q)
-                if (n + q < p.N) store1(p.Y, p.ydt, at + q, e[q]);
+                if (n + q < p.N) store1(p.Y, p.ydt, at + q, o[q]);
             }
           }
           __syncwarp();
