@@ -330,12 +330,16 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
 // ---------------------------------------------------------------------------
 constexpr int kManyStages = 4;
 constexpr uint32_t kManyStage = 3 * kATile;
-constexpr int kManyWarps = 8;                         // scaling warps
-constexpr int kManyThreads = 32 * (kManyWarps + 2);   // + TMA warp, MMA warp
-constexpr int kStageLd = 20;                          // floats per row of the store staging: 16-byte accesses, no bank conflict
-constexpr uint32_t kStaging = 32 * kStageLd * 4;      // per warp
-constexpr uint32_t kManyBars = kManyStages * kManyStage + kManyWarps * kStaging;
+constexpr int kManyWarps = 16;                        // scaling warps: 4 column quarters x 4 lane quadrants
+constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup with the TMA and the MMA warp
+constexpr int kStageLd = 12;                          // words per row of the staging (8 used): 16-byte accesses, no bank conflict
+constexpr int kStaging = 32 * kStageLd;               // words per warp
+constexpr uint32_t kManyBars = kManyStages * kManyStage + kManyWarps * kStaging * 4 + 2 * 128 * 4;
 constexpr size_t kManySmem = 1024 + kManyBars + 256;
+// Registers: 640 threads are launched with 96 each; the scaling warps (64
+// fp32 sums and 32 loaded values a thread) take what the last warpgroup gives
+// back: 4 x 128 x 112 + 128 x 32 = 640 x 96.
+constexpr int kScaleRegs = 112, kIssueRegs = 32;
 
 struct ManyParams {
   int nkb, N, Nb, n_tiles;            // n_tiles: feature tiles (256 wide, or 128 of gate and up)
@@ -357,15 +361,15 @@ struct ManyParams {
   unsigned long long timeout_ns;
 };
 
-// Barrier of two warps; the second form also tells both whether either of
-// them passed true.
+// Barriers of the warps that share rows: two of them (64 threads), or all
+// four column quarters, who learn whether any of them passed true.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool pair_sync_or(int id, bool x) {
+__device__ __forceinline__ bool quad_sync_or(int id, bool x) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %2, 0;\n\t"
-      "bar.red.or.pred q, %1, 64, p;\n\t"
+      "bar.red.or.pred q, %1, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"(id), "r"((uint32_t)x)
@@ -373,17 +377,17 @@ __device__ __forceinline__ bool pair_sync_or(int id, bool x) {
   return r != 0;
 }
 
-// 16 accumulators of chunk c (0..7): a uniform branch to the one copy of the
+// 8 accumulators of chunk c (0..7): a uniform branch to the one copy of the
 // moves, so that loops over chunks can stay loops and hold their body once.
 template <bool TO_ACC>
-__device__ __forceinline__ void move_chunk(int c, float (&acc)[128], float (&t)[16]) {
+__device__ __forceinline__ void move_chunk(int c, f32x2 (&acc)[32], float (&t)[8]) {
 #pragma unroll
   for (int q = 0; q < 8; ++q)
     if (c == q) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (TO_ACC) acc[16 * q + j] = t[j];
-        else t[j] = acc[16 * q + j];
+      for (int j = 0; j < 4; ++j) {
+        if (TO_ACC) acc[4 * q + j] = pair(t[2 * j], t[2 * j + 1]);
+        else unpair(acc[4 * q + j], t[2 * j], t[2 * j + 1]);
       }
     }
 }
@@ -395,6 +399,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* staging = reinterpret_cast<float*>(smem + kManyStages * kManyStage);
+  uint32_t* row_max = reinterpret_cast<uint32_t*>(staging + kManyWarps * kStaging);  // [2][128]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kManyBars);
   uint64_t* empty = full + kManyStages;
   uint64_t* acc_full = empty + kManyStages;  // [2]
@@ -425,9 +430,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == kManyWarps) {
-    // ------------------------------------------------------------ TMA
-    if (lane == 0) {
+  if (warp >= kManyWarps) {
+    regs_dec<kIssueRegs>();
+    if (warp == kManyWarps && lane == 0) {
+      // ---------------------------------------------------------- TMA
       uint32_t it = 0;
       for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
         const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
@@ -451,10 +457,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
         flag(p.status, MTC_STATUS_TIMEOUT);
       }
-    }
-  } else if (warp == kManyWarps + 1) {
-    // ------------------------------------------------------------ MMA
-    if (lane == 0) {
+    } else if (warp == kManyWarps + 1 && lane == 0) {
+      // ---------------------------------------------------------- MMA
       constexpr uint32_t idesc = idesc_e4m3_f32(128, 256);
       uint32_t it = 0;
       for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
@@ -478,156 +482,186 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ scale and add, then store
-    const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
-    float* stg = staging + warp * (kStaging / 4);
+    regs_inc<kScaleRegs>();
+    const int quad = warp & 3, qt = warp >> 2;  // TMEM lanes 32 quad .., columns 64 qt ..
+    float* stg = staging + warp * kStaging;
     uint32_t it = 0;
     bool stop = false;
     for (int t = blockIdx.x; t < n_work && !stop; t += gridDim.x) {
       const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
       const int nt = t / n_slots;
       const int row = slot.row0 + 32 * quad + lane;
-      const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
+      const int n0 = GATED ? nt * 128 + 64 * (qt & 1) : nt * 256 + 64 * qt;  // first feature of this warp
       const bool row_ok = row < slot.end;
-      const int nb = min(n0 >> 7, p.Nb - 1);
-      const float* swp = p.sw[GATED ? hf : 0] + ((long long)slot.e * p.Nb + nb) * p.nkb;
-      const float* sxp = p.sx + row;
-      // scales of the blocks kb and kb + 1, multiplied where they are used so
-      // that nothing waits for the loads before that
-      auto sx_at = [&](int kb) { return (row_ok && kb < p.nkb) ? sxp[(long long)kb * p.lds] : 0.0f; };
-      auto sw_at = [&](int kb) { return kb < p.nkb ? __ldg(swp + kb) : 0.0f; };
-      float x0 = sx_at(0), x1 = sx_at(1), w0 = sw_at(0), w1 = sw_at(1);
-      float acc[128];
+      // Scales of the blocks kb and kb + 1, multiplied where they are used so
+      // that nothing waits for the loads before that.  A row past the end
+      // takes the last row's scales (its values are never stored).
+      const float* swp =
+          p.sw[GATED ? qt >> 1 : 0] + ((long long)slot.e * p.Nb + min(n0 >> 7, p.Nb - 1)) * p.nkb;
+      const float* sxp = p.sx + min(row, slot.end - 1);
+      float x0 = *sxp, w0 = __ldg(swp), x1 = x0, w1 = w0;
+      if (p.nkb > 1) {
+        x1 = sxp[p.lds];
+        w1 = __ldg(swp + 1);
+      }
+      const float* sxn = sxp + 2 * p.lds;
+      f32x2 acc[32];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < 32; ++j) acc[j] = 0ull;
       bool ok = true;
+#pragma unroll 1
       for (int kb = 0; kb < p.nkb; ++kb, ++it) {
         const int b = it & 1;
-        const float sc = x0 * w0;
+        const f32x2 sc = pair(x0 * w0, x0 * w0);
         x0 = x1;
         w0 = w1;
-        x1 = sx_at(kb + 2);
-        w1 = sw_at(kb + 2);
-        if (!__all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(&acc_full[b], (it >> 1) & 1, p.timeout_ns))) {
+        if (kb + 2 < p.nkb) {
+          x1 = *sxn;
+          w1 = __ldg(swp + kb + 2);
+          sxn += p.lds;
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (it >> 1) & 1, p.timeout_ns))) {
           abort_flag[0] = 1;
           ok = false;
           break;
         }
         tc::fence_after();
-        uint32_t v[2][16];
-        const uint32_t ta = tmem + b * 256 + 128 * hf + ((uint32_t)(32 * quad) << 16);
-        tmem_ld16(ta, v[0]);
+        uint32_t v[32];
+        const uint32_t ta = tmem + b * 256 + 64 * qt + ((uint32_t)(32 * quad) << 16);
+        tmem_ld32(ta, v);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_wait16(v[c & 1]);
-          if (c < 7) {
-            tmem_ld16(ta + 16 * (c + 1), v[(c + 1) & 1]);
-          } else {
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
-          }
+        for (int j = 0; j < 16; ++j) fma2(acc[j], pair(v[2 * j], v[2 * j + 1]), sc);
+        tmem_ld32(ta + 32, v);
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[b]);
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) fma2(acc[16 * c + j], acc[16 * c + j + 1], v[c & 1][j], v[c & 1][j + 1], sc);
-        }
+        for (int j = 0; j < 16; ++j) fma2(acc[16 + j], pair(v[2 * j], v[2 * j + 1]), sc);
       }
       if constexpr (GATED) {
-        // warps 4..7 hand their up values, 16 columns at a time, to the gate
-        // warps of the same rows through two of the staging areas
-        float* ex[2] = {staging + quad * (kStaging / 4), staging + (4 + quad) * (kStaging / 4)};
-        if (hf == 1) {
+        // Quarters 2 and 3 (up) hand their values, 8 columns at a time,
+        // to quarters 0 and 1 (gate) of the same rows through the staging
+        // areas of the two warps in turn.
+        const int g = qt & 1, id = 5 + 2 * quad + g;
+        float* ex[2] = {staging + (4 * g + quad) * kStaging, staging + (4 * (g + 2) + quad) * kStaging};
+        if (qt >= 2) {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             float* d = ex[c & 1] + lane * kStageLd;
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(d + j) =
-                  make_float4(acc[16 * c + j], acc[16 * c + j + 1], acc[16 * c + j + 2], acc[16 * c + j + 3]);
-            pair_sync(1 + quad);
+            *reinterpret_cast<ulonglong2*>(d) = make_ulonglong2(acc[4 * c], acc[4 * c + 1]);
+            *reinterpret_cast<ulonglong2*>(d + 4) = make_ulonglong2(acc[4 * c + 2], acc[4 * c + 3]);
+            pair_sync(id);
           }
+          (void)quad_sync_or(1 + quad, false);
         } else {
           uint32_t am = 0;
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
-            pair_sync(1 + quad);
+            pair_sync(id);
             const float* u = ex[c & 1] + lane * kStageLd;
-            float g[16];
-            move_chunk<false>(c, acc, g);
+            const float4 ua = *reinterpret_cast<const float4*>(u), ub = *reinterpret_cast<const float4*>(u + 4);
+            const float uu[8] = {ua.x, ua.y, ua.z, ua.w, ub.x, ub.y, ub.z, ub.w};
+            float h[8];
+            move_chunk<false>(c, acc, h);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 u4 = *reinterpret_cast<const float4*>(u + j);
-              const float uu[4] = {u4.x, u4.y, u4.z, u4.w};
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                g[j + q] = n0 + 16 * c + j + q < p.N ? epi_act(g[j + q], p.act) * uu[q] : 0.0f;
-                am = max(am, abs_bits(g[j + q]));
-              }
-            }
-            move_chunk<true>(c, acc, g);
+            for (int j = 0; j < 8; ++j) h[j] = n0 + 8 * c + j < p.N ? epi_act(h[j], p.act) * uu[j] : 0.0f;
+            am = max(am, amax8(h));
+            move_chunk<true>(c, acc, h);
           }
+          // the scale covers both gate warps' columns
+          row_max[g * 128 + 32 * quad + lane] = am;
+          (void)quad_sync_or(1 + quad, false);
+          am = max(am, row_max[(g ^ 1) * 128 + 32 * quad + lane]);
           if (row_ok && ok) {
-            const GroupScale g = group_scale(am);
-            p.hs[(long long)nt * p.hs_ld + row] = g.scale;
+            const GroupScale gs = group_scale(am);
+            if (g == 0) p.hs[(long long)nt * p.hs_ld + row] = gs.scale;
+            uint8_t* out = p.hq + (long long)row * p.ldh + n0;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
+            for (int c = 0; c < 4; ++c)
               if (n0 + 16 * c < p.ldh) {
                 uint32_t w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  const int q = 16 * c + 4 * j;
-                  w[j] = g.mul == 0.0f ? 0u
-                                       : codes2(acc[q], acc[q + 1], g.mul) | codes2(acc[q + 2], acc[q + 3], g.mul) << 16;
+                  float h[4];
+                  unpair(acc[8 * c + 2 * j], h[0], h[1]);
+                  unpair(acc[8 * c + 2 * j + 1], h[2], h[3]);
+                  w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
                 }
-                *reinterpret_cast<uint4*>(p.hq + (long long)row * p.ldh + n0 + 16 * c) =
-                    make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
               }
           }
         }
-        // the areas are free for the next tile; both warps of the pair stop at the same one
-        stop = pair_sync_or(1 + quad, !ok);
+        // the areas are free for the next tile; the four warps stop at the same one
+        stop = quad_sync_or(1 + quad, !ok);
       } else if (!ok) {
         stop = true;
       } else {
-        // 16 columns at a time through the warp's staging area: rows in, row
+        // 8 columns at a time through the warp's staging area: rows in, row
         // pieces out (a loop, so that the epilogue's code stands once)
 #pragma unroll 1
         for (int c = 0; c < 8; ++c) {
-          const int nc = n0 + 16 * c;
-          float* d = stg + lane * kStageLd;
-          float t16[16];
-          move_chunk<false>(c, acc, t16);
+          const int nc = n0 + 8 * c;
+          float o[8];
+          move_chunk<false>(c, acc, o);
+          if (p.bias || p.act) {
 #pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<float4*>(d + j) = make_float4(t16[j], t16[j + 1], t16[j + 2], t16[j + 3]);
-          __syncwarp();
-          // lane: 4 columns of row 8 r + lane / 4
-#pragma unroll 1
-          for (int r = 0; r < 4; ++r) {
-            const int rr = 8 * r + (lane >> 2), n = nc + 4 * (lane & 3);
-            const long long m = slot.row0 + 32 * quad + rr;
-            if (m >= slot.end) continue;
-            const float4 o4 = *reinterpret_cast<const float4*>(stg + rr * kStageLd + 4 * (lane & 3));
-            float o[4] = {o4.x, o4.y, o4.z, o4.w};
-            if (p.bias || p.act) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if (p.bias && n + q < p.N) o[q] += __ldg(p.bias + n + q);
-                if (p.act) o[q] = epi_act(o[q], p.act);
-              }
-            }
-            const long long at = m * p.ldy + n;
-            if (p.vec && n + 3 < p.N) {
-              if (p.ydt == MTC_F32)
-                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + at) = make_float4(o[0], o[1], o[2], o[3]);
-              else
-                *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.Y) + at) =
-                    make_uint2(pack2(p.ydt, o[0], o[1]), pack2(p.ydt, o[2], o[3]));
-            } else {
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (n + q < p.N) store1(p.Y, p.ydt, at + q, o[q]);
+            for (int j = 0; j < 8; ++j) {
+              if (p.bias && nc + j < p.N) o[j] += __ldg(p.bias + nc + j);
+              if (p.act) o[j] = epi_act(o[j], p.act);
             }
           }
-          __syncwarp();
+          uint32_t* d = reinterpret_cast<uint32_t*>(stg) + lane * kStageLd;
+          if (!p.vec) {
+            if (row_ok) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (nc + j < p.N) store1(p.Y, p.ydt, row * p.ldy + nc + j, o[j]);
+            }
+          } else if (p.ydt == MTC_F32) {
+            // lane: 4 columns of row 16 r + lane / 2
+            *reinterpret_cast<float4*>(d) = make_float4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<float4*>(d + 4) = make_float4(o[4], o[5], o[6], o[7]);
+            __syncwarp();
+            const int n = nc + 4 * (lane & 1);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int rr = 16 * r + (lane >> 1), m = slot.row0 + 32 * quad + rr;
+              if (m >= slot.end || n >= p.N) continue;
+              const float4 x = *reinterpret_cast<const float4*>(stg + rr * kStageLd + 4 * (lane & 1));
+              float* y = reinterpret_cast<float*>(p.Y) + m * p.ldy + n;
+              if (n + 3 < p.N) {
+                *reinterpret_cast<float4*>(y) = x;
+              } else {
+                y[0] = x.x;
+                if (n + 1 < p.N) y[1] = x.y;
+                if (n + 2 < p.N) y[2] = x.z;
+              }
+            }
+            __syncwarp();
+          } else {
+            // 16-bit outputs: two chunks fill a row piece of 16 columns
+            *reinterpret_cast<uint4*>(d + 4 * (c & 1)) = make_uint4(pack2(p.ydt, o[0], o[1]), pack2(p.ydt, o[2], o[3]),
+                                                                    pack2(p.ydt, o[4], o[5]), pack2(p.ydt, o[6], o[7]));
+            if ((c & 1) == 0) continue;
+            __syncwarp();
+            const int n = nc - 8 + 8 * (lane & 1);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int rr = 16 * r + (lane >> 1), m = slot.row0 + 32 * quad + rr;
+              if (m >= slot.end || n >= p.N) continue;
+              const uint4 x = *reinterpret_cast<const uint4*>(stg + rr * kStageLd + 4 * (lane & 1));
+              uint16_t* y = reinterpret_cast<uint16_t*>(p.Y) + m * p.ldy + n;
+              if (n + 7 < p.N) {
+                *reinterpret_cast<uint4*>(y) = x;
+              } else {
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (n + j < p.N) y[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+              }
+            }
+            __syncwarp();
+          }
         }
       }
     }
@@ -762,8 +796,7 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
     p.Y = a.Y;
     p.ydt = a.ydt;
     p.ldy = a.ldy;
-    const uintptr_t align = a.ydt == MTC_F32 ? 16 : 8;
-    p.vec = (reinterpret_cast<uintptr_t>(a.Y) & (align - 1)) == 0 && (a.ldy & 3) == 0;
+    p.vec = (reinterpret_cast<uintptr_t>(a.Y) & 15) == 0 && (a.ldy & (a.ydt == MTC_F32 ? 3 : 7)) == 0;
     p.bias = a.bias;
     p.act = n_mats == 2 ? a.gate_act : a.act;
     p.hq = a.hq;
