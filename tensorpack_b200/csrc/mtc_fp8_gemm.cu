@@ -330,16 +330,16 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
 // ---------------------------------------------------------------------------
 constexpr int kManyStages = 4;
 constexpr uint32_t kManyStage = 3 * kATile;
-constexpr int kManyWarps = 16;                        // scaling warps: 4 column quarters x 4 lane quadrants
+constexpr int kManyWarps = 8;                         // scaling warps: 2 column halves x 4 lane quadrants
 constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup with the TMA and the MMA warp
-constexpr int kStageLd = 12;                          // words per row of the staging (8 used): 16-byte accesses, no bank conflict
+constexpr int kStageLd = 20;                          // words per row of the staging (16 used): 16-byte accesses, no bank conflict
 constexpr int kStaging = 32 * kStageLd;               // words per warp
-constexpr uint32_t kManyBars = kManyStages * kManyStage + kManyWarps * kStaging * 4 + 2 * 128 * 4;
+constexpr uint32_t kManyBars = kManyStages * kManyStage + kManyWarps * kStaging * 4;
 constexpr size_t kManySmem = 1024 + kManyBars + 256;
-// Registers: 640 threads are launched with 96 each; the scaling warps (64
+// Registers: 384 threads are launched with 168 each; the scaling warps (128
 // fp32 sums and 32 loaded values a thread) take what the last warpgroup gives
-// back: 4 x 128 x 112 + 128 x 32 = 640 x 96.
-constexpr int kScaleRegs = 112, kIssueRegs = 32;
+// back: 2 x 128 x 224 + 128 x 24 <= 384 x 168.
+constexpr int kScaleRegs = 224, kIssueRegs = 24;
 
 struct ManyParams {
   int nkb, N, Nb, n_tiles;            // n_tiles: feature tiles (256 wide, or 128 of gate and up)
@@ -361,15 +361,15 @@ struct ManyParams {
   unsigned long long timeout_ns;
 };
 
-// Barriers of the warps that share rows: two of them (64 threads), or all
-// four column quarters, who learn whether any of them passed true.
+// Barriers of the two warps that share rows (64 threads); the second form
+// tells both whether either of them passed true.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool quad_sync_or(int id, bool x) {
+__device__ __forceinline__ bool pair_sync_or(int id, bool x) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %2, 0;\n\t"
-      "bar.red.or.pred q, %1, 128, p;\n\t"
+      "bar.red.or.pred q, %1, 64, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"(id), "r"((uint32_t)x)
@@ -377,17 +377,17 @@ __device__ __forceinline__ bool quad_sync_or(int id, bool x) {
   return r != 0;
 }
 
-// 8 accumulators of chunk c (0..7): a uniform branch to the one copy of the
+// 16 accumulators of chunk c (0..7): a uniform branch to the one copy of the
 // moves, so that loops over chunks can stay loops and hold their body once.
 template <bool TO_ACC>
-__device__ __forceinline__ void move_chunk(int c, f32x2 (&acc)[32], float (&t)[8]) {
+__device__ __forceinline__ void move_chunk(int c, f32x2 (&acc)[64], float (&t)[16]) {
 #pragma unroll
   for (int q = 0; q < 8; ++q)
     if (c == q) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (TO_ACC) acc[4 * q + j] = pair(t[2 * j], t[2 * j + 1]);
-        else unpair(acc[4 * q + j], t[2 * j], t[2 * j + 1]);
+      for (int j = 0; j < 8; ++j) {
+        if (TO_ACC) acc[8 * q + j] = pair(t[2 * j], t[2 * j + 1]);
+        else unpair(acc[8 * q + j], t[2 * j], t[2 * j + 1]);
       }
     }
 }
@@ -399,7 +399,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* staging = reinterpret_cast<float*>(smem + kManyStages * kManyStage);
-  uint32_t* row_max = reinterpret_cast<uint32_t*>(staging + kManyWarps * kStaging);  // [2][128]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kManyBars);
   uint64_t* empty = full + kManyStages;
   uint64_t* acc_full = empty + kManyStages;  // [2]
@@ -483,7 +482,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   } else {
     // ------------------------------------------------------------ scale and add, then store
     regs_inc<kScaleRegs>();
-    const int quad = warp & 3, qt = warp >> 2;  // TMEM lanes 32 quad .., columns 64 qt ..
+    const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
     float* stg = staging + warp * kStaging;
     uint32_t it = 0;
     bool stop = false;
@@ -491,13 +490,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
       const int nt = t / n_slots;
       const int row = slot.row0 + 32 * quad + lane;
-      const int n0 = GATED ? nt * 128 + 64 * (qt & 1) : nt * 256 + 64 * qt;  // first feature of this warp
+      const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
       const bool row_ok = row < slot.end;
       // Scales of the blocks kb and kb + 1, multiplied where they are used so
       // that nothing waits for the loads before that.  A row past the end
       // takes the last row's scales (its values are never stored).
-      const float* swp =
-          p.sw[GATED ? qt >> 1 : 0] + ((long long)slot.e * p.Nb + min(n0 >> 7, p.Nb - 1)) * p.nkb;
+      const float* swp = p.sw[GATED ? hf : 0] + ((long long)slot.e * p.Nb + min(n0 >> 7, p.Nb - 1)) * p.nkb;
       const float* sxp = p.sx + min(row, slot.end - 1);
       float x0 = *sxp, w0 = __ldg(swp), x1 = x0, w1 = w0;
       if (p.nkb > 1) {
@@ -505,9 +503,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         w1 = __ldg(swp + 1);
       }
       const float* sxn = sxp + 2 * p.lds;
-      f32x2 acc[32];
+      f32x2 acc[64];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) acc[j] = 0ull;
+      for (int j = 0; j < 64; ++j) acc[j] = 0ull;
       bool ok = true;
 #pragma unroll 1
       for (int kb = 0; kb < p.nkb; ++kb, ++it) {
@@ -526,58 +524,60 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           break;
         }
         tc::fence_after();
-        uint32_t v[32];
-        const uint32_t ta = tmem + b * 256 + 64 * qt + ((uint32_t)(32 * quad) << 16);
-        tmem_ld32(ta, v);
+        const uint32_t ta = tmem + b * 256 + 128 * hf + ((uint32_t)(32 * quad) << 16);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) fma2(acc[j], pair(v[2 * j], v[2 * j + 1]), sc);
-        tmem_ld32(ta + 32, v);
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[b]);
+        for (int c = 0; c < 8; ++c) {
+          uint32_t v[16];
+          tmem_ld16(ta + 16 * c, v);
+          tmem_wait16(v);
+          if (c == 7) {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+          }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) fma2(acc[16 + j], pair(v[2 * j], v[2 * j + 1]), sc);
+          for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[2 * j], v[2 * j + 1]), sc);
+        }
       }
       if constexpr (GATED) {
-        // Quarters 2 and 3 (up) hand their values, 8 columns at a time,
-        // to quarters 0 and 1 (gate) of the same rows through the staging
-        // areas of the two warps in turn.
-        const int g = qt & 1, id = 5 + 2 * quad + g;
-        float* ex[2] = {staging + (4 * g + quad) * kStaging, staging + (4 * (g + 2) + quad) * kStaging};
-        if (qt >= 2) {
+        // Warps 4..7 (up) hand their values, 16 columns at a time, to the gate
+        // warps of the same rows through the staging areas of the two in turn.
+        float* ex[2] = {staging + quad * kStaging, staging + (4 + quad) * kStaging};
+        if (hf == 1) {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             float* d = ex[c & 1] + lane * kStageLd;
-            *reinterpret_cast<ulonglong2*>(d) = make_ulonglong2(acc[4 * c], acc[4 * c + 1]);
-            *reinterpret_cast<ulonglong2*>(d + 4) = make_ulonglong2(acc[4 * c + 2], acc[4 * c + 3]);
-            pair_sync(id);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              *reinterpret_cast<ulonglong2*>(d + 2 * j) = make_ulonglong2(acc[8 * c + j], acc[8 * c + j + 1]);
+            pair_sync(1 + quad);
           }
-          (void)quad_sync_or(1 + quad, false);
         } else {
           uint32_t am = 0;
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
-            pair_sync(id);
+            pair_sync(1 + quad);
             const float* u = ex[c & 1] + lane * kStageLd;
-            const float4 ua = *reinterpret_cast<const float4*>(u), ub = *reinterpret_cast<const float4*>(u + 4);
-            const float uu[8] = {ua.x, ua.y, ua.z, ua.w, ub.x, ub.y, ub.z, ub.w};
-            float h[8];
+            float h[16];
             move_chunk<false>(c, acc, h);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = n0 + 8 * c + j < p.N ? epi_act(h[j], p.act) * uu[j] : 0.0f;
-            am = max(am, amax8(h));
+            for (int j = 0; j < 16; j += 4) {
+              const float4 u4 = *reinterpret_cast<const float4*>(u + j);
+              const float uu[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                h[j + q] = n0 + 16 * c + j + q < p.N ? epi_act(h[j + q], p.act) * uu[q] : 0.0f;
+                am = max(am, abs_bits(h[j + q]));
+              }
+            }
             move_chunk<true>(c, acc, h);
           }
-          // the scale covers both gate warps' columns
-          row_max[g * 128 + 32 * quad + lane] = am;
-          (void)quad_sync_or(1 + quad, false);
-          am = max(am, row_max[(g ^ 1) * 128 + 32 * quad + lane]);
           if (row_ok && ok) {
             const GroupScale gs = group_scale(am);
-            if (g == 0) p.hs[(long long)nt * p.hs_ld + row] = gs.scale;
+            p.hs[(long long)nt * p.hs_ld + row] = gs.scale;
             uint8_t* out = p.hq + (long long)row * p.ldh + n0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 8; ++c)
               if (n0 + 16 * c < p.ldh) {
                 uint32_t w[4];
 #pragma unroll
@@ -591,43 +591,44 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               }
           }
         }
-        // the areas are free for the next tile; the four warps stop at the same one
-        stop = quad_sync_or(1 + quad, !ok);
+        // the areas are free for the next tile; both warps of the pair stop at the same one
+        stop = pair_sync_or(1 + quad, !ok);
       } else if (!ok) {
         stop = true;
       } else {
-        // 8 columns at a time through the warp's staging area: rows in, row
+        // 16 columns at a time through the warp's staging area: rows in, row
         // pieces out (a loop, so that the epilogue's code stands once)
 #pragma unroll 1
         for (int c = 0; c < 8; ++c) {
-          const int nc = n0 + 8 * c;
-          float o[8];
+          const int nc = n0 + 16 * c;
+          float o[16];
           move_chunk<false>(c, acc, o);
           if (p.bias || p.act) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 16; ++j) {
               if (p.bias && nc + j < p.N) o[j] += __ldg(p.bias + nc + j);
               if (p.act) o[j] = epi_act(o[j], p.act);
             }
           }
           uint32_t* d = reinterpret_cast<uint32_t*>(stg) + lane * kStageLd;
+          const int sub = 4 * (lane & 3);  // this lane's 4 words of a row piece
           if (!p.vec) {
             if (row_ok) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
+              for (int j = 0; j < 16; ++j)
                 if (nc + j < p.N) store1(p.Y, p.ydt, row * p.ldy + nc + j, o[j]);
             }
           } else if (p.ydt == MTC_F32) {
-            // lane: 4 columns of row 16 r + lane / 2
-            *reinterpret_cast<float4*>(d) = make_float4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<float4*>(d + 4) = make_float4(o[4], o[5], o[6], o[7]);
-            __syncwarp();
-            const int n = nc + 4 * (lane & 1);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int rr = 16 * r + (lane >> 1), m = slot.row0 + 32 * quad + rr;
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(d + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            __syncwarp();
+            const int n = nc + sub;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int rr = 8 * r + (lane >> 2), m = slot.row0 + 32 * quad + rr;
               if (m >= slot.end || n >= p.N) continue;
-              const float4 x = *reinterpret_cast<const float4*>(stg + rr * kStageLd + 4 * (lane & 1));
+              const float4 x = *reinterpret_cast<const float4*>(stg + rr * kStageLd + sub);
               float* y = reinterpret_cast<float*>(p.Y) + m * p.ldy + n;
               if (n + 3 < p.N) {
                 *reinterpret_cast<float4*>(y) = x;
@@ -639,25 +640,28 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
             __syncwarp();
           } else {
-            // 16-bit outputs: two chunks fill a row piece of 16 columns
-            *reinterpret_cast<uint4*>(d + 4 * (c & 1)) = make_uint4(pack2(p.ydt, o[0], o[1]), pack2(p.ydt, o[2], o[3]),
-                                                                    pack2(p.ydt, o[4], o[5]), pack2(p.ydt, o[6], o[7]));
+            // 16-bit outputs: two chunks fill a row piece of 32 columns
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = pack2(p.ydt, o[2 * j], o[2 * j + 1]);
+            *reinterpret_cast<uint4*>(d + 8 * (c & 1)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(d + 8 * (c & 1) + 4) = make_uint4(w[4], w[5], w[6], w[7]);
             if ((c & 1) == 0) continue;
             __syncwarp();
-            const int n = nc - 8 + 8 * (lane & 1);
+            const int n = nc - 16 + 2 * sub;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int rr = 16 * r + (lane >> 1), m = slot.row0 + 32 * quad + rr;
+            for (int r = 0; r < 4; ++r) {
+              const int rr = 8 * r + (lane >> 2), m = slot.row0 + 32 * quad + rr;
               if (m >= slot.end || n >= p.N) continue;
-              const uint4 x = *reinterpret_cast<const uint4*>(stg + rr * kStageLd + 4 * (lane & 1));
+              const uint4 x = *reinterpret_cast<const uint4*>(stg + rr * kStageLd + sub);
               uint16_t* y = reinterpret_cast<uint16_t*>(p.Y) + m * p.ldy + n;
               if (n + 7 < p.N) {
                 *reinterpret_cast<uint4*>(y) = x;
               } else {
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                  if (n + j < p.N) y[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                  if (n + j < p.N) y[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
               }
             }
             __syncwarp();
