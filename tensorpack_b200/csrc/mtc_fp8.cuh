@@ -135,6 +135,20 @@ __device__ __forceinline__ uint32_t pack2(int dt, float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Activations with the hardware exponential and division (a few ulp; the
+// relative error of exp grows with |x|, but the result is then next to 0 or
+// x), short enough to be unrolled over a thread's sums: the many-row kernel's
+// epilogue.  GELU (tanh form) as x / (1 + exp(-2 u)), since
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)).
+template <int ACT>
+__device__ __forceinline__ float act_fast(float x) {
+  if constexpr (ACT == MTC_ACT_RELU) return x < 0.0f ? 0.0f : x;
+  else if constexpr (ACT == MTC_ACT_SILU) return __fdividef(x, 1.0f + __expf(-x));
+  else if constexpr (ACT == MTC_ACT_GELU_TANH)
+    return __fdividef(x, 1.0f + __expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+  else return x;
+}
+
 // ---------------------------------------------------------------------------
 // tcgen05, 8-bit operands
 // ---------------------------------------------------------------------------
@@ -172,46 +186,16 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
                : "memory");
 }
 
-// The same for 32 columns, completed before it returns.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr)
-      : "memory");
+// Asynchronous copies of this thread, shared memory -> global (both 16-byte
+// aligned, a multiple of 16 bytes), in groups; wait_read: the sources of all
+// of them have been read, wait_all: they are complete.
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
 }
-
-// Bounded wait without mbar_wait's suspend hint: the products hand an
-// accumulator back and forth every few hundred cycles, and a thread that was
-// put to sleep wakes too late for that.
-__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  const uint32_t addr = smem_u32(bar);
-  auto done = [&]() -> bool {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    return ok != 0;
-  };
-  if (done()) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (done()) return true;
-    if (globaltimer_ns() - t0 > limit_ns) return false;
-  }
-}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Registers per thread of a warpgroup, after the launch.
 template <int N>

@@ -13,10 +13,10 @@
 //    splits the inputs and adds its partial sums through distributed shared
 //    memory in rank order: no workspace, no atomics, the same result every
 //    time.
-//  * many_kernel<GATED>: 128 tokens x 256 features (TMEM lane = token), one
+//  * many_kernel<MODE>: 128 tokens x 256 features (TMEM lane = token), one
 //    persistent CTA per SM, two 256-column accumulators that alternate
 //    between the MMA and eight warps that scale and add.  Bound by the
-//    tensor cores.  GATED: the 256 features are 128 of the gate matrix and
+//    tensor cores.  kGated: the 256 features are 128 of the gate matrix and
 //    the same 128 of the up matrix; the output is act(gate) * up, quantized.
 #include "mtc_fp8.cuh"
 #include "mtc_internal.h"
@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
   uint64_t* empty = full + C::kStages;
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAcc;
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(acc_empty + C::kAcc);
+  uint64_t* drain = acc_empty + C::kAcc;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + 1);
   uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
   float* sring = reinterpret_cast<float*>(smem + C::kBars + 512);
 
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 4);
     }
+    mbar_init(drain, 1);
     abort_flag[0] = 0;
     fence_barrier_init();
   }
@@ -174,8 +176,13 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
         for (int j = 0; j < 4; ++j)
           mma_e4m3_ss(tmem + b * BN, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
                       j > 0);
-        tc::commit(&empty[s]);
         tc::commit(&acc_full[b]);
+        tc::commit(&empty[s]);
+      }
+      if (abort_flag[0]) {
+        // no MMA may read shared memory or write TMEM after this CTA has left
+        tc::commit(drain);
+        (void)mbar_wait(drain, 0, 100000000ull);
       }
     }
   } else if (warp < 4) {
@@ -328,18 +335,29 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
 // ---------------------------------------------------------------------------
 // many_kernel
 // ---------------------------------------------------------------------------
-constexpr int kManyStages = 4;
+constexpr int kManyStages = 3;
 constexpr uint32_t kManyStage = 3 * kATile;
 constexpr int kManyWarps = 8;                         // scaling warps: 2 column halves x 4 lane quadrants
 constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup with the TMA and the MMA warp
-constexpr int kStageLd = 20;                          // words per row of the staging (16 used): 16-byte accesses, no bank conflict
-constexpr int kStaging = 32 * kStageLd;               // words per warp
-constexpr uint32_t kManyBars = kManyStages * kManyStage + kManyWarps * kStaging * 4;
+// Staging of the output, per warp 32 rows of 256 bytes; the row stride of 17
+// 16-byte units keeps rows aligned for bulk copies and free of bank conflicts.
+constexpr uint32_t kRowBytes = 256, kRowLd = 272;
+constexpr uint32_t kStaging = 32 * kRowLd;
+// Scales of an iteration: the products sx * sw of 128 rows x 2 scale blocks
+// of the features, in a ring that the TMA warp fills together with a stage.
+// It writes iteration i after the MMA of i - kManyStages has completed, which
+// was issued after the sums of i - kManyStages - 2 were read: more slots than
+// kManyStages + 2 are never overwritten early.
+constexpr int kScaleSlots = 8;
+static_assert(kScaleSlots > kManyStages + 2, "a scale slot must outlive its reader");
+constexpr uint32_t kManyScales = kManyStages * kManyStage + kManyWarps * kStaging;
+constexpr uint32_t kManyBars = kManyScales + kScaleSlots * 256 * 4;
 constexpr size_t kManySmem = 1024 + kManyBars + 256;
+static_assert(kManySmem <= 227 * 1024, "shared memory of one CTA");
 // Registers: 384 threads are launched with 168 each; the scaling warps (128
-// fp32 sums and 32 loaded values a thread) take what the last warpgroup gives
-// back: 2 x 128 x 224 + 128 x 24 <= 384 x 168.
-constexpr int kScaleRegs = 224, kIssueRegs = 24;
+// fp32 sums and the values loaded) take what the last warpgroup gives back:
+// 2 x 128 x 208 + 128 x 64 <= 384 x 168.
+constexpr int kScaleRegs = 208, kIssueRegs = 64;
 
 struct ManyParams {
   int nkb, N, Nb, n_tiles;            // n_tiles: feature tiles (256 wide, or 128 of gate and up)
@@ -349,7 +367,7 @@ struct ManyParams {
   const float* sx;
   long long lds;
   void* Y;
-  int ydt, vec;
+  int ydt, y_bytes, vec;
   long long ldy;
   const float* bias;
   int act;
@@ -377,33 +395,52 @@ __device__ __forceinline__ bool pair_sync_or(int id, bool x) {
   return r != 0;
 }
 
-// 16 accumulators of chunk c (0..7): a uniform branch to the one copy of the
-// moves, so that loops over chunks can stay loops and hold their body once.
-template <bool TO_ACC>
-__device__ __forceinline__ void move_chunk(int c, f32x2 (&acc)[64], float (&t)[16]) {
+// Bias and activation of a warp's 128 columns, in place.
+template <int ACT>
+__device__ __forceinline__ void finish(f32x2 (&acc)[64], const float* bias, int left) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q)
-    if (c == q) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (TO_ACC) acc[8 * q + j] = pair(t[2 * j], t[2 * j + 1]);
-        else unpair(acc[8 * q + j], t[2 * j], t[2 * j + 1]);
-      }
+  for (int j = 0; j < 64; ++j) {
+    float x, y;
+    unpair(acc[j], x, y);
+    if (bias) {
+      if (2 * j < left) x += __ldg(bias + 2 * j);
+      if (2 * j + 1 < left) y += __ldg(bias + 2 * j + 1);
     }
+    acc[j] = pair(act_fast<ACT>(x), act_fast<ACT>(y));
+  }
 }
 
-template <bool GATED>
+// A staged row to global memory: up to 256 bytes, of which `left` exist (less
+// than that at the matrix edge); what does not fill 16 bytes goes as 16-bit
+// stores.
+__device__ __forceinline__ void store_row(uint8_t* dst, const uint8_t* src, int left, bool on) {
+  if (!on || left <= 0) return;
+  const int n = min(left, (int)kRowBytes), whole = n & ~15;
+  fence_proxy_async();
+  if (whole) bulk_s2g(dst, src, (uint32_t)whole);
+  for (int i = whole; i < n; i += 2) *reinterpret_cast<uint16_t*>(dst + i) = *reinterpret_cast<const uint16_t*>(src + i);
+  bulk_commit();
+}
+
+// What becomes of the sums: stored as they are, after bias and activation, or
+// (kGated + activation) act(gate) * up, quantized.
+enum { kPlain = 0, kEpilogue = 1, kGated = 2 };
+
+template <int MODE>
 __global__ void __launch_bounds__(kManyThreads, 1)
     many_kernel(const __grid_constant__ CUtensorMap tw0, const __grid_constant__ CUtensorMap tw1,
                 const __grid_constant__ CUtensorMap tx, const ManyParams p) {
+  constexpr bool GATED = MODE >= kGated;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* staging = reinterpret_cast<float*>(smem + kManyStages * kManyStage);
+  uint8_t* staging = smem + kManyStages * kManyStage;
+  float* scales = reinterpret_cast<float*>(smem + kManyScales);  // [kScaleSlots][2][128]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kManyBars);
   uint64_t* empty = full + kManyStages;
   uint64_t* acc_full = empty + kManyStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2]
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(acc_empty + 2);
+  uint64_t* drain = acc_empty + 2;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + 1);
   uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -413,13 +450,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kManyStages; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 2);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], kManyWarps);
     }
+    mbar_init(drain, 1);
     abort_flag[0] = 0;
     fence_barrier_init();
   }
@@ -431,30 +469,65 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (warp >= kManyWarps) {
     regs_dec<kIssueRegs>();
-    if (warp == kManyWarps && lane == 0) {
-      // ---------------------------------------------------------- TMA
+    if (warp == kManyWarps) {
+      // ------------------------------------------------------------ TMA (lane 0) and scales (all lanes)
       uint32_t it = 0;
-      for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
+      for (int t = blockIdx.x; t < n_work; t += gridDim.x) {
         const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
         const int nt = t / n_slots;
         const int f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
+        const long long sb = (long long)slot.e * p.Nb;
+        const float* sw0 = p.sw[0] + (sb + min(GATED ? nt : 2 * nt, p.Nb - 1)) * p.nkb;
+        const float* sw1 = GATED ? p.sw[1] + (sb + nt) * p.nkb : p.sw[0] + (sb + min(2 * nt + 1, p.Nb - 1)) * p.nkb;
+        // rows lane, lane + 32, ...; a row past the end takes the last row's
+        // scale (its values are never stored); loaded one block ahead
+        float x[4], w0, w1;
+        auto load = [&](int kb) {
+          const float* sx = p.sx + (long long)kb * p.lds;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = sx[min(slot.row0 + lane + 32 * j, slot.end - 1)];
+          w0 = __ldg(sw0 + kb);
+          w1 = __ldg(sw1 + kb);
+        };
+        load(0);
+        bool ok = true;
         for (int kb = 0; kb < p.nkb; ++kb, ++it) {
           const int s = it % kManyStages;
-          if (it >= kManyStages && !mbar_wait(&empty[s], ((it / kManyStages) & 1) ^ 1, p.timeout_ns)) {
-            abort_flag[0] = 1;
+          float a[4], b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            a[j] = x[j] * w0;
+            b[j] = x[j] * w1;
+          }
+          if (kb + 1 < p.nkb) load(kb + 1);
+          if (!__all_sync(0xffffffffu, it < kManyStages || mbar_wait(&empty[s], ((it / kManyStages) & 1) ^ 1, p.timeout_ns))) {
+            ok = false;
             break;
           }
-          uint8_t* st = smem + s * kManyStage;
-          mbar_expect_tx(&full[s], kManyStage);
-          tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
-          tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
-          tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
+          if (lane == 0) {
+            uint8_t* st = smem + s * kManyStage;
+            mbar_expect_tx(&full[s], kManyStage);
+            tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
+            tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
+            tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
+          }
+          float* sc = scales + (it % kScaleSlots) * 256 + lane;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[32 * j] = a[j];
+            sc[128 + 32 * j] = b[j];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
         }
+        if (!ok && lane == 0) abort_flag[0] = 1;
+        if (__any_sync(0xffffffffu, !ok || abort_flag[0])) break;
       }
-      if (abort_flag[0]) {
+      if (lane == 0) {
+        // nothing of this CTA may be in flight when it leaves
         for (uint32_t j = it > kManyStages ? it - kManyStages : 0; j < it; ++j)
           (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
-        flag(p.status, MTC_STATUS_TIMEOUT);
+        if (abort_flag[0]) flag(p.status, MTC_STATUS_TIMEOUT);
       }
     } else if (warp == kManyWarps + 1 && lane == 0) {
       // ---------------------------------------------------------- MMA
@@ -474,35 +547,29 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           for (int j = 0; j < 4; ++j)
             mma_e4m3_ss(tmem + b * 256, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
                         j > 0);
-          tc::commit(&empty[s]);
           tc::commit(&acc_full[b]);
+          tc::commit(&empty[s]);
         }
+      }
+      if (abort_flag[0]) {
+        // no MMA may read shared memory or write TMEM after this CTA has left
+        tc::commit(drain);
+        (void)mbar_wait(drain, 0, 100000000ull);
       }
     }
   } else {
     // ------------------------------------------------------------ scale and add, then store
     regs_inc<kScaleRegs>();
     const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
-    float* stg = staging + warp * kStaging;
+    uint8_t* my_row = staging + warp * kStaging + lane * kRowLd;
+    const float* my_scale = scales + 128 * hf + 32 * quad + lane;
+    // TMEM columns of the sums 0..63 and 64..127 (an up warp takes its halves
+    // the other way round: see below)
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16) + 128 * hf;
+    const uint32_t tm_a = lanes + (GATED ? 64 * hf : 0), tm_b = lanes + (GATED ? 64 * (hf ^ 1) : 64);
     uint32_t it = 0;
     bool stop = false;
     for (int t = blockIdx.x; t < n_work && !stop; t += gridDim.x) {
-      const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
-      const int nt = t / n_slots;
-      const int row = slot.row0 + 32 * quad + lane;
-      const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
-      const bool row_ok = row < slot.end;
-      // Scales of the blocks kb and kb + 1, multiplied where they are used so
-      // that nothing waits for the loads before that.  A row past the end
-      // takes the last row's scales (its values are never stored).
-      const float* swp = p.sw[GATED ? hf : 0] + ((long long)slot.e * p.Nb + min(n0 >> 7, p.Nb - 1)) * p.nkb;
-      const float* sxp = p.sx + min(row, slot.end - 1);
-      float x0 = *sxp, w0 = __ldg(swp), x1 = x0, w1 = w0;
-      if (p.nkb > 1) {
-        x1 = sxp[p.lds];
-        w1 = __ldg(swp + 1);
-      }
-      const float* sxn = sxp + 2 * p.lds;
       f32x2 acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0ull;
@@ -510,25 +577,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll 1
       for (int kb = 0; kb < p.nkb; ++kb, ++it) {
         const int b = it & 1;
-        const f32x2 sc = pair(x0 * w0, x0 * w0);
-        x0 = x1;
-        w0 = w1;
-        if (kb + 2 < p.nkb) {
-          x1 = *sxn;
-          w1 = __ldg(swp + kb + 2);
-          sxn += p.lds;
-        }
         if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (it >> 1) & 1, p.timeout_ns))) {
           abort_flag[0] = 1;
           ok = false;
           break;
         }
         tc::fence_after();
-        const uint32_t ta = tmem + b * 256 + 128 * hf + ((uint32_t)(32 * quad) << 16);
+        // the TMA warp wrote this block's scales before its MMA ran
+        const float sc1 = my_scale[(it % kScaleSlots) * 256];
+        const f32x2 sc = pair(sc1, sc1);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           uint32_t v[16];
-          tmem_ld16(ta + 16 * c, v);
+          tmem_ld16((c < 4 ? tm_a : tm_b) + b * 256 + 16 * (c & 3), v);
           tmem_wait16(v);
           if (c == 7) {
             tc::fence_before();
@@ -539,136 +600,119 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[2 * j], v[2 * j + 1]), sc);
         }
       }
+      // Every lane stages and stores its own row: the row goes out as one
+      // asynchronous copy while the next tile runs, and is waited for before
+      // the lane writes its staging again.
+      const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
+      const int nt = t / n_slots;
+      const int row = slot.row0 + 32 * quad + lane;
+      const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
+      const bool row_ok = row < slot.end && ok;
+      bulk_wait_read();
       if constexpr (GATED) {
-        // Warps 4..7 (up) hand their values, 16 columns at a time, to the gate
-        // warps of the same rows through the staging areas of the two in turn.
-        float* ex[2] = {staging + quad * kStaging, staging + (4 + quad) * kStaging};
-        if (hf == 1) {
+        // The gate warp and the up warp of the same rows each finish half of
+        // the columns: sums 0..63 stay, 64..127 go to the other warp through
+        // the staged row.  The gate warp keeps columns 0..63, the up warp
+        // 64..127.
+        const uint8_t* other = staging + (warp ^ 4) * kStaging + lane * kRowLd;
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float* d = ex[c & 1] + lane * kStageLd;
+        for (int j = 32; j < 64; j += 2)
+          *reinterpret_cast<ulonglong2*>(my_row + 8 * (j - 32)) = make_ulonglong2(acc[j], acc[j + 1]);
+        pair_sync(1 + quad);
+        const int n = n0 + 64 * hf, left = p.N - n;
+        uint32_t am = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j += 2)
-              *reinterpret_cast<ulonglong2*>(d + 2 * j) = make_ulonglong2(acc[8 * c + j], acc[8 * c + j + 1]);
-            pair_sync(1 + quad);
+        for (int j = 0; j < 32; j += 2) {
+          const float4 o4 = *reinterpret_cast<const float4*>(other + 8 * j);
+          const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+          float h[4];
+          unpair(acc[j], h[0], h[1]);
+          unpair(acc[j + 1], h[2], h[3]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float g = hf ? o[q] : h[q], u = hf ? h[q] : o[q];
+            h[q] = 2 * j + q < left ? act_fast<MODE - kGated>(g) * u : 0.0f;
+            am = max(am, abs_bits(h[q]));
           }
-        } else {
-          uint32_t am = 0;
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            pair_sync(1 + quad);
-            const float* u = ex[c & 1] + lane * kStageLd;
-            float h[16];
-            move_chunk<false>(c, acc, h);
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 u4 = *reinterpret_cast<const float4*>(u + j);
-              const float uu[4] = {u4.x, u4.y, u4.z, u4.w};
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                h[j + q] = n0 + 16 * c + j + q < p.N ? epi_act(h[j + q], p.act) * uu[q] : 0.0f;
-                am = max(am, abs_bits(h[j + q]));
-              }
-            }
-            move_chunk<true>(c, acc, h);
-          }
-          if (row_ok && ok) {
-            const GroupScale gs = group_scale(am);
-            p.hs[(long long)nt * p.hs_ld + row] = gs.scale;
-            uint8_t* out = p.hq + (long long)row * p.ldh + n0;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              if (n0 + 16 * c < p.ldh) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  float h[4];
-                  unpair(acc[8 * c + 2 * j], h[0], h[1]);
-                  unpair(acc[8 * c + 2 * j + 1], h[2], h[3]);
-                  w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
-                }
-                *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-          }
+          acc[j] = pair(h[0], h[1]);
+          acc[j + 1] = pair(h[2], h[3]);
         }
-        // the areas are free for the next tile; both warps of the pair stop at the same one
+        // the scale covers both warps' columns; both stop at the same tile
+        *reinterpret_cast<uint32_t*>(my_row + kRowBytes) = am;
         stop = pair_sync_or(1 + quad, !ok);
+        am = max(am, *reinterpret_cast<const uint32_t*>(other + kRowBytes));
+        if (row_ok && left > 0) {
+          const GroupScale gs = group_scale(am);
+          if (hf == 0) p.hs[(long long)nt * p.hs_ld + row] = gs.scale;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float h[4];
+              unpair(acc[8 * c + 2 * j], h[0], h[1]);
+              unpair(acc[8 * c + 2 * j + 1], h[2], h[3]);
+              w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
+            }
+            *reinterpret_cast<uint4*>(my_row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          // (n and ldh are multiples of 16; codes past N are zero)
+          fence_proxy_async();
+          bulk_s2g(p.hq + (long long)row * p.ldh + n, my_row, (uint32_t)min(64ll, p.ldh - n));
+          bulk_commit();
+        }
+        // (the other warp reads this row's maximum before it can reach the
+        // next tile's first barrier, and only that barrier lets this warp on)
       } else if (!ok) {
         stop = true;
       } else {
-        // 16 columns at a time through the warp's staging area: rows in, row
-        // pieces out (a loop, so that the epilogue's code stands once)
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          const int nc = n0 + 16 * c;
-          float o[16];
-          move_chunk<false>(c, acc, o);
-          if (p.bias || p.act) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (p.bias && nc + j < p.N) o[j] += __ldg(p.bias + nc + j);
-              if (p.act) o[j] = epi_act(o[j], p.act);
-            }
+        const int left = p.N - n0;  // features of this warp that exist
+        uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + ((long long)row * p.ldy + n0) * p.y_bytes;
+        if constexpr (MODE == kEpilogue) {
+          const float* bias = p.bias ? p.bias + n0 : nullptr;
+          switch (p.act) {
+            case MTC_ACT_RELU: finish<MTC_ACT_RELU>(acc, bias, left); break;
+            case MTC_ACT_SILU: finish<MTC_ACT_SILU>(acc, bias, left); break;
+            case MTC_ACT_GELU_TANH: finish<MTC_ACT_GELU_TANH>(acc, bias, left); break;
+            default: finish<MTC_ACT_NONE>(acc, bias, left);
           }
-          uint32_t* d = reinterpret_cast<uint32_t*>(stg) + lane * kStageLd;
-          const int sub = 4 * (lane & 3);  // this lane's 4 words of a row piece
-          if (!p.vec) {
-            if (row_ok) {
+        }
+        if (!p.vec) {
+          // an output whose rows do not start on 16 bytes: one value at a time
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (nc + j < p.N) store1(p.Y, p.ydt, row * p.ldy + nc + j, o[j]);
-            }
-          } else if (p.ydt == MTC_F32) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(d + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            __syncwarp();
-            const int n = nc + sub;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int rr = 8 * r + (lane >> 2), m = slot.row0 + 32 * quad + rr;
-              if (m >= slot.end || n >= p.N) continue;
-              const float4 x = *reinterpret_cast<const float4*>(stg + rr * kStageLd + sub);
-              float* y = reinterpret_cast<float*>(p.Y) + m * p.ldy + n;
-              if (n + 3 < p.N) {
-                *reinterpret_cast<float4*>(y) = x;
-              } else {
-                y[0] = x.x;
-                if (n + 1 < p.N) y[1] = x.y;
-                if (n + 2 < p.N) y[2] = x.z;
-              }
-            }
-            __syncwarp();
-          } else {
-            // 16-bit outputs: two chunks fill a row piece of 32 columns
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = pack2(p.ydt, o[2 * j], o[2 * j + 1]);
-            *reinterpret_cast<uint4*>(d + 8 * (c & 1)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(d + 8 * (c & 1) + 4) = make_uint4(w[4], w[5], w[6], w[7]);
-            if ((c & 1) == 0) continue;
-            __syncwarp();
-            const int n = nc - 16 + 2 * sub;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int rr = 8 * r + (lane >> 2), m = slot.row0 + 32 * quad + rr;
-              if (m >= slot.end || n >= p.N) continue;
-              const uint4 x = *reinterpret_cast<const uint4*>(stg + rr * kStageLd + sub);
-              uint16_t* y = reinterpret_cast<uint16_t*>(p.Y) + m * p.ldy + n;
-              if (n + 7 < p.N) {
-                *reinterpret_cast<uint4*>(y) = x;
-              } else {
-                const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (n + j < p.N) y[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
-              }
-            }
-            __syncwarp();
+          for (int j = 0; j < 64; ++j) {
+            float o[2];
+            unpair(acc[j], o[0], o[1]);
+            if (row_ok && 2 * j < left) store1(p.Y, p.ydt, row * p.ldy + n0 + 2 * j, o[0]);
+            if (row_ok && 2 * j + 1 < left) store1(p.Y, p.ydt, row * p.ldy + n0 + 2 * j + 1, o[1]);
           }
+        } else if (p.ydt == MTC_F32) {
+          // 64 columns fill a staged row
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c) bulk_wait_read();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              *reinterpret_cast<ulonglong2*>(my_row + 8 * j) = make_ulonglong2(acc[32 * c + j], acc[32 * c + j + 1]);
+            store_row(y + 256 * c, my_row, 4 * (left - 64 * c), row_ok);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float o[2];
+              unpair(acc[4 * c + j], o[0], o[1]);
+              w[j] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[0], o[1]) : pack2(MTC_F16, o[0], o[1]);
+            }
+            *reinterpret_cast<uint4*>(my_row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          store_row(y, my_row, 2 * left, row_ok);
         }
       }
     }
+    bulk_wait_all();
   }
 
   __syncwarp();
@@ -799,17 +843,25 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
     p.lds = a.lds;
     p.Y = a.Y;
     p.ydt = a.ydt;
+    p.y_bytes = a.ydt == MTC_F32 ? 4 : 2;
     p.ldy = a.ldy;
     p.vec = (reinterpret_cast<uintptr_t>(a.Y) & 15) == 0 && (a.ldy & (a.ydt == MTC_F32 ? 3 : 7)) == 0;
     p.bias = a.bias;
-    p.act = n_mats == 2 ? a.gate_act : a.act;
+    p.act = a.act;
     p.hq = a.hq;
     p.ldh = a.ldh;
     p.hs = a.hs;
     p.hs_ld = a.hs_ld;
     p.status = a.status;
     p.timeout_ns = wait_limit_ns();
-    auto kernel = n_mats == 2 ? many_kernel<true> : many_kernel<false>;
+    auto kernel = many_kernel<kPlain>;
+    if (n_mats == 2)
+      kernel = a.gate_act == MTC_ACT_RELU   ? many_kernel<kGated + MTC_ACT_RELU>
+               : a.gate_act == MTC_ACT_SILU ? many_kernel<kGated + MTC_ACT_SILU>
+               : a.gate_act == MTC_ACT_NONE ? many_kernel<kGated + MTC_ACT_NONE>
+                                            : many_kernel<kGated + MTC_ACT_GELU_TANH>;
+    else if (a.bias || a.act)
+      kernel = many_kernel<kEpilogue>;
     MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kManySmem), who);
     const long long work = (long long)a.slot_bound * p.n_tiles;
     kernel<<<(int)(work < sms ? work : sms), kManyThreads, kManySmem, st>>>(tw[0], tw[1], tx, p);
