@@ -186,16 +186,14 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&v)[16]) {
                : "memory");
 }
 
-// Asynchronous copies of this thread, shared memory -> global (both 16-byte
-// aligned, a multiple of 16 bytes), in groups; wait_read: the sources of all
-// of them have been read, wait_all: they are complete.
-__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
-               : "memory");
+// 4-byte asynchronous copy global -> shared memory, and this thread's arrival
+// (counted like any other) on `bar` once all its earlier ones have landed.
+__device__ __forceinline__ void copy4_async(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void copy4_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 // Registers per thread of a warpgroup, after the launch.
 template <int N>

@@ -335,29 +335,34 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
 // ---------------------------------------------------------------------------
 // many_kernel
 // ---------------------------------------------------------------------------
-constexpr int kManyStages = 3;
+constexpr int kManyStages = 4;
 constexpr uint32_t kManyStage = 3 * kATile;
 constexpr int kManyWarps = 8;                         // scaling warps: 2 column halves x 4 lane quadrants
 constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup with the TMA and the MMA warp
-// Staging of the output, per warp 32 rows of 256 bytes; the row stride of 17
-// 16-byte units keeps rows aligned for bulk copies and free of bank conflicts.
-constexpr uint32_t kRowBytes = 256, kRowLd = 272;
+// Staging of the output, per warp 32 rows of 64 bytes; the row stride of 5
+// 16-byte units keeps 16-byte accesses free of bank conflicts.  (More stages
+// beat more staging: with 3 stages and whole rows staged for asynchronous
+// copies the loads' latency showed, 281 against 2xx us.)
+constexpr int kRowLd = 80;
 constexpr uint32_t kStaging = 32 * kRowLd;
-// Scales of an iteration: the products sx * sw of 128 rows x 2 scale blocks
-// of the features, in a ring that the TMA warp fills together with a stage.
-// It writes iteration i after the MMA of i - kManyStages has completed, which
-// was issued after the sums of i - kManyStages - 2 were read: more slots than
-// kManyStages + 2 are never overwritten early.
-constexpr int kScaleSlots = 8;
+// Scales of an iteration: sx of 128 rows, sw of the two scale blocks of the
+// features, and the tile {first row, end row, feature tile}, in a ring that
+// the TMA warp fills together with a stage (4-byte asynchronous copies: rows
+// start anywhere, and no copy waits for a load).  It writes iteration i after
+// the MMA of i - kManyStages has completed, which was issued after the sums
+// of i - kManyStages - 2 were read: more slots than kManyStages + 2 are never
+// overwritten early.
+constexpr int kScaleSlots = 8, kScaleLd = 132;
 static_assert(kScaleSlots > kManyStages + 2, "a scale slot must outlive its reader");
 constexpr uint32_t kManyScales = kManyStages * kManyStage + kManyWarps * kStaging;
-constexpr uint32_t kManyBars = kManyScales + kScaleSlots * 256 * 4;
+constexpr uint32_t kManyTiles = kManyScales + kScaleSlots * kScaleLd * 4;
+constexpr uint32_t kManyBars = kManyTiles + kScaleSlots * 16;
 constexpr size_t kManySmem = 1024 + kManyBars + 256;
 static_assert(kManySmem <= 227 * 1024, "shared memory of one CTA");
 // Registers: 384 threads are launched with 168 each; the scaling warps (128
 // fp32 sums and the values loaded) take what the last warpgroup gives back:
-// 2 x 128 x 208 + 128 x 64 <= 384 x 168.
-constexpr int kScaleRegs = 208, kIssueRegs = 64;
+// 2 x 128 x 224 + 128 x 56 <= 384 x 168.
+constexpr int kScaleRegs = 224, kIssueRegs = 56;
 
 struct ManyParams {
   int nkb, N, Nb, n_tiles;            // n_tiles: feature tiles (256 wide, or 128 of gate and up)
@@ -410,16 +415,26 @@ __device__ __forceinline__ void finish(f32x2 (&acc)[64], const float* bias, int 
   }
 }
 
-// A staged row to global memory: up to 256 bytes, of which `left` exist (less
-// than that at the matrix edge); what does not fill 16 bytes goes as 16-bit
-// stores.
-__device__ __forceinline__ void store_row(uint8_t* dst, const uint8_t* src, int left, bool on) {
-  if (!on || left <= 0) return;
-  const int n = min(left, (int)kRowBytes), whole = n & ~15;
-  fence_proxy_async();
-  if (whole) bulk_s2g(dst, src, (uint32_t)whole);
-  for (int i = whole; i < n; i += 2) *reinterpret_cast<uint16_t*>(dst + i) = *reinterpret_cast<const uint16_t*>(src + i);
-  bulk_commit();
+// The warp's staged rows (64 bytes each) to row pieces: 4 lanes per row, 16
+// bytes per lane.  `left` bytes of every piece exist, rows from `rows` on do
+// not.  Called by whole warps.
+__device__ __forceinline__ void store_rows(uint8_t* dst, long long ld, const uint8_t* stg, int lane, int left, int rows) {
+  __syncwarp();
+  const int sub = 16 * (lane & 3);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int rr = 8 * r + (lane >> 2);
+    if (rr < rows && sub < left) {
+      const uint8_t* src = stg + rr * kRowLd + sub;
+      uint8_t* d = dst + rr * ld + sub;
+      if (sub + 16 <= left) {
+        *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(src);
+      } else {
+        for (int i = 0; i < left - sub; i += 2) *reinterpret_cast<uint16_t*>(d + i) = *reinterpret_cast<const uint16_t*>(src + i);
+      }
+    }
+  }
+  __syncwarp();
 }
 
 // What becomes of the sums: stored as they are, after bias and activation, or
@@ -434,7 +449,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* staging = smem + kManyStages * kManyStage;
-  float* scales = reinterpret_cast<float*>(smem + kManyScales);  // [kScaleSlots][2][128]
+  float* scales = reinterpret_cast<float*>(smem + kManyScales);  // [kScaleSlots][kScaleLd]
+  int4* tiles = reinterpret_cast<int4*>(smem + kManyTiles);      // [kScaleSlots]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kManyBars);
   uint64_t* empty = full + kManyStages;
   uint64_t* acc_full = empty + kManyStages;  // [2]
@@ -450,7 +466,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kManyStages; ++i) {
-      mbar_init(&full[i], 2);
+      mbar_init(&full[i], 1 + 32);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -472,53 +488,43 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (warp == kManyWarps) {
       // ------------------------------------------------------------ TMA (lane 0) and scales (all lanes)
       uint32_t it = 0;
+      Slot next = slot_at(p.slots, p.M, 128, blockIdx.x % n_slots);  // one tile ahead
       for (int t = blockIdx.x; t < n_work; t += gridDim.x) {
-        const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
-        const int nt = t / n_slots;
-        const int f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
-        const long long sb = (long long)slot.e * p.Nb;
-        const float* sw0 = p.sw[0] + (sb + min(GATED ? nt : 2 * nt, p.Nb - 1)) * p.nkb;
-        const float* sw1 = GATED ? p.sw[1] + (sb + nt) * p.nkb : p.sw[0] + (sb + min(2 * nt + 1, p.Nb - 1)) * p.nkb;
+        const Slot slot = next;
+        if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, p.M, 128, (t + gridDim.x) % n_slots);
+        const int nt = t / n_slots, f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
+        // lanes 0 and 1 fetch the features' scales, every lane those of the
         // rows lane, lane + 32, ...; a row past the end takes the last row's
-        // scale (its values are never stored); loaded one block ahead
-        float x[4], w0, w1;
-        auto load = [&](int kb) {
-          const float* sx = p.sx + (long long)kb * p.lds;
+        // scale (its values are never stored)
+        const long long sb = (long long)slot.e * p.Nb;
+        const float* sw = GATED ? p.sw[lane & 1] + (sb + nt) * p.nkb
+                                : p.sw[0] + (sb + min(2 * nt + (lane & 1), p.Nb - 1)) * p.nkb;
+        const float* sx[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = sx[min(slot.row0 + lane + 32 * j, slot.end - 1)];
-          w0 = __ldg(sw0 + kb);
-          w1 = __ldg(sw1 + kb);
-        };
-        load(0);
+        for (int j = 0; j < 4; ++j) sx[j] = p.sx + min(slot.row0 + lane + 32 * j, slot.end - 1);
         bool ok = true;
         for (int kb = 0; kb < p.nkb; ++kb, ++it) {
           const int s = it % kManyStages;
-          float a[4], b[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            a[j] = x[j] * w0;
-            b[j] = x[j] * w1;
-          }
-          if (kb + 1 < p.nkb) load(kb + 1);
           if (!__all_sync(0xffffffffu, it < kManyStages || mbar_wait(&empty[s], ((it / kManyStages) & 1) ^ 1, p.timeout_ns))) {
             ok = false;
             break;
           }
           if (lane == 0) {
             uint8_t* st = smem + s * kManyStage;
+            tiles[it % kScaleSlots] = make_int4(slot.row0, slot.end, nt, 0);
             mbar_expect_tx(&full[s], kManyStage);
             tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
             tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
             tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
           }
-          float* sc = scales + (it % kScaleSlots) * 256 + lane;
+          float* sc = scales + (it % kScaleSlots) * kScaleLd;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sc[32 * j] = a[j];
-            sc[128 + 32 * j] = b[j];
+            copy4_async(sc + lane + 32 * j, sx[j]);
+            sx[j] += p.lds;
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[s]);
+          if (lane < 2) copy4_async(sc + 128 + lane, sw + kb);
+          copy4_arrive(&full[s]);
         }
         if (!ok && lane == 0) abort_flag[0] = 1;
         if (__any_sync(0xffffffffu, !ok || abort_flag[0])) break;
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     regs_inc<kScaleRegs>();
     const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
     uint8_t* my_row = staging + warp * kStaging + lane * kRowLd;
-    const float* my_scale = scales + 128 * hf + 32 * quad + lane;
+    const int my_scale = 32 * quad + lane;
     // TMEM columns of the sums 0..63 and 64..127 (an up warp takes its halves
     // the other way round: see below)
     const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16) + 128 * hf;
@@ -584,7 +590,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         tc::fence_after();
         // the TMA warp wrote this block's scales before its MMA ran
-        const float sc1 = my_scale[(it % kScaleSlots) * 256];
+        const float* slot = scales + (it % kScaleSlots) * kScaleLd;
+        const float sc1 = slot[my_scale] * slot[128 + hf];
         const f32x2 sc = pair(sc1, sc1);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -600,74 +607,68 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[2 * j], v[2 * j + 1]), sc);
         }
       }
-      // Every lane stages and stores its own row: the row goes out as one
-      // asynchronous copy while the next tile runs, and is waited for before
-      // the lane writes its staging again.
-      const Slot slot = slot_at(p.slots, p.M, 128, t % n_slots);
-      const int nt = t / n_slots;
-      const int row = slot.row0 + 32 * quad + lane;
+      const int4 tile = tiles[(it - 1) % kScaleSlots];
+      const int nt = tile.z, m0 = tile.x + 32 * quad;
       const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
-      const bool row_ok = row < slot.end && ok;
-      bulk_wait_read();
+      const int rows = ok ? tile.y - m0 : 0;                  // rows of this warp that exist (more than 32: all)
       if constexpr (GATED) {
         // The gate warp and the up warp of the same rows each finish half of
         // the columns: sums 0..63 stay, 64..127 go to the other warp through
-        // the staged row.  The gate warp keeps columns 0..63, the up warp
-        // 64..127.
+        // the staged rows, 16 at a time.  The gate warp keeps columns 0..63,
+        // the up warp 64..127.
         const uint8_t* other = staging + (warp ^ 4) * kStaging + lane * kRowLd;
-#pragma unroll
-        for (int j = 32; j < 64; j += 2)
-          *reinterpret_cast<ulonglong2*>(my_row + 8 * (j - 32)) = make_ulonglong2(acc[j], acc[j + 1]);
-        pair_sync(1 + quad);
         const int n = n0 + 64 * hf, left = p.N - n;
         uint32_t am = 0;
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float4 o4 = *reinterpret_cast<const float4*>(other + 8 * j);
-          const float o[4] = {o4.x, o4.y, o4.z, o4.w};
-          float h[4];
-          unpair(acc[j], h[0], h[1]);
-          unpair(acc[j + 1], h[2], h[3]);
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float g = hf ? o[q] : h[q], u = hf ? h[q] : o[q];
-            h[q] = 2 * j + q < left ? act_fast<MODE - kGated>(g) * u : 0.0f;
-            am = max(am, abs_bits(h[q]));
+          for (int j = 0; j < 8; j += 2)
+            *reinterpret_cast<ulonglong2*>(my_row + 8 * j) = make_ulonglong2(acc[32 + 8 * c + j], acc[33 + 8 * c + j]);
+          pair_sync(1 + quad);
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const float4 o4 = *reinterpret_cast<const float4*>(other + 8 * j);
+            const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+            float h[4];
+            unpair(acc[8 * c + j], h[0], h[1]);
+            unpair(acc[8 * c + j + 1], h[2], h[3]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float g = hf ? o[q] : h[q], u = hf ? h[q] : o[q];
+              h[q] = 16 * c + 2 * j + q < left ? act_fast<MODE - kGated>(g) * u : 0.0f;
+              am = max(am, abs_bits(h[q]));
+            }
+            acc[8 * c + j] = pair(h[0], h[1]);
+            acc[8 * c + j + 1] = pair(h[2], h[3]);
           }
-          acc[j] = pair(h[0], h[1]);
-          acc[j + 1] = pair(h[2], h[3]);
+          pair_sync(1 + quad);
         }
         // the scale covers both warps' columns; both stop at the same tile
-        *reinterpret_cast<uint32_t*>(my_row + kRowBytes) = am;
+        *reinterpret_cast<uint32_t*>(my_row + 64) = am;
         stop = pair_sync_or(1 + quad, !ok);
-        am = max(am, *reinterpret_cast<const uint32_t*>(other + kRowBytes));
-        if (row_ok && left > 0) {
-          const GroupScale gs = group_scale(am);
-          if (hf == 0) p.hs[(long long)nt * p.hs_ld + row] = gs.scale;
+        am = max(am, *reinterpret_cast<const uint32_t*>(other + 64));
+        const GroupScale gs = group_scale(am);
+        if (hf == 0 && lane < rows) p.hs[(long long)nt * p.hs_ld + m0 + lane] = gs.scale;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[4];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float h[4];
-              unpair(acc[8 * c + 2 * j], h[0], h[1]);
-              unpair(acc[8 * c + 2 * j + 1], h[2], h[3]);
-              w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
-            }
-            *reinterpret_cast<uint4*>(my_row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int j = 0; j < 4; ++j) {
+            float h[4];
+            unpair(acc[8 * c + 2 * j], h[0], h[1]);
+            unpair(acc[8 * c + 2 * j + 1], h[2], h[3]);
+            w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
           }
-          // (n and ldh are multiples of 16; codes past N are zero)
-          fence_proxy_async();
-          bulk_s2g(p.hq + (long long)row * p.ldh + n, my_row, (uint32_t)min(64ll, p.ldh - n));
-          bulk_commit();
+          *reinterpret_cast<uint4*>(my_row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        // (n and ldh are multiples of 16; codes past N are zero)
+        store_rows(p.hq + (long long)m0 * p.ldh + n, p.ldh, staging + warp * kStaging, lane, (int)min(64ll, p.ldh - n), rows);
         // (the other warp reads this row's maximum before it can reach the
-        // next tile's first barrier, and only that barrier lets this warp on)
+        // next tile's barriers, and only those let this warp write it again)
       } else if (!ok) {
         stop = true;
       } else {
         const int left = p.N - n0;  // features of this warp that exist
-        uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + ((long long)row * p.ldy + n0) * p.y_bytes;
         if constexpr (MODE == kEpilogue) {
           const float* bias = p.bias ? p.bias + n0 : nullptr;
           switch (p.act) {
@@ -677,42 +678,44 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             default: finish<MTC_ACT_NONE>(acc, bias, left);
           }
         }
-        if (!p.vec) {
-          // an output whose rows do not start on 16 bytes: one value at a time
+        uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + ((long long)m0 * p.ldy + n0) * p.y_bytes;
+        const long long ldy = p.ldy * p.y_bytes;
+        if (p.ydt == MTC_F32 || !p.vec) {
+          // 16 columns at a time; an output whose rows do not start on 16
+          // bytes takes them one value at a time
 #pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            float o[2];
-            unpair(acc[j], o[0], o[1]);
-            if (row_ok && 2 * j < left) store1(p.Y, p.ydt, row * p.ldy + n0 + 2 * j, o[0]);
-            if (row_ok && 2 * j + 1 < left) store1(p.Y, p.ydt, row * p.ldy + n0 + 2 * j + 1, o[1]);
-          }
-        } else if (p.ydt == MTC_F32) {
-          // 64 columns fill a staged row
+          for (int c = 0; c < 8; ++c) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c) bulk_wait_read();
-#pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              *reinterpret_cast<ulonglong2*>(my_row + 8 * j) = make_ulonglong2(acc[32 * c + j], acc[32 * c + j + 1]);
-            store_row(y + 256 * c, my_row, 4 * (left - 64 * c), row_ok);
+            for (int j = 0; j < 8; j += 2)
+              *reinterpret_cast<ulonglong2*>(my_row + 8 * j) = make_ulonglong2(acc[8 * c + j], acc[8 * c + j + 1]);
+            if (p.vec) {
+              store_rows(y + 64 * c, ldy, staging + warp * kStaging, lane, 4 * (left - 16 * c), rows);
+            } else if (lane < rows) {
+#pragma unroll 1
+              for (int j = 0; j < min(16, left - 16 * c); ++j)
+                store1(y + lane * ldy, p.ydt, 16 * c + j, reinterpret_cast<const float*>(my_row)[j]);
+            }
           }
         } else {
+          // 16-bit outputs, 32 columns at a time
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            uint32_t w[4];
+          for (int c = 0; c < 4; ++c) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float o[2];
-              unpair(acc[4 * c + j], o[0], o[1]);
-              w[j] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[0], o[1]) : pack2(MTC_F16, o[0], o[1]);
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float o[2];
+                unpair(acc[16 * c + 4 * i + j], o[0], o[1]);
+                w[j] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[0], o[1]) : pack2(MTC_F16, o[0], o[1]);
+              }
+              *reinterpret_cast<uint4*>(my_row + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            *reinterpret_cast<uint4*>(my_row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+            store_rows(y + 64 * c, ldy, staging + warp * kStaging, lane, 2 * (left - 32 * c), rows);
           }
-          store_row(y, my_row, 2 * left, row_ok);
         }
       }
     }
-    bulk_wait_all();
   }
 
   __syncwarp();
