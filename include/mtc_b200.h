@@ -430,14 +430,21 @@ enum { MTC_F32 = 0, MTC_BF16 = 1, MTC_F16 = 2 };
  * [E][N][ldk] (one row of K codes per output feature, ldk a multiple of 16,
  * 16-byte aligned), scales as [E][ceil(N/128)][ceil(K/128)], one fp32 scale
  * per 128 x 128 block.  W[e][k][n] = code[e][n][k] * scale[e][n/128][k/128].
- * A NaN code makes the outputs of its feature NaN. */
+ * A NaN code makes the outputs of its feature NaN.  `map` is the TMA
+ * descriptor of `codes`, filled by mtc_fp8_matrix_init (map_ready = 1); with
+ * map_ready = 0 every product encodes its own. */
 typedef struct mtc_fp8_matrix {
   const uint8_t* codes;
   const float* scales;
   int64_t ldk;
   int32_t E, K, N;
-  int32_t pad_;
+  int32_t map_ready;
+  uint64_t map[16];
 } mtc_fp8_matrix;
+
+/* Checks the fields and fills `map` (host only; to be repeated when `codes`
+ * or a size changes). */
+MTC_API int mtc_fp8_matrix_init(mtc_fp8_matrix* w);
 
 /* W (K x N fp32, row stride ldw) to codes and scales of one matrix: per block
  * amax = max(max|w|, 2^-100), scale = amax / 448, code = e4m3(w * (448 /

@@ -81,10 +81,10 @@ class FP8Desc(ctypes.Structure):
     """struct mtc_fp8_matrix: E stacked K x N matrices of e4m3 codes."""
 
     _fields_ = [("codes", c_p), ("scales", c_p), ("ldk", c_i64), ("E", c_i32), ("K", c_i32), ("N", c_i32),
-                ("pad_", c_i32)]
+                ("map_ready", c_i32), ("map", c_u64 * 16)]
 
 
-assert ctypes.sizeof(FP8Desc) == 40
+assert ctypes.sizeof(FP8Desc) == 168
 _FP8 = ctypes.POINTER(FP8Desc)
 F32, BF16, F16 = 0, 1, 2
 SCORES = {"softmax": 0, "sigmoid": 1}
@@ -125,6 +125,7 @@ SIGNATURES = {
     "mtc_prefill_gemm": (c_i32, [ctypes.POINTER(StreamDesc), c_i32, c_p, c_i64, c_i32, c_p, c_size, c_p, _EP,
                                  c_p]),
     "mtc_prefill_scatter": (c_i32, [ctypes.POINTER(StreamDesc), c_i32, c_p, c_p, c_i64, c_p, c_size, _EP, c_p]),
+    "mtc_fp8_matrix_init": (c_i32, [_FP8]),
     "mtc_fp8_pack": (c_i32, [c_p, c_i32, c_i32, c_i64, c_p, c_i64, c_p, c_p]),
     "mtc_fp8_unpack": (c_i32, [_FP8, c_i32, c_p, c_i64, c_p]),
     "mtc_fp8_quantize": (c_i32, [c_p, c_i32, c_i32, c_i32, c_i64, c_p, c_i64, c_p, c_i64, c_p]),

@@ -41,6 +41,8 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   extern __shared__ double route_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * (blockDim.x >> 5) + warp;
+  griddep_wait();
+  griddep_launch_dependents();
   if (t >= p.T) return;
   const T* z = reinterpret_cast<const T*>(p.logits) + t * p.ld;
   float v[NPL];
@@ -204,6 +206,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < 32 * p.E; i += kPlanThreads) hist[i] = 0;
   __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
   const int piece = (((p.R + 31) >> 5) + 31) & ~31;
   const int r0 = min((long long)warp * piece, (long long)p.R), r1 = min(r0 + piece, p.R);
   int32_t* mine = hist + warp * p.E;
@@ -271,6 +275,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
   const int t = blockIdx.x;
   __shared__ int at[kMaxTopK];
   __shared__ float w[kMaxTopK];
+  griddep_wait();
+  griddep_launch_dependents();
   if (threadIdx.x < p.k) {
     at[threadIdx.x] = p.pos[(long long)t * p.k + threadIdx.x];
     w[threadIdx.x] = p.weights[(long long)t * p.k + threadIdx.x];
@@ -368,8 +374,8 @@ int launch_route(const RouteParams& p, cudaStream_t st) {
     if (smem > 48 * 1024)
       MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                      "mtc_route_experts");
-    kernel<<<(p.T + warps - 1) / warps, 32 * warps, smem, st>>>(p);
-    MTC_CHECK_LAUNCH("mtc_route_experts");
+    MTC_CHECK_CUDA(launch_chained(kernel, dim3((p.T + warps - 1) / warps), dim3(32 * warps), smem, st, 1, p),
+                   "mtc_route_experts");
     return MTC_OK;
   };
   if (p.E <= 32) return go(route_kernel<T, 1>);
@@ -465,8 +471,7 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
     const size_t smem = (size_t)32 * E * 4;
     if (smem > 48 * 1024)
       MTC_CHECK_CUDA(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-    plan_kernel<<<1, kPlanThreads, smem, st>>>(p);
-    MTC_CHECK_LAUNCH(who);
+    MTC_CHECK_CUDA(launch_chained(plan_kernel, dim3(1), dim3(kPlanThreads), smem, st, 1, p), who);
   }
   Product a;
   a.w[0] = gate;
@@ -482,6 +487,7 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   Product b = a;
   b.w[0] = down;
   b.w[1] = nullptr;
+  b.early = true;  // the plan ran before the first product
   if (!pl.raw) {
     QuantRows q;
     q.X = X;
@@ -554,9 +560,9 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   if (rc != MTC_OK) return rc;
   CombineParams c = {base + pl.out, pl.ldo, pos, weights, T, k, D, Y, ldy, y_type, 0};
   c.vec = (reinterpret_cast<uintptr_t>(Y) & 15) == 0 && ldy % (y_type == MTC_F32 ? 4 : 8) == 0;
-  if (y_type == MTC_F32) combine_kernel<float><<<T, 256, 0, st>>>(c);
-  else if (y_type == MTC_BF16) combine_kernel<__nv_bfloat16><<<T, 256, 0, st>>>(c);
-  else combine_kernel<__half><<<T, 256, 0, st>>>(c);
-  MTC_CHECK_LAUNCH(who);
+  auto kernel = y_type == MTC_F32    ? combine_kernel<float>
+                : y_type == MTC_BF16 ? combine_kernel<__nv_bfloat16>
+                                     : combine_kernel<__half>;
+  MTC_CHECK_CUDA(launch_chained(kernel, dim3(T), dim3(256), 0, st, 1, c), who);
   return MTC_OK;
 }

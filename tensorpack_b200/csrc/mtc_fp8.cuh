@@ -231,18 +231,19 @@ __device__ __forceinline__ void fma2(f32x2& acc, f32x2 v, f32x2 s) {
 // ---------------------------------------------------------------------------
 // Slot list written by the plan kernel for a grouped product: word 0 is the
 // number of slots, slot i is {expert, first row, end row of the expert, 0} at
-// words 4 + 4 i.  A dense product has no list: slot i covers rows from
-// i * size of the single matrix.
+// words 4 + 4 i.  (Read from L2: a product may read it before its predecessor
+// in the stream has ended.)  A dense product has no list: slot i covers rows
+// from i * size of the single matrix.
 struct Slot {
   int e, row0, end;
 };
 __device__ __forceinline__ int slot_count(const int32_t* slots, int M, int size) {
-  return slots ? __ldg(slots) : (M + size - 1) / size;
+  return slots ? __ldcg(slots) : (M + size - 1) / size;
 }
 __device__ __forceinline__ Slot slot_at(const int32_t* slots, int M, int size, int i) {
   Slot s;
   if (slots) {
-    const int4 v = *reinterpret_cast<const int4*>(slots + 4 + 4 * i);
+    const int4 v = __ldcg(reinterpret_cast<const int4*>(slots + 4 + 4 * i));
     s.e = v.x;
     s.row0 = v.y;
     s.end = v.z;

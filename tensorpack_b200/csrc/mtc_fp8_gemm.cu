@@ -18,6 +18,8 @@
 //    between the MMA and eight warps that scale and add.  Bound by the
 //    tensor cores.  kGated: the 256 features are 128 of the gate matrix and
 //    the same 128 of the up matrix; the output is act(gate) * up, quantized.
+#include <string.h>
+
 #include "mtc_fp8.cuh"
 #include "mtc_internal.h"
 #include "mtc_fp8_internal.h"
@@ -69,6 +71,7 @@ struct FewParams {
   const float* bias;
   int act;
   int split;                          // CTAs of a cluster
+  int early;                          // slots and weights may be read before the predecessor ends
   uint32_t* status;
   unsigned long long timeout_ns;
 };
@@ -109,8 +112,12 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = p.split, rank = split > 1 ? (int)tc::cluster_rank() : 0;
+  if (p.slots && !p.early) griddep_wait();
   // every CTA of a cluster has the same blockIdx.y, so a cluster leaves together
-  if ((int)blockIdx.y >= slot_count(p.slots, p.M, BN)) return;
+  if ((int)blockIdx.y >= slot_count(p.slots, p.M, BN)) {
+    griddep_wait();  // no CTA ends before the predecessor has
+    return;
+  }
   const Slot slot = slot_at(p.slots, p.M, BN, blockIdx.y);
   const int ntok = min(BN, slot.end - slot.row0);
   const int t = blockIdx.x / split, mat = t / p.n_tiles, f0 = (t - mat * p.n_tiles) * 128;
@@ -135,6 +142,15 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
+  auto load_weights = [&](int i) {
+    const int s = i % C::kStages;
+    mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : kATile);
+    tc::tma_load_2d(smem + s * C::kStage, mat ? &tw1 : &tw0, (kb0 + i) * 128, slot.e * p.N + f0, &full[s]);
+  };
+  if (p.early && tid == 128)
+    for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i);
+  griddep_wait();
+  griddep_launch_dependents();
 
   float acc[BN];
   if (warp == 4) {
@@ -148,8 +164,7 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
           break;
         }
         uint8_t* st = smem + s * C::kStage;
-        mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : kATile);
-        tc::tma_load_2d(st, mat ? &tw1 : &tw0, (kb0 + i) * 128, slot.e * p.N + f0, &full[s]);
+        if (!p.early || i >= C::kStages) load_weights(i);
         if constexpr (SRC == SRC_CODES) tc::tma_load_2d(st + kATile, &tx, (kb0 + i) * 128, slot.row0, &full[s]);
       }
       if (abort_flag[0]) {
@@ -460,6 +475,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  griddep_wait();
+  griddep_launch_dependents();
   const int n_slots = slot_count(p.slots, p.M, 128);
   const int n_work = n_slots * p.n_tiles;
   if ((int)blockIdx.x >= n_work) return;
@@ -733,22 +750,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 template <int BN, int SRC>
 int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid_x,
                int grid_y, cudaStream_t st, const char* who) {
-  auto kernel = few_kernel<BN, SRC>;
+  static std::atomic<uint64_t> ready{0};
   constexpr size_t smem = FewCfg<BN>::kSmem;
-  MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(grid_x, grid_y, 1);
-  cfg.blockDim = dim3(SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 1 : 0;
-  MTC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw0, tw1, tx, p), who);
+  MTC_CHECK_CUDA(allow_smem(few_kernel<BN, SRC>, smem, ready), who);
+  constexpr int threads = SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps;
+  MTC_CHECK_CUDA(launch_chained(few_kernel<BN, SRC>, dim3(grid_x, grid_y), dim3(threads), smem, st, p.split, tw0, tw1,
+                                tx, p),
+                 who);
+  return MTC_OK;
+}
+
+template <int MODE>
+int launch_many(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const ManyParams& p, int grid,
+                cudaStream_t st, const char* who) {
+  static std::atomic<uint64_t> ready{0};
+  MTC_CHECK_CUDA(allow_smem(many_kernel<MODE>, kManySmem, ready), who);
+  MTC_CHECK_CUDA(launch_chained(many_kernel<MODE>, dim3(grid), dim3(kManyThreads), kManySmem, st, 1, tw0, tw1, tx, p),
+                 who);
   return MTC_OK;
 }
 
@@ -807,10 +825,12 @@ int check_matrix(const mtc_fp8_matrix* w, const char* who) {
 }
 
 int sm_count() {
+  static std::atomic<int> known[64];
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 
@@ -822,11 +842,16 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
   if (a.slot_bound <= 0) return MTC_OK;
   CUtensorMap tw[2], tx;
-  for (int i = 0; i < 2; ++i) {
-    const mtc_fp8_matrix* m = a.w[i] ? a.w[i] : w;
-    const int rc = encode_codes_map(&tw[i], m->codes, m->ldk, m->K, (long long)m->E * m->N, 128, who);
-    if (rc != MTC_OK) return rc;
+  for (int i = 0; i < n_mats; ++i) {
+    const mtc_fp8_matrix* m = a.w[i];
+    if (m->map_ready) {
+      memcpy(&tw[i], m->map, sizeof(CUtensorMap));
+    } else {
+      const int rc = encode_codes_map(&tw[i], m->codes, m->ldk, m->K, (long long)m->E * m->N, 128, who);
+      if (rc != MTC_OK) return rc;
+    }
   }
+  if (n_mats == 1) tw[1] = tw[0];
   tx = tw[0];
   if (a.xq) {
     const int rc = encode_codes_map(&tx, a.xq, a.ldq, w->K, a.rows, a.tile, who);
@@ -857,19 +882,18 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
     p.hs_ld = a.hs_ld;
     p.status = a.status;
     p.timeout_ns = wait_limit_ns();
-    auto kernel = many_kernel<kPlain>;
-    if (n_mats == 2)
-      kernel = a.gate_act == MTC_ACT_RELU   ? many_kernel<kGated + MTC_ACT_RELU>
-               : a.gate_act == MTC_ACT_SILU ? many_kernel<kGated + MTC_ACT_SILU>
-               : a.gate_act == MTC_ACT_NONE ? many_kernel<kGated + MTC_ACT_NONE>
-                                            : many_kernel<kGated + MTC_ACT_GELU_TANH>;
-    else if (a.bias || a.act)
-      kernel = many_kernel<kEpilogue>;
-    MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kManySmem), who);
     const long long work = (long long)a.slot_bound * p.n_tiles;
-    kernel<<<(int)(work < sms ? work : sms), kManyThreads, kManySmem, st>>>(tw[0], tw[1], tx, p);
-    MTC_CHECK_LAUNCH(who);
-    return MTC_OK;
+    const int grid = (int)(work < sms ? work : sms);
+    if (n_mats == 2) {
+      switch (a.gate_act) {
+        case MTC_ACT_RELU: return launch_many<kGated + MTC_ACT_RELU>(tw[0], tw[1], tx, p, grid, st, who);
+        case MTC_ACT_SILU: return launch_many<kGated + MTC_ACT_SILU>(tw[0], tw[1], tx, p, grid, st, who);
+        case MTC_ACT_GELU_TANH: return launch_many<kGated + MTC_ACT_GELU_TANH>(tw[0], tw[1], tx, p, grid, st, who);
+        default: return launch_many<kGated + MTC_ACT_NONE>(tw[0], tw[1], tx, p, grid, st, who);
+      }
+    }
+    if (a.bias || a.act) return launch_many<kEpilogue>(tw[0], tw[1], tx, p, grid, st, who);
+    return launch_many<kPlain>(tw[0], tw[1], tx, p, grid, st, who);
   }
   FewParams p = {};
   p.K = w->K;
@@ -901,6 +925,7 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   int split = 1;
   while (split < 8 && tiles * split * 2 <= 2 * sms && nkb >= 4 * split) split *= 2;
   p.split = split;
+  p.early = a.early;
   const int gx = Nb * n_mats * split;
   MTC_REQUIRE(a.slot_bound <= 65535, "%s: %d token tiles in one launch", who, a.slot_bound);
   if (a.xq) {
@@ -925,3 +950,17 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
 
 }  // namespace fp8
 }  // namespace mtc
+
+extern "C" int mtc_fp8_matrix_init(mtc_fp8_matrix* w) {
+  mtc::clear_error();
+  const int rc = mtc::fp8::check_matrix(w, "mtc_fp8_matrix_init");
+  if (rc != MTC_OK) return rc;
+  static_assert(sizeof(CUtensorMap) == sizeof(w->map), "TMA descriptor size");
+  CUtensorMap map;
+  const int re = mtc::fp8::encode_codes_map(&map, w->codes, w->ldk, w->K, (long long)w->E * w->N, 128,
+                                            "mtc_fp8_matrix_init");
+  if (re != MTC_OK) return re;
+  memcpy(w->map, &map, sizeof(map));
+  w->map_ready = 1;
+  return MTC_OK;
+}

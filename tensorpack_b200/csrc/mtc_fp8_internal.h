@@ -2,6 +2,9 @@
 // points.
 #pragma once
 
+#include <atomic>
+#include <utility>
+
 #include "mtc_internal.h"
 
 namespace mtc {
@@ -41,11 +44,52 @@ struct Product {
   long long ldh = 0;
   float* hs = nullptr;
   long long hs_ld = 0;
+  bool early = false;                               // the weights (and slots) may be read before the predecessor ends
   uint32_t* status = nullptr;
 };
 
 int check_matrix(const mtc_fp8_matrix* w, const char* who);
 int sm_count();
+
+// Launch with programmatic stream serialization: the kernel may start while
+// its predecessor in the stream still runs.  Every kernel launched like this
+// calls griddep_wait() before its first access to global memory that the
+// predecessor may have written or still reads, and
+// griddep_launch_dependents() only after that: so whatever was enqueued
+// before the predecessor has completed when a kernel starts, and may be read
+// before its griddep_wait().
+template <typename... Params, typename... Args>
+cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster,
+                           Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// The dynamic shared-memory limit of a kernel, raised once per device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 int launch_product(const Product& a, cudaStream_t st, const char* who);
 
 // Rows of activations (or of fp32 {gate, up}) to codes and scales; with `pos`

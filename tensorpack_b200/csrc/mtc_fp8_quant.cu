@@ -25,6 +25,8 @@ struct QuantParams {
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
+  griddep_wait();
+  griddep_launch_dependents();
   const int rows = p.n_rows ? min(p.M, *p.n_rows) : p.M;
   const long long groups = (long long)rows * p.Kb;
   const long long step = (long long)gridDim.x * 16;
@@ -136,11 +138,11 @@ int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
   const int sms = sm_count();
   MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
   const int grid = (int)(blocks < 8ll * sms ? blocks : 8ll * sms);
-  if (a.gated) quantize_kernel<float, true><<<grid, 256, 0, st>>>(p);
-  else if (a.dt == MTC_F32) quantize_kernel<float, false><<<grid, 256, 0, st>>>(p);
-  else if (a.dt == MTC_BF16) quantize_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(p);
-  else quantize_kernel<__half, false><<<grid, 256, 0, st>>>(p);
-  MTC_CHECK_LAUNCH(who);
+  auto kernel = a.gated             ? quantize_kernel<float, true>
+                : a.dt == MTC_F32   ? quantize_kernel<float, false>
+                : a.dt == MTC_BF16  ? quantize_kernel<__nv_bfloat16, false>
+                                    : quantize_kernel<__half, false>;
+  MTC_CHECK_CUDA(launch_chained(kernel, dim3(grid), dim3(256), 0, st, 1, p), who);
   return MTC_OK;
 }
 
@@ -285,6 +287,7 @@ extern "C" int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_ty
     a.ldq = q.ldq;
     a.sx = q.s;
     a.lds = q.lds;
+    a.early = true;
   }
   return launch_product(a, st, "mtc_fp8_gemm");
 }

@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .fp8 import _TYPES, FP8Experts, _ld, _on, _output, _rows, _stream
+from .fp8 import _TYPES, FP8Experts, _check_output, _current_device, _ld, _raw_stream, _rows
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
@@ -49,18 +49,23 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     if not 1 <= top_k <= min(MAX_TOP_K, top_groups * (E // n_groups)):
         raise ValueError(f"route_experts: top_k={top_k} outside 1..{min(MAX_TOP_K, top_groups * (E // n_groups))}")
     dev = logits.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return route_experts(logits, top_k, score=score, bias=bias, n_groups=n_groups, top_groups=top_groups,
+                                 renormalize=renormalize, scale=scale)
     if bias is not None:
         bias = torch.as_tensor(bias, dtype=torch.float32, device=dev).reshape(-1).contiguous()
         if bias.numel() != E:
             raise ValueError(f"route_experts: bias has {bias.numel()} values, there are {E} experts")
-    ids = torch.empty(T, top_k, dtype=torch.int32, device=dev)
-    weights = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    ids = logits.new_empty((T, top_k), dtype=torch.int32)
+    weights = logits.new_empty((T, top_k), dtype=torch.float32)
     if T:
-        with _on(dev):
-            _lib.check(_lib.load().mtc_route_experts(
-                logits.data_ptr(), _TYPES[logits.dtype], T, E, _ld(logits), top_k, _lib.SCORES[score],
-                None if bias is None else bias.data_ptr(), n_groups, top_groups, int(bool(renormalize)), scale,
-                ids.data_ptr(), weights.data_ptr(), _stream(dev)), "route experts")
+        rc = _lib.load().mtc_route_experts(
+            logits.data_ptr(), _TYPES[logits.dtype], T, E, _ld(logits), top_k, _lib.SCORES[score],
+            None if bias is None else bias.data_ptr(), n_groups, top_groups, bool(renormalize), scale, ids.data_ptr(),
+            weights.data_ptr(), _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "route experts")
     return ids, weights
 
 
@@ -80,6 +85,9 @@ def experts_forward(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, g
     for m in (gate, up, down):
         if not isinstance(m, FP8Experts) or len(m.shape) != 3:
             raise TypeError("experts_forward: gate, up and down must be FP8Experts")
+    if _current_device() != X.device.index:
+        with torch.cuda.device(X.device):
+            return experts_forward(X, ids, weights, gate, up, down, activation=activation, Y=Y, out_dtype=out_dtype)
     T, D = X.shape
     E, K, I = gate.shape
     dev = X.device
@@ -101,18 +109,30 @@ def experts_forward(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, g
             torch.int32)
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r} (one of relu, silu, gelu_tanh)")
-    ids, weights = ids.contiguous(), weights.to(torch.float32).contiguous()
+    if weights.dtype != torch.float32:
+        weights = weights.to(torch.float32)
+    ids, weights = ids.contiguous(), weights.contiguous()
     k = ids.shape[1]
-    Y = _output(Y, (T, D), out_dtype, dev, (X, ids, weights), "experts_forward")
+    if Y is None:
+        if out_dtype is None:
+            out_dtype = torch.float32
+        elif out_dtype not in _TYPES:
+            raise ValueError(f"experts_forward: output type {out_dtype} (one of float32, bfloat16, float16)")
+        Y, ldy = X.new_empty((T, D), dtype=out_dtype), D
+    else:
+        _check_output(Y, (T, D), out_dtype, dev, (X, ids, weights), "experts_forward")
+        ldy = Y.stride(0) if T > 1 else D
     if T:
         lib = _lib.load()
-        with _on(dev):
-            need = lib.mtc_experts_workspace_bytes(gate._ref, T, k, _TYPES[Y.dtype])
-            if not need:
-                raise ValueError(f"experts_forward: too many rows ({T} x {k})")
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            _lib.check(lib.mtc_experts_forward(
-                gate._ref, up._ref, down._ref, X.data_ptr(), _TYPES[X.dtype], T, _ld(X), ids.data_ptr(),
-                weights.data_ptr(), k, _lib.ACTIVATIONS[activation], Y.data_ptr(), _TYPES[Y.dtype],
-                Y.stride(0) if T > 1 else D, ws.data_ptr(), need, gate.status.data_ptr(), _stream(dev)), "experts")
+        y_type = _TYPES[Y.dtype]
+        need = lib.mtc_experts_workspace_bytes(gate._ref, T, k, y_type)
+        if not need:
+            raise ValueError(f"experts_forward: too many rows ({T} x {k})")
+        ws = X.new_empty(need, dtype=torch.uint8)
+        rc = lib.mtc_experts_forward(
+            gate._ref, up._ref, down._ref, X.data_ptr(), _TYPES[X.dtype], T, _ld(X), ids.data_ptr(),
+            weights.data_ptr(), k, _lib.ACTIVATIONS[activation], Y.data_ptr(), y_type, ldy, ws.data_ptr(), need,
+            gate._status_ptr, _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "experts")
     return Y

@@ -32,6 +32,13 @@ _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _li
 _CODES = torch.float8_e4m3fn
 
 
+# torch.cuda.current_stream builds a Stream object (2 us, as long as a launch);
+# torch's own code generator asks for the bare handle like this.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = torch.cuda.current_device
+
+
 def _cuda_device(device=None) -> torch.device:
     if not torch.cuda.is_available():
         raise RuntimeError("the 8-bit kernels need a CUDA device (B200, sm_100a); none is available")
@@ -41,23 +48,8 @@ def _cuda_device(device=None) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
 
 
-class _on:
-    """The tensor's device as the current one, at no cost when it already is."""
-
-    def __init__(self, dev: torch.device):
-        self.ctx = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-
-
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(dev.index)
 
 
 def _rows(X: torch.Tensor, what: str) -> torch.Tensor:
@@ -65,12 +57,14 @@ def _rows(X: torch.Tensor, what: str) -> torch.Tensor:
     do not overlap."""
     if not isinstance(X, torch.Tensor):
         raise TypeError(f"{what}: unsupported operand type {type(X).__name__}")
-    if X.device.type != "cuda":
+    if not X.is_cuda:
         raise ValueError(f"{what}: activations must be a CUDA tensor (no CPU path)")
     if X.dim() != 2:
         raise ValueError(f"{what}: activations must be a matrix, got shape {tuple(X.shape)}")
     if X.dtype not in _TYPES:
         X = X.float()
+    if X.is_contiguous():
+        return X
     if (X.shape[1] > 1 and X.stride(1) != 1) or (X.shape[0] > 1 and X.stride(0) < X.shape[1]):
         X = X.contiguous()
     return X
@@ -87,16 +81,12 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _output(Y, shape, out_dtype, dev, inputs, what: str) -> torch.Tensor:
-    """The output tensor: a new one, or the caller's after its checks."""
-    if out_dtype is None:
-        out_dtype = torch.float32 if Y is None else Y.dtype
-    if out_dtype not in _TYPES:
-        raise ValueError(f"{what}: output type {out_dtype} (one of float32, bfloat16, float16)")
-    if Y is None:
-        return torch.empty(shape, dtype=out_dtype, device=dev)
-    if tuple(Y.shape) != tuple(shape) or Y.dtype != out_dtype or Y.device != dev:
-        raise ValueError(f"{what}: Y must be a {out_dtype} {tuple(shape)} tensor on {dev}")
+def _check_output(Y, shape, out_dtype, dev, inputs, what: str) -> None:
+    """The caller's output tensor: shape, type, rows, no overlap with an input."""
+    if out_dtype is not None and Y.dtype != out_dtype or Y.dtype not in _TYPES:
+        raise ValueError(f"{what}: Y must be a {out_dtype or 'float32, bfloat16 or float16'} tensor, got {Y.dtype}")
+    if tuple(Y.shape) != tuple(shape) or Y.device != dev:
+        raise ValueError(f"{what}: Y must be a {tuple(shape)} tensor on {dev}")
     if (shape[1] > 1 and Y.stride(1) != 1) or (shape[0] > 1 and Y.stride(0) < shape[1]):
         raise ValueError(f"{what}: Y's rows must be contiguous and must not overlap")
     lo, hi = _span(Y)
@@ -104,7 +94,6 @@ def _output(Y, shape, out_dtype, dev, inputs, what: str) -> torch.Tensor:
         a, b = _span(t)
         if a < hi and lo < b:
             raise ValueError(f"{what}: Y overlaps an input")
-    return Y
 
 
 class FP8Experts:
@@ -141,6 +130,8 @@ class FP8Experts:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.desc = _lib.FP8Desc(codes=store.data_ptr(), scales=self.scales.data_ptr(), ldk=ld, E=E, K=K, N=N)
         self._ref = ctypes.byref(self.desc)
+        _lib.check(_lib.load().mtc_fp8_matrix_init(self._ref), what)
+        self._status_ptr = self.status.data_ptr()
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "FP8Experts":
@@ -161,7 +152,7 @@ class FP8Experts:
         codes = torch.zeros(E, N, ld, dtype=torch.uint8, device=dev)
         scales = torch.empty(E, -(-N // BLOCK), -(-K // BLOCK), dtype=torch.float32, device=dev)
         lib = _lib.load()
-        with _on(dev):
+        with torch.cuda.device(dev):
             for e in range(E):
                 We = Wd[e] if Wd[e].stride(1) == 1 and Wd[e].stride(0) >= N else Wd[e].contiguous()
                 _lib.check(lib.mtc_fp8_pack(We.data_ptr(), K, N, max(We.stride(0), N), codes[e].data_ptr(), ld,
@@ -188,7 +179,7 @@ class FP8Experts:
         E, K, N = self.shape
         out = torch.empty(E, K, N, dtype=torch.float32, device=self.device)
         lib = _lib.load()
-        with _on(self.device):
+        with torch.cuda.device(self.device):
             for e in range(E):
                 _lib.check(lib.mtc_fp8_unpack(self._ref, e, out[e].data_ptr(), N, _stream(self.device)), "fp8 unpack")
         return out
@@ -245,7 +236,7 @@ class FP8Matrix(FP8Experts):
         """The weights as fp32 (K, N): code times scale."""
         K, N = self.shape
         out = torch.empty(K, N, dtype=torch.float32, device=self.device)
-        with _on(self.device):
+        with torch.cuda.device(self.device):
             _lib.check(_lib.load().mtc_fp8_unpack(self._ref, 0, out.data_ptr(), N, _stream(self.device)), "fp8 unpack")
         return out
 
@@ -256,16 +247,21 @@ def fp8_quantize(X: torch.Tensor):
     The tensors are views: rows of codes are padded to a multiple of 16
     bytes, the scales are stored by group (their column stride is M)."""
     X = _rows(X, "fp8_quantize")
+    dev = X.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return fp8_quantize(X)
     M, K = X.shape
     if K < 1:
         raise ValueError("fp8_quantize: rows without values")
     ld, kb = -(-K // 16) * 16, -(-K // BLOCK)
-    codes = torch.empty(M, ld, dtype=_CODES, device=X.device)
-    scales = torch.empty(kb, M, dtype=torch.float32, device=X.device)
+    codes = X.new_empty((M, ld), dtype=_CODES)
+    scales = X.new_empty((kb, M), dtype=torch.float32)
     if M:
-        with _on(X.device):
-            _lib.check(_lib.load().mtc_fp8_quantize(X.data_ptr(), _TYPES[X.dtype], M, K, _ld(X), codes.data_ptr(), ld,
-                                                    scales.data_ptr(), M, _stream(X.device)), "fp8 quantize")
+        rc = _lib.load().mtc_fp8_quantize(X.data_ptr(), _TYPES[X.dtype], M, K, _ld(X), codes.data_ptr(), ld,
+                                          scales.data_ptr(), M, _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "fp8 quantize")
     return codes[:, :K] if ld != K else codes, scales.T
 
 
@@ -280,33 +276,45 @@ def fp8_gemm(X, W: FP8Matrix, bias=None, activation: Optional[str] = None, Y=Non
     if not isinstance(W, FP8Matrix):
         raise TypeError("fp8_gemm: the right operand must be an FP8Matrix")
     dev = W.device
-    was_numpy = isinstance(X, np.ndarray)
-    if was_numpy:
-        X = torch.from_numpy(np.ascontiguousarray(X, dtype=np.float32)).to(dev)
+    if isinstance(X, np.ndarray):
+        Xd = torch.from_numpy(np.ascontiguousarray(X, dtype=np.float32)).to(dev)
+        y = fp8_gemm(Xd, W, bias, activation, Y, out_dtype=out_dtype)
+        W.check_status()
+        return y.float().cpu().numpy()
     X = _rows(X, "fp8_gemm")
     if X.device != dev:
         raise ValueError(f"fp8_gemm: activations on {X.device}, weights on {dev}")
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return fp8_gemm(X, W, bias, activation, Y, out_dtype=out_dtype)
     (M, K), (K2, N) = X.shape, W.shape
     assert K == K2, f"Shape mismatch: {tuple(X.shape)} vs {W.shape}"
+    ep = None
     if bias is not None:
         if not (isinstance(bias, torch.Tensor) and bias.dtype == torch.float32 and bias.device == dev
                 and bias.dim() == 1 and bias.is_contiguous()):
             bias = torch.as_tensor(bias, dtype=torch.float32, device=dev).reshape(-1).contiguous()
-        if bias.numel() != N:
-            raise ValueError(f"bias has {bias.numel()} values, the output {N} columns")
-    ep = epilogue(bias, activation)
-    Y = _output(Y, (M, N), out_dtype, dev, (X,) if bias is None else (X, bias), "fp8_gemm")
+        if bias.shape[0] != N:
+            raise ValueError(f"bias has {bias.shape[0]} values, the output {N} columns")
+    if bias is not None or activation is not None:
+        ep = _ep(epilogue(bias, activation))
+    if Y is None:
+        if out_dtype is None:
+            out_dtype = torch.float32
+        elif out_dtype not in _TYPES:
+            raise ValueError(f"fp8_gemm: output type {out_dtype} (one of float32, bfloat16, float16)")
+        Y, ldy = X.new_empty((M, N), dtype=out_dtype), N
+    else:
+        _check_output(Y, (M, N), out_dtype, dev, (X,) if bias is None else (X, bias), "fp8_gemm")
+        ldy = Y.stride(0) if M > 1 else N
     if M:
         lib = _lib.load()
-        with _on(dev):
-            ws, need = None, 0
-            if M > RAW_MAX_M:
-                need = lib.mtc_fp8_gemm_workspace_bytes(W._ref, M)
-                ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            _lib.check(lib.mtc_fp8_gemm(W._ref, X.data_ptr(), _TYPES[X.dtype], M, _ld(X), Y.data_ptr(),
-                                        _TYPES[Y.dtype], Y.stride(0) if M > 1 else N, None if ws is None else
-                                        ws.data_ptr(), need, W.status.data_ptr(), _ep(ep), _stream(dev)), "fp8 gemm")
-    if was_numpy:
-        W.check_status()
-        return Y.float().cpu().numpy()
+        ws, need = None, 0
+        if M > RAW_MAX_M:
+            need = lib.mtc_fp8_gemm_workspace_bytes(W._ref, M)
+            ws = X.new_empty(need, dtype=torch.uint8)
+        rc = lib.mtc_fp8_gemm(W._ref, X.data_ptr(), _TYPES[X.dtype], M, _ld(X), Y.data_ptr(), _TYPES[Y.dtype], ldy,
+                              None if ws is None else ws.data_ptr(), need, W._status_ptr, ep, _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "fp8 gemm")
     return Y
