@@ -166,7 +166,6 @@ struct PlanParams {
   int32_t* order;        // [R] row (t * k + j) at each sorted place
   int32_t* pos;          // [R] sorted place of each row, -1 for an id outside 0..E-1
   int32_t* slots;        // slot list
-  int32_t* n_rows;       // rows that have an expert
 };
 
 constexpr int kPlanThreads = 1024;
@@ -233,10 +232,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     for (int i = 0; i < ns; ++i)
       *reinterpret_cast<int4*>(p.slots + 4 + 4 * (sl + i)) = make_int4(e, off + i * p.size, off + count, 0);
   }
-  if (threadIdx.x == 0) {
-    p.slots[0] = n_slots;
-    *p.n_rows = total;
-  }
+  if (threadIdx.x == 0) p.slots[0] = n_slots;
   __syncthreads();
   for (int rb = r0; rb < r1; rb += 32) {
     const int r = rb + lane;
@@ -316,13 +312,13 @@ bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16;
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How the experts' products run, from the mean number of rows of an expert:
-// up to 8, 16-row tiles whose tokens the products quantize themselves; up to
-// 96, wider tiles of codes; above, the 128-token kernel.
+// up to 8, 16-row tiles whose tokens the first product quantizes itself; up
+// to 48, wider tiles of codes; above, the 128-token kernel.
 struct ExpertsPlan {
-  int R, tile, slot_bound, slot_expect;
+  int R, tile, slot_bound;
   bool raw, many;
-  long long ldx, ldh, ldg, lds, ldo;
-  size_t order, pos, slots, n_rows, xq, xs, gu, hq, hs, out, bytes;
+  long long ldx, ldh, lds, ldo;
+  size_t order, pos, slots, xq, xs, hq, hs, out, bytes;
 };
 bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   const long long R = (long long)T * k;
@@ -330,17 +326,14 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   pl->R = (int)R;
   const double mean = (double)R / E;
   pl->raw = mean <= 8.0;
-  pl->many = mean > 96.0;
-  pl->tile = pl->raw ? 16 : mean <= 20.0 ? 32 : mean <= 40.0 ? 64 : 128;
+  pl->many = mean > 48.0;
+  pl->tile = pl->raw ? 16 : mean <= 24.0 ? 32 : pl->many ? 128 : 64;
   const long long used = R < E ? R : E;
   long long bound = R / pl->tile + used;
   if (bound > R) bound = R;
   pl->slot_bound = (int)bound;
-  const long long expect = used + (long long)(mean / pl->tile) * E;
-  pl->slot_expect = (int)(expect < bound ? expect : bound);
   pl->ldx = (D + 15) & ~15ll;
   pl->ldh = (I + 15) & ~15ll;
-  pl->ldg = (I + 3) & ~3ll;
   pl->lds = (R + 3) & ~3ll;
   pl->ldo = (D + 7) & ~7ll;
   size_t at = 0;
@@ -352,15 +345,13 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   pl->order = take(4 * (size_t)R);
   pl->pos = take(4 * (size_t)R);
   pl->slots = take(16 * (size_t)(pl->slot_bound + 1));
-  pl->n_rows = take(4);
-  pl->xq = pl->xs = pl->gu = pl->hq = pl->hs = 0;
+  pl->xq = pl->xs = 0;
   if (!pl->raw) {
     pl->xq = take((size_t)R * pl->ldx);
     pl->xs = take((size_t)((D + 127) / 128) * pl->lds * 4);
-    pl->hq = take((size_t)R * pl->ldh);
-    pl->hs = take((size_t)((I + 127) / 128) * pl->lds * 4);
   }
-  if (!pl->many) pl->gu = take((size_t)R * 2 * pl->ldg * 4);
+  pl->hq = take((size_t)R * pl->ldh);
+  pl->hs = take((size_t)((I + 127) / 128) * pl->lds * 4);
   pl->out = take((size_t)R * pl->ldo * (ydt == MTC_F32 ? 4 : 2));
   pl->bytes = at;
   return true;
@@ -464,10 +455,8 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   int32_t* order = reinterpret_cast<int32_t*>(base + pl.order);
   int32_t* pos = reinterpret_cast<int32_t*>(base + pl.pos);
   int32_t* slots = reinterpret_cast<int32_t*>(base + pl.slots);
-  int32_t* n_rows = reinterpret_cast<int32_t*>(base + pl.n_rows);
-  float* gu = reinterpret_cast<float*>(base + pl.gu);
   {
-    PlanParams p = {ids, pl.R, E, pl.tile, order, pos, slots, n_rows};
+    PlanParams p = {ids, pl.R, E, pl.tile, order, pos, slots};
     const size_t smem = (size_t)32 * E * 4;
     if (smem > 48 * 1024)
       MTC_CHECK_CUDA(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
@@ -478,7 +467,6 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   a.w[1] = up;
   a.slots = slots;
   a.slot_bound = pl.slot_bound;
-  a.slot_expect = pl.slot_expect;
   a.rows = pl.R;
   a.tile = pl.tile;
   a.many = pl.many;
@@ -507,52 +495,23 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
     a.ldq = q.ldq;
     a.sx = q.s;
     a.lds = q.lds;
-    b.xq = base + pl.hq;
-    b.ldq = pl.ldh;
-    b.sx = reinterpret_cast<float*>(base + pl.hs);
-    b.lds = pl.lds;
   } else {
     a.X = X;
     a.xdt = x_type;
     a.ldx = ldx;
     a.order = order;
     a.kdiv = k;
-    b.gated_src = true;
-    b.X = gu;
-    b.ldx = 2 * pl.ldg;
-    b.src_off = pl.ldg;
   }
-  if (pl.many) {
-    a.hq = base + pl.hq;
-    a.ldh = pl.ldh;
-    a.hs = reinterpret_cast<float*>(base + pl.hs);
-    a.hs_ld = pl.lds;
-  } else {
-    a.Y = gu;
-    a.ydt = MTC_F32;
-    a.ldy = 2 * pl.ldg;
-    a.mat_off = pl.ldg;
-  }
+  a.hq = base + pl.hq;
+  a.ldh = pl.ldh;
+  a.hs = reinterpret_cast<float*>(base + pl.hs);
+  a.hs_ld = pl.lds;
   rc = launch_product(a, st, who);
   if (rc != MTC_OK) return rc;
-  if (!pl.raw && !pl.many) {
-    QuantRows q;
-    q.X = gu;
-    q.dt = MTC_F32;
-    q.M = pl.R;
-    q.K = I;
-    q.ldx = 2 * pl.ldg;
-    q.gated = true;
-    q.src_off = pl.ldg;
-    q.gate_act = act;
-    q.n_rows = n_rows;
-    q.q = base + pl.hq;
-    q.ldq = pl.ldh;
-    q.s = reinterpret_cast<float*>(base + pl.hs);
-    q.lds = pl.lds;
-    rc = launch_quantize(q, st, who);
-    if (rc != MTC_OK) return rc;
-  }
+  b.xq = a.hq;
+  b.ldq = a.ldh;
+  b.sx = a.hs;
+  b.lds = a.hs_ld;
   b.Y = base + pl.out;
   b.ydt = y_type;
   b.ldy = pl.ldo;

@@ -5,14 +5,16 @@
 //
 // Two kernels, by the number of rows that share a weight tile:
 //
-//  * few_kernel<BN, SRC>: 128 output features x BN <= 128 tokens.  The
+//  * few_kernel<BN, SRC, PAIR>: 128 output features x BN <= 128 tokens.  The
 //    features are the M side of the MMA (TMEM lane = feature), so one token
 //    costs 16 columns instead of 128 rows, and a warp's stores are
-//    consecutive features.  Bound by the weight bytes: each CTA streams its
-//    features' codes once through a TMA ring.  A cluster of up to 8 CTAs
-//    splits the inputs and adds its partial sums through distributed shared
-//    memory in rank order: no workspace, no atomics, the same result every
-//    time.
+//    consecutive features.  Bound by the weight bytes: a persistent CTA per
+//    SM streams its features' codes once through a TMA ring of 200 KB.  When
+//    there are few tiles a cluster of up to 8 CTAs splits the inputs and adds
+//    its partial sums through distributed shared memory in rank order: no
+//    workspace, no atomics, the same result every time.  PAIR: the gate and
+//    up matrices of a gated product side by side; the output is
+//    act(gate) * up, quantized.
 //  * many_kernel<MODE>: 128 tokens x 256 features (TMEM lane = token), one
 //    persistent CTA per SM, two 256-column accumulators that alternate
 //    between the MMA and eight warps that scale and add.  Bound by the
@@ -37,68 +39,117 @@ __device__ __forceinline__ void flag(uint32_t* st, uint32_t bits) {
 // ---------------------------------------------------------------------------
 // few_kernel
 // ---------------------------------------------------------------------------
-enum { SRC_CODES = 0, SRC_ROWS = 1, SRC_GATED = 2 };
+// Where the tokens come from: codes and scales in memory, or activations that
+// six more warps of the kernel quantize on the way (at most 16 rows per tile).
+enum { SRC_CODES = 0, SRC_F32 = 1, SRC_BF16 = 2, SRC_F16 = 3 };
 
-template <int BN>
+template <int BN, bool PAIR>
 struct FewCfg {
-  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
-  static constexpr int kAcc = BN <= 64 ? 4 : 2;        // TMEM accumulators
+  static constexpr int kMats = PAIR ? 2 : 1;
   static constexpr uint32_t kBTile = BN * 128;
-  static constexpr uint32_t kStage = kATile + kBTile;
+  static constexpr uint32_t kStage = kMats * kATile + kBTile;
+  static constexpr int kCols = kMats * BN;              // TMEM columns of one accumulator
+  static constexpr int kAcc = 4;
+  static constexpr uint32_t kRed = 16 * 128 * 4 * kMats;  // staged sums of 16 tokens
+  static constexpr uint32_t kRoom = 227 * 1024 - 1024 - 512 - 1024 - kRed;
+  static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
   static constexpr int kRing = kStages + kAcc;          // slots of in-kernel token scales
   static constexpr uint32_t kBars = kStages * kStage;
-  static constexpr size_t kSmem = 1024 + kBars + 512 + (BN == 16 ? kRing * BN * 4 : 0);
+  static constexpr uint32_t kRedAt = kBars + 512;
+  static constexpr uint32_t kScaleAt = kRedAt + kRed;
+  static constexpr size_t kSmem = 1024 + kScaleAt + (BN == 16 ? kRing * BN * 4 : 0);
+  static_assert(kCols * kAcc <= 512 && kSmem <= 227 * 1024, "TMEM and shared memory of one CTA");
+  static_assert(kMats * BN * 128 * 4 <= kStages * kStage, "a cluster's partial sums fit the stages");
 };
 constexpr int kFewThreads = 192;      // 4 scaling warps, TMA warp, MMA warp
-constexpr int kQuantWarps = 4;        // more when the kernel quantizes its tokens itself
+constexpr int kQuantWarps = 6;        // more when the kernel quantizes its tokens itself
 
 struct FewParams {
-  int K, nkb, N, Nb, n_tiles;         // n_tiles: 128-feature tiles of one matrix
+  int K, nkb, N, Nb;                  // Nb: 128-feature tiles
   const float* sw[2];                 // scales of the matrix (or of gate and up)
   const int32_t* slots;
   int M;
   const float* sx;                    // SRC_CODES: token scales [nkb][lds]
   long long lds;
-  const void* X;                      // SRC_ROWS: activations; SRC_GATED: fp32 {gate, up} rows
-  int xdt, vec;
+  const void* X;                      // else: activations
+  int vec;
   long long ldx;
-  const int32_t* order;               // SRC_ROWS, grouped: row r is token order[r] / kdiv
+  const int32_t* order;               // grouped: row r is token order[r] / kdiv
   int kdiv;
-  int gate_act;
   void* Y;
   int ydt;
-  long long ldy, mat_off;             // matrix i writes at column i * mat_off
+  long long ldy;
   const float* bias;
-  int act;
+  int act;                            // PAIR: of the gate
+  uint8_t* hq;                        // PAIR: codes [row][ldh] and scales [n / 128][hs_ld] of act(gate) * up
+  long long ldh;
+  float* hs;
+  long long hs_ld;
   int split;                          // CTAs of a cluster
   int early;                          // slots and weights may be read before the predecessor ends
   uint32_t* status;
   unsigned long long timeout_ns;
 };
 
-// One group of 128 inputs of one row by a half warp: 8 values per lane.
 template <int SRC>
-__device__ __forceinline__ void load_group(const FewParams& p, long long row, int k, float (&v)[8]) {
-  const int n = p.K - k;
-  if constexpr (SRC == SRC_GATED) {
-    const float* g = reinterpret_cast<const float*>(p.X) + row * p.ldx;
-    float u[8];
-    load8(g + k, n, p.vec, v);
-    load8(g + p.mat_off + k, n, p.vec, u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = epi_act(v[i], p.gate_act) * u[i];
-  } else {
-    if (p.xdt == MTC_F32) load8(reinterpret_cast<const float*>(p.X) + row * p.ldx + k, n, p.vec, v);
-    else if (p.xdt == MTC_BF16) load8(reinterpret_cast<const __nv_bfloat16*>(p.X) + row * p.ldx + k, n, p.vec, v);
-    else load8(reinterpret_cast<const __half*>(p.X) + row * p.ldx + k, n, p.vec, v);
+struct SrcType {
+  typedef float T;
+};
+template <>
+struct SrcType<SRC_BF16> {
+  typedef __nv_bfloat16 T;
+};
+template <>
+struct SrcType<SRC_F16> {
+  typedef __half T;
+};
+
+// Barrier of the four scaling warps; the second form tells all whether any
+// of them passed true.
+__device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool few_sync_or(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
+// Staged values [i][128 features] of the tokens j0 + i * step, i < count, to
+// codes and scales: one half warp per token.  Called by the four scaling warps.
+__device__ __forceinline__ void quantize_staged(const FewParams& p, const float* h, int row0, int j0, int step,
+                                                int count, int f0, int warp, int lane) {
+  const int l = lane & 15;
+#pragma unroll 1
+  for (int i = 2 * warp + (lane >> 4); i < ((count + 7) & ~7); i += 8) {
+    float v[8];
+    const float4 a = *reinterpret_cast<const float4*>(h + i * 128 + 8 * l);
+    const float4 b = *reinterpret_cast<const float4*>(h + i * 128 + 8 * l + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    const GroupScale g = group_scale(half_warp_max(amax8(v)));
+    const uint2 c = codes8(v, g.mul);
+    if (i < count) {
+      const long long row = row0 + j0 + i * step;
+      if (f0 + 8 * l < p.ldh) *reinterpret_cast<uint2*>(p.hq + row * p.ldh + f0 + 8 * l) = c;
+      if (l == 0) p.hs[(long long)(f0 >> 7) * p.hs_ld + row] = g.scale;
+    }
   }
 }
 
-template <int BN, int SRC>
-__global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps, 2)
+// Persistent: CTAs (or clusters, which then have one work item each) take the
+// items slot + n_slots * feature tile in turn, so that neighbours in time
+// share weights, and the TMA warp runs ahead over their boundaries.
+template <int BN, int SRC, bool PAIR>
+__global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps, 1)
     few_kernel(const __grid_constant__ CUtensorMap tw0, const __grid_constant__ CUtensorMap tw1,
                const __grid_constant__ CUtensorMap tx, const FewParams p) {
-  using C = FewCfg<BN>;
+  using C = FewCfg<BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
@@ -108,19 +159,12 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
   uint64_t* drain = acc_empty + C::kAcc;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + 1);
   uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
-  float* sring = reinterpret_cast<float*>(smem + C::kBars + 512);
+  float* red = reinterpret_cast<float*>(smem + C::kRedAt);
+  float* sring = reinterpret_cast<float*>(smem + C::kScaleAt);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = p.split, rank = split > 1 ? (int)tc::cluster_rank() : 0;
-  if (p.slots && !p.early) griddep_wait();
-  // every CTA of a cluster has the same blockIdx.y, so a cluster leaves together
-  if ((int)blockIdx.y >= slot_count(p.slots, p.M, BN)) {
-    griddep_wait();  // no CTA ends before the predecessor has
-    return;
-  }
-  const Slot slot = slot_at(p.slots, p.M, BN, blockIdx.y);
-  const int ntok = min(BN, slot.end - slot.row0);
-  const int t = blockIdx.x / split, mat = t / p.n_tiles, f0 = (t - mat * p.n_tiles) * 128;
+  const int cid = blockIdx.x / split, n_cid = gridDim.x / split;
   const int kb0 = (int)((long long)rank * p.nkb / split), kb1 = (int)((long long)(rank + 1) * p.nkb / split);
   const int n_it = kb1 - kb0;
 
@@ -137,39 +181,52 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     abort_flag[0] = 0;
     fence_barrier_init();
   }
-  if (warp == 5) tc::tmem_alloc(tmem_slot, C::kAcc * BN);
+  if (warp == 5) tc::tmem_alloc(tmem_slot, C::kAcc * C::kCols);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto load_weights = [&](int i) {
-    const int s = i % C::kStages;
-    mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : kATile);
-    tc::tma_load_2d(smem + s * C::kStage, mat ? &tw1 : &tw0, (kb0 + i) * 128, slot.e * p.N + f0, &full[s]);
+  if (!p.early) griddep_wait();
+  const int n_slots = slot_count(p.slots, p.M, BN), n_items = n_slots * p.Nb;
+  auto load_weights = [&](int s, const Slot& slot, int f0, int kb) {
+    mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : C::kStage - C::kBTile);
+    tc::tma_load_2d(smem + s * C::kStage, &tw0, kb * 128, slot.e * p.N + f0, &full[s]);
+    if constexpr (PAIR) tc::tma_load_2d(smem + s * C::kStage + kATile, &tw1, kb * 128, slot.e * p.N + f0, &full[s]);
   };
-  if (p.early && tid == 128)
-    for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i);
-  griddep_wait();
+  if (p.early) {
+    if (tid == 128 && cid < n_items) {
+      const Slot slot = slot_at(p.slots, p.M, BN, cid % n_slots);
+      for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i, slot, cid / n_slots * 128, kb0 + i);
+    }
+    griddep_wait();
+  }
   griddep_launch_dependents();
 
-  float acc[BN];
+  float acc[C::kCols];
   if (warp == 4) {
     // ------------------------------------------------------------ weights (and codes of the tokens) by TMA
     if (lane == 0) {
-      int i = 0;
-      for (; i < n_it && !abort_flag[0]; ++i) {
-        const int s = i % C::kStages;
-        if (i >= C::kStages && !mbar_wait(&empty[s], ((i / C::kStages) & 1) ^ 1, p.timeout_ns)) {
-          abort_flag[0] = 1;
-          break;
+      uint32_t it = 0;
+      Slot next = {};
+      if (cid < n_items) next = slot_at(p.slots, p.M, BN, cid % n_slots);  // one item ahead
+      for (int w = cid; w < n_items && !abort_flag[0]; w += n_cid) {
+        const Slot slot = next;
+        if (w + n_cid < n_items) next = slot_at(p.slots, p.M, BN, (w + n_cid) % n_slots);
+        const int f0 = w / n_slots * 128;
+        for (int i = 0; i < n_it; ++i, ++it) {
+          const int s = it % C::kStages;
+          if (it >= C::kStages && !mbar_wait(&empty[s], ((it / C::kStages) & 1) ^ 1, p.timeout_ns)) {
+            abort_flag[0] = 1;
+            break;
+          }
+          if (!p.early || it >= C::kStages || w != cid) load_weights(s, slot, f0, kb0 + i);
+          if constexpr (SRC == SRC_CODES)
+            tc::tma_load_2d(smem + s * C::kStage + C::kMats * kATile, &tx, (kb0 + i) * 128, slot.row0, &full[s]);
         }
-        uint8_t* st = smem + s * C::kStage;
-        if (!p.early || i >= C::kStages) load_weights(i);
-        if constexpr (SRC == SRC_CODES) tc::tma_load_2d(st + kATile, &tx, (kb0 + i) * 128, slot.row0, &full[s]);
       }
       if (abort_flag[0]) {
         // this CTA's copies in flight must land before it leaves
-        for (int j = i > C::kStages ? i - C::kStages : 0; j < i; ++j)
+        for (uint32_t j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
           (void)mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, 10000000ull);
         flag(p.status, MTC_STATUS_TIMEOUT);
       }
@@ -178,21 +235,26 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     // ------------------------------------------------------------ MMA
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_e4m3_f32(128, BN);
-      for (int i = 0; i < n_it && !abort_flag[0]; ++i) {
-        const int s = i % C::kStages, b = i % C::kAcc;
-        if (!mbar_wait(&full[s], (i / C::kStages) & 1, p.timeout_ns) ||
-            (i >= C::kAcc && !mbar_wait(&acc_empty[b], ((i / C::kAcc) & 1) ^ 1, p.timeout_ns))) {
-          abort_flag[0] = 1;
-          break;
-        }
-        tc::fence_after();
-        const uint32_t a0 = smem_u32(smem + s * C::kStage), b0 = a0 + kATile;
+      uint32_t it = 0;
+      for (int w = cid; w < n_items && !abort_flag[0]; w += n_cid) {
+        for (int i = 0; i < n_it; ++i, ++it) {
+          const int s = it % C::kStages, b = it % C::kAcc;
+          if (!mbar_wait(&full[s], (it / C::kStages) & 1, p.timeout_ns) ||
+              (it >= C::kAcc && !mbar_wait(&acc_empty[b], ((it / C::kAcc) & 1) ^ 1, p.timeout_ns))) {
+            abort_flag[0] = 1;
+            break;
+          }
+          tc::fence_after();
+          const uint32_t a0 = smem_u32(smem + s * C::kStage), b0 = a0 + C::kMats * kATile;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma_e4m3_ss(tmem + b * BN, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
-                      j > 0);
-        tc::commit(&acc_full[b]);
-        tc::commit(&empty[s]);
+          for (int m = 0; m < C::kMats; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma_e4m3_ss(tmem + b * C::kCols + m * BN, tc::smem_desc_k_sw128(a0 + m * kATile + 32 * j),
+                          tc::smem_desc_k_sw128(b0 + 32 * j), idesc, j > 0);
+          tc::commit(&acc_full[b]);
+          tc::commit(&empty[s]);
+        }
       }
       if (abort_flag[0]) {
         // no MMA may read shared memory or write TMEM after this CTA has left
@@ -202,148 +264,248 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     }
   } else if (warp < 4) {
     // ------------------------------------------------------------ scale and add
-    const float* swp = p.sw[mat] + ((long long)slot.e * p.Nb + (f0 >> 7)) * p.nkb + kb0;
-    constexpr int kCols = (BN + 31) / 32;
+    constexpr int kLanes = (BN + 31) / 32;  // tokens per lane
+    const int feat = 32 * warp + lane;
+    uint32_t it = 0;
+    for (int w = cid; w < n_items; w += n_cid) {
+      const Slot slot = slot_at(p.slots, p.M, BN, w % n_slots);
+      const int ft = w / n_slots, ntok = min(BN, slot.end - slot.row0);
+      const float* swp[C::kMats];
 #pragma unroll
-    for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
-    // The next block's scales, columns lane, lane + 32, ...; multiplied where
-    // they are used, so that nothing waits for the loads before that.
-    float sn[kCols], wn;
-    auto load_scales = [&](int i) {
-      wn = __ldg(swp + i);
+      for (int m = 0; m < C::kMats; ++m) swp[m] = p.sw[m] + ((long long)slot.e * p.Nb + ft) * p.nkb + kb0;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const int m = 32 * c + lane;
-        if constexpr (SRC == SRC_CODES) sn[c] = m < ntok ? p.sx[(long long)(kb0 + i) * p.lds + slot.row0 + m] : 0.0f;
+      for (int j = 0; j < C::kCols; ++j) acc[j] = 0.0f;
+      // The next block's scales, tokens lane, lane + 32, ...; multiplied
+      // where they are used, so that nothing waits for the loads before that.
+      float sn[kLanes], wn[C::kMats];
+      auto load_scales = [&](int i) {
+#pragma unroll
+        for (int m = 0; m < C::kMats; ++m) wn[m] = __ldg(swp[m] + i);
+#pragma unroll
+        for (int c = 0; c < kLanes; ++c) {
+          const int t = 32 * c + lane;
+          if constexpr (SRC == SRC_CODES)
+            sn[c] = t < ntok ? p.sx[(long long)(kb0 + i) * p.lds + slot.row0 + t] : 0.0f;
+        }
+      };
+      load_scales(0);
+      bool ok = true;
+#pragma unroll 1
+      for (int i = 0; i < n_it; ++i, ++it) {
+        const int b = it % C::kAcc;
+        float sc[kLanes], wc[C::kMats];
+#pragma unroll
+        for (int c = 0; c < kLanes; ++c) sc[c] = SRC == SRC_CODES ? sn[c] : 0.0f;
+#pragma unroll
+        for (int m = 0; m < C::kMats; ++m) wc[m] = wn[m];
+        if (i + 1 < n_it) load_scales(i + 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (it / C::kAcc) & 1, p.timeout_ns))) {
+          abort_flag[0] = 1;
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+        // the quantizing warps wrote this block's token scales before its MMA ran
+        if constexpr (SRC != SRC_CODES) sc[0] = sring[(it % C::kRing) * BN + (lane & (BN - 1))];
+        const uint32_t ta = tmem + b * C::kCols + ((uint32_t)(32 * warp) << 16);
+#pragma unroll
+        for (int c = 0; c < C::kCols / 16; ++c) {
+          uint32_t v[16];
+          tmem_ld16(ta + 16 * c, v);
+          tmem_wait16(v);
+          if (c == C::kCols / 16 - 1) {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+          }
+          const int m = 16 * c / BN, t0 = 16 * c - m * BN;
+          const float sm = sc[t0 / 32] * wc[m];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float s = __shfl_sync(0xffffffffu, sm, (t0 + j) & 31);
+            acc[16 * c + j] = fmaf(__uint_as_float(v[j]), s, acc[16 * c + j]);
+          }
+        }
       }
-    };
-    load_scales(0);
-    for (int i = 0; i < n_it; ++i) {
-      const int b = i % C::kAcc;
-      float sc[kCols];
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) sc[c] = SRC == SRC_CODES ? sn[c] * wn : wn;
-      if (i + 1 < n_it) load_scales(i + 1);
-      if (!__all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(&acc_full[b], (i / C::kAcc) & 1, p.timeout_ns))) {
-        abort_flag[0] = 1;
+      if (split > 1) break;  // one item per cluster; its sums are completed below
+      // The sums go to shared memory, 16 tokens at a time, and are finished
+      // in loops (the epilogue's code once, not once per token: unrolled, its
+      // instruction fetches took longer than the product).
+      const int f0 = 128 * ft, n = f0 + feat;
+      if constexpr (PAIR) {
+        if (few_sync_or(!ok)) break;
+      } else if (!ok) {
         break;
       }
-      tc::fence_after();
-      // the quantizing warps wrote this block's token scales before its MMA ran
-      if constexpr (SRC != SRC_CODES) sc[0] *= sring[(i % C::kRing) * BN + (lane & (BN - 1))];
-      uint32_t v[2][16];
-      const uint32_t ta = tmem + b * BN + ((uint32_t)(32 * warp) << 16);
-      tmem_ld16(ta, v[0]);
+      const float bias = (!PAIR && p.bias && n < p.N) ? __ldg(p.bias + n) : 0.0f;
 #pragma unroll
       for (int c = 0; c < BN / 16; ++c) {
-        tmem_wait16(v[c & 1]);
-        if (c + 1 < BN / 16) {
-          tmem_ld16(ta + 16 * (c + 1), v[(c + 1) & 1]);
-        } else {
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[b]);
-        }
+        if (16 * c < ntok) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float s = __shfl_sync(0xffffffffu, sc[(16 * c + j) / 32], (16 * c + j) & 31);
-          acc[16 * c + j] = fmaf(__uint_as_float(v[c & 1][j]), s, acc[16 * c + j]);
+          for (int j = 0; j < 16; ++j) {
+            red[j * 128 + feat] = acc[16 * c + j];
+            if constexpr (PAIR) red[(16 + j) * 128 + feat] = acc[BN + 16 * c + j];
+          }
+          const int count = min(16, ntok - 16 * c);
+          if constexpr (PAIR) {
+#pragma unroll 1
+            for (int j = 0; j < count; ++j)
+              red[j * 128 + feat] = n < p.N ? epi_act(red[j * 128 + feat], p.act) * red[(16 + j) * 128 + feat] : 0.0f;
+            few_sync();
+            quantize_staged(p, red, slot.row0, 16 * c, 1, count, f0, warp, lane);
+            few_sync();
+          } else if (n < p.N) {
+#pragma unroll 1
+            for (int j = 0; j < count; ++j) {
+              const float a = red[j * 128 + feat] + bias;
+              store1(p.Y, p.ydt, (slot.row0 + 16 * c + j) * p.ldy + n, p.act ? epi_act(a, p.act) : a);
+            }
+          }
         }
       }
     }
   } else if constexpr (SRC != SRC_CODES) {
-    // ------------------------------------------------------------ quantize the tokens: warp w takes blocks w, w + 4, ...
+    // ------------------------------------------------------------ quantize the tokens: warp q takes iterations q, q + 6, ...
     static_assert(SRC == SRC_CODES || BN == 16, "in-kernel quantization serves 16 tokens");
-    const int qw = warp - 6, half = lane >> 4, l = lane & 15;
-    const int rounds = (ntok + 1) >> 1;
-    for (int i = qw; i < n_it; i += kQuantWarps) {
-      const int s = i % C::kStages;
-      const int k = (kb0 + i) * 128 + 8 * l;
-      bool waited = false;
-      for (int r0 = 0; r0 < rounds; r0 += 4) {
-        float v[4][8];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int m = 2 * (r0 + r) + half;
-          if (m < ntok) {
-            long long row = slot.row0 + m;
-            if (SRC == SRC_ROWS && p.order) row = p.order[row] / p.kdiv;
-            load_group<SRC>(p, row, k, v[r]);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[r][q] = 0.0f;
-          }
+    // A warp at iteration i has seen the MMA of i - kQuantWarps - kStages
+    // complete; that must cover i - 2 kStages, or the parity it waits for
+    // would be that of the phase before.
+    static_assert(SRC == SRC_CODES || kQuantWarps <= C::kStages, "a quantizing warp may not lap the stages");
+    typedef typename SrcType<SRC>::T T;
+    const int half = lane >> 4, l = lane & 15;
+    uint32_t it = 0, mine = warp - 6;
+    bool ok = true;
+    for (int w = cid; w < n_items && ok; w += n_cid) {
+      const Slot slot = slot_at(p.slots, p.M, BN, w % n_slots);
+      const int ntok = min(BN, slot.end - slot.row0);
+      const uint32_t end = it + n_it;
+      if (mine < end) {
+        // lane m < 16 knows where row m is
+        long long at = 0;
+        if (l < ntok) {
+          at = slot.row0 + l;
+          if (p.order) at = p.order[at] / p.kdiv;
+          at *= p.ldx;
         }
-        if (!waited) {
-          waited = true;
-          if (i >= C::kStages &&
-              !__all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / C::kStages) & 1) ^ 1, p.timeout_ns)))
-            abort_flag[0] = 1;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int m = 2 * (r0 + r) + half;
-          const GroupScale g = group_scale(half_warp_max(amax8(v[r])));
-          const uint2 c = codes8(v[r], g.mul);
-          if (m < BN) {
+        for (; mine < end; mine += kQuantWarps) {
+          const int s = mine % C::kStages, k0 = (kb0 + (int)(mine - it)) * 128, k = k0 + 8 * l;
+          uint8_t* tile = smem + s * C::kStage + C::kMats * kATile;
+          auto put = [&](int m, const float (&v)[8]) {
+            const GroupScale g = group_scale(half_warp_max(amax8(v)));
+            const uint2 c = codes8(v, g.mul);
             // row m of the K-major SWIZZLE_128B tile: 16-byte chunk j sits at chunk j ^ (m % 8)
-            uint8_t* dst = smem + s * C::kStage + kATile + m * 128 + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8;
-            *reinterpret_cast<uint2*>(dst) = c;
-            if (l == 0) sring[(i % C::kRing) * BN + m] = g.scale;
+            *reinterpret_cast<uint2*>(tile + m * 128 + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8) = c;
+            if (l == 0) sring[(mine % C::kRing) * BN + m] = g.scale;
+          };
+          auto stage_free = [&]() -> bool {
+            return __all_sync(0xffffffffu, mine < C::kStages ||
+                                               mbar_wait(&empty[s], ((mine / C::kStages) & 1) ^ 1, p.timeout_ns));
+          };
+          if (p.vec && k0 + 128 <= p.K) {
+            // all loads of (half) a block in flight before the first value is used
+            constexpr int kVec = sizeof(T) == 4 ? 2 : 1, kRounds = 8 / kVec;
+#pragma unroll
+            for (int r0 = 0; r0 < 8; r0 += kRounds) {
+              if (2 * r0 < ntok) {
+                uint4 raw[kRounds][kVec];
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) {
+                  const int m = 2 * (r0 + r) + half;
+                  const long long row = __shfl_sync(0xffffffffu, at, m);
+#pragma unroll
+                  for (int q = 0; q < kVec; ++q)
+                    raw[r][q] = m < ntok ? *(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.X) + row + k) + q)
+                                         : make_uint4(0u, 0u, 0u, 0u);
+                }
+                if (r0 == 0 && !stage_free()) ok = false;
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) {
+                  const int m = 2 * (r0 + r);
+                  if (m < ntok) {
+                    float v[8];
+                    load8(reinterpret_cast<const T*>(raw[r]), 8, true, v);
+                    put(m + half, v);
+                  }
+                }
+              }
+            }
+          } else {
+            if (!stage_free()) ok = false;
+#pragma unroll 1
+            for (int m = half; m < ((ntok + 1) & ~1); m += 2) {
+              const long long row = __shfl_sync(0xffffffffu, at, m);
+              float v[8];
+              load8(reinterpret_cast<const T*>(p.X) + row + k, m < ntok ? p.K - k : 0, false, v);
+              put(m, v);
+            }
           }
+          if (!ok) {
+            abort_flag[0] = 1;
+            break;
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
         }
       }
-      if (__any_sync(0xffffffffu, abort_flag[0])) break;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[s]);
+      it = end;
     }
   }
   __syncwarp();
 
-  // ------------------------------------------------------------ sum over the cluster, epilogue, store
-  const int feat = 32 * warp + lane;  // warps 0..3
-  const int n = f0 + feat;
-  const bool live = warp < 4 && n < p.N && !abort_flag[0];
-  const long long col = (long long)mat * p.mat_off + n;
-  const float bias = (live && p.bias) ? __ldg(p.bias + n) : 0.0f;
-  // All stages have been consumed: their memory takes the sums, [token]
-  // [feature].  The loops over tokens stay loops (the epilogue's code once,
-  // not once per token: unrolled, its instruction fetches took longer than
-  // the product).
-  float* red = reinterpret_cast<float*>(smem);
-  if (warp < 4) {
-#pragma unroll
-    for (int j = 0; j < BN; ++j)
-      if (j < ntok) red[j * 128 + feat] = acc[j];
-  }
   if (split > 1) {
+    // ------------------------------------------------------------ sums over the cluster
+    // All stages have been consumed: their memory takes the partial sums,
+    // [matrix][token][feature]; rank r completes the tokens r, r + split, ...,
+    // the partial sums added in rank order.
+    float* part = reinterpret_cast<float*>(smem);
+    const bool on = cid < n_items;
+    const Slot slot = on ? slot_at(p.slots, p.M, BN, cid % n_slots) : Slot{};
+    const int ft = on ? cid / n_slots : 0, ntok = on ? min(BN, slot.end - slot.row0) : 0;
+    const int feat = 32 * warp + lane, f0 = 128 * ft, n = f0 + feat;
+    if (warp < 4 && on) {
+#pragma unroll
+      for (int j = 0; j < C::kCols; ++j)
+        if ((j & (BN - 1)) < ntok) part[j * 128 + feat] = acc[j];
+    }
     __syncthreads();
     tc::cluster_sync();
-  }
-  if (live) {
+    if (warp < 4 && on && !abort_flag[0]) {
+      const float bias = (!PAIR && p.bias && n < p.N) ? __ldg(p.bias + n) : 0.0f;
+      int count = 0;
 #pragma unroll 1
-    for (int j = rank; j < ntok; j += split) {
-      float a = 0.0f;
-      if (split == 1) {
-        a = red[j * 128 + feat];
-      } else {
-        for (int q = 0; q < split; ++q) {
-          float x;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::mapa(red + j * 128 + feat, q)) : "memory");
-          a += x;
+      for (int j = rank; j < ntok; j += split, ++count) {
+        float a[C::kMats];
+#pragma unroll
+        for (int m = 0; m < C::kMats; ++m) {
+          a[m] = 0.0f;
+          for (int q = 0; q < split; ++q) {
+            float x;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(x)
+                         : "r"(tc::mapa(part + (m * BN + j) * 128 + feat, q))
+                         : "memory");
+            a[m] += x;
+          }
+        }
+        if constexpr (PAIR) {
+          red[count * 128 + feat] = n < p.N ? epi_act(a[0], p.act) * a[C::kMats - 1] : 0.0f;
+        } else if (n < p.N) {
+          const float y = a[0] + bias;
+          store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + n, p.act ? epi_act(y, p.act) : y);
         }
       }
-      a += bias;
-      store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + col, p.act ? epi_act(a, p.act) : a);
+      if constexpr (PAIR) {
+        if (!few_sync_or(false)) quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
+      }
     }
+    tc::cluster_sync();  // no CTA leaves while another reads its partial sums
   }
-  if (split > 1) tc::cluster_sync();  // no CTA leaves while another reads its partial sums
   tc::fence_before();
   __syncthreads();
   if (warp == 5) {
     tc::fence_after();
-    tc::tmem_dealloc(tmem, C::kAcc * BN);
+    tc::tmem_dealloc(tmem, C::kAcc * C::kCols);
   }
 }
 
@@ -747,17 +909,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
-template <int BN, int SRC>
-int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid_x,
-               int grid_y, cudaStream_t st, const char* who) {
+template <int BN, int SRC, bool PAIR>
+int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid,
+               cudaStream_t st, const char* who) {
   static std::atomic<uint64_t> ready{0};
-  constexpr size_t smem = FewCfg<BN>::kSmem;
-  MTC_CHECK_CUDA(allow_smem(few_kernel<BN, SRC>, smem, ready), who);
+  constexpr size_t smem = FewCfg<BN, PAIR>::kSmem;
+  MTC_CHECK_CUDA(allow_smem(few_kernel<BN, SRC, PAIR>, smem, ready), who);
   constexpr int threads = SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps;
-  MTC_CHECK_CUDA(launch_chained(few_kernel<BN, SRC>, dim3(grid_x, grid_y), dim3(threads), smem, st, p.split, tw0, tw1,
-                                tx, p),
+  MTC_CHECK_CUDA(launch_chained(few_kernel<BN, SRC, PAIR>, dim3(grid), dim3(threads), smem, st, p.split, tw0, tw1, tx,
+                                p),
                  who);
   return MTC_OK;
+}
+
+template <int BN, int SRC>
+int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid,
+               bool pair, cudaStream_t st, const char* who) {
+  return pair ? launch_few<BN, SRC, true>(tw0, tw1, tx, p, grid, st, who)
+              : launch_few<BN, SRC, false>(tw0, tw1, tx, p, grid, st, who);
 }
 
 template <int MODE>
@@ -900,7 +1069,6 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   p.nkb = nkb;
   p.N = w->N;
   p.Nb = Nb;
-  p.n_tiles = Nb;
   p.sw[0] = w->scales;
   p.sw[1] = a.w[1] ? a.w[1]->scales : w->scales;
   p.slots = a.slots;
@@ -909,43 +1077,44 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   p.lds = a.lds;
   p.order = a.order;
   p.kdiv = a.kdiv;
-  p.gate_act = a.gate_act;
   p.Y = a.Y;
   p.ydt = a.ydt;
   p.ldy = a.ldy;
-  p.mat_off = a.mat_off;
   p.bias = a.bias;
-  p.act = a.act;
+  p.act = n_mats == 2 ? a.gate_act : a.act;
+  p.hq = a.hq;
+  p.ldh = a.ldh;
+  p.hs = a.hs;
+  p.hs_ld = a.hs_ld;
+  p.early = a.early;
   p.status = a.status;
   p.timeout_ns = wait_limit_ns();
-  // Split the inputs over a cluster while the CTAs of the expected slots
-  // leave SMs idle (two CTAs are resident per SM) and every CTA keeps at
-  // least two blocks of 128 inputs.
-  const long long tiles = (long long)Nb * n_mats * a.slot_expect;
+  // Split the inputs over a cluster while the items would leave more than
+  // half of the SMs idle and every CTA keeps at least four blocks of 128
+  // inputs.  (One SM streams at most about twice its share of the memory
+  // bandwidth.)  A split launch has one cluster per item.
+  const long long bound = (long long)Nb * a.slot_bound;
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * sms && nkb >= 4 * split) split *= 2;
+  while (split < 8 && bound * split * 2 <= sms && nkb >= 8 * split) split *= 2;
   p.split = split;
-  p.early = a.early;
-  const int gx = Nb * n_mats * split;
-  MTC_REQUIRE(a.slot_bound <= 65535, "%s: %d token tiles in one launch", who, a.slot_bound);
+  const int grid = split > 1 ? (int)bound * split : (int)(bound < sms ? bound : sms);
+  const bool pair = n_mats == 2;
   if (a.xq) {
     switch (a.tile) {
-      case 16: return launch_few<16, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
-      case 32: return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
-      case 64: return launch_few<64, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
-      default: return launch_few<128, SRC_CODES>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+      case 16: return launch_few<16, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
+      case 32: return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
+      case 64: return launch_few<64, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
+      default:
+        MTC_REQUIRE(!pair, "%s: a gate / up pair in tiles of %d rows", who, a.tile);
+        return launch_few<128, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
     }
   }
   p.X = a.X;
-  p.xdt = a.xdt;
   p.ldx = a.ldx;
-  const int per16 = a.gated_src || a.xdt == MTC_F32 ? 4 : 8;
-  p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % per16 == 0 && (!a.gated_src || a.src_off % 4 == 0);
-  if (a.gated_src) {
-    p.mat_off = a.src_off;
-    return launch_few<16, SRC_GATED>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
-  }
-  return launch_few<16, SRC_ROWS>(tw[0], tw[1], tx, p, gx, a.slot_bound, st, who);
+  p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % (a.xdt == MTC_F32 ? 4 : 8) == 0;
+  if (a.xdt == MTC_F32) return launch_few<16, SRC_F32>(tw[0], tw[1], tx, p, grid, pair, st, who);
+  if (a.xdt == MTC_BF16) return launch_few<16, SRC_BF16>(tw[0], tw[1], tx, p, grid, pair, st, who);
+  return launch_few<16, SRC_F16>(tw[0], tw[1], tx, p, grid, pair, st, who);
 }
 
 }  // namespace fp8

@@ -12,14 +12,12 @@ namespace fp8 {
 
 // One product over token tiles ("slots", mtc_fp8.cuh): a dense matrix, or the
 // matrices of several experts.  The tokens are either codes with scales
-// (xq), activations that the kernel quantizes itself (X, 16 rows per slot at
-// most), or fp32 {gate, up} rows (gated_src) whose act(gate) * up it
-// quantizes.
+// (xq), or activations that the kernel quantizes itself (X, 16 rows per slot
+// at most).  A gate / up pair leaves act(gate) * up as codes and scales.
 struct Product {
   const mtc_fp8_matrix* w[2] = {nullptr, nullptr};  // w[1]: the up matrix of a gate / up pair
   const int32_t* slots = nullptr;                   // device slot list, or null for a dense product
   int slot_bound = 0;                               // slots of the launch at most
-  int slot_expect = 0;                              // slots that are likely to have rows
   int rows = 0;                                     // rows of the token operand
   int tile = 128;                                   // rows per slot
   bool many = false;                                // 128 tokens x 256 features per tile
@@ -32,15 +30,13 @@ struct Product {
   long long ldx = 0;
   const int32_t* order = nullptr;
   int kdiv = 1;
-  bool gated_src = false;
-  long long src_off = 0;                            // gated_src: column of up
   int gate_act = 0;
   void* Y = nullptr;
   int ydt = 0;
-  long long ldy = 0, mat_off = 0;
+  long long ldy = 0;
   const float* bias = nullptr;
   int act = 0;
-  uint8_t* hq = nullptr;                            // many with w[1]: quantized act(gate) * up
+  uint8_t* hq = nullptr;                            // with w[1]: quantized act(gate) * up
   long long ldh = 0;
   float* hs = nullptr;
   long long hs_ld = 0;
@@ -92,16 +88,12 @@ cudaError_t allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done)
 }
 int launch_product(const Product& a, cudaStream_t st, const char* who);
 
-// Rows of activations (or of fp32 {gate, up}) to codes and scales; with `pos`
-// row m goes to the rows pos[m * copies ..] that are not negative.
+// Rows of activations to codes and scales; with `pos` row m goes to the rows
+// pos[m * copies ..] that are not negative.
 struct QuantRows {
   const void* X = nullptr;
   int dt = 0, M = 0, K = 0;
   long long ldx = 0;
-  bool gated = false;
-  long long src_off = 0;
-  int gate_act = 0;
-  const int32_t* n_rows = nullptr;  // device row count (at most M), or null
   const int32_t* pos = nullptr;
   int copies = 1;
   uint8_t* q = nullptr;

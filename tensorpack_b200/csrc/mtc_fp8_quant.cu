@@ -10,9 +10,7 @@ namespace {
 struct QuantParams {
   const void* X;
   int M, K, Kb, vec;
-  long long ldx, src_off;
-  int gate_act;
-  const int32_t* n_rows;
+  long long ldx;
   const int32_t* pos;
   int copies;
   uint8_t* q;
@@ -22,13 +20,12 @@ struct QuantParams {
 };
 
 // One half warp per group of 128 inputs, 8 values per lane.
-template <typename T, bool GATED>
+template <typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
   griddep_wait();
   griddep_launch_dependents();
-  const int rows = p.n_rows ? min(p.M, *p.n_rows) : p.M;
-  const long long groups = (long long)rows * p.Kb;
+  const long long groups = (long long)p.M * p.Kb;
   const long long step = (long long)gridDim.x * 16;
   const long long last = (groups + 15) & ~15ll;  // whole warps take part in the shuffles
   for (long long g = (long long)blockIdx.x * 16 + half; g < last; g += step) {
@@ -38,12 +35,6 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
     float v[8];
     const T* x = reinterpret_cast<const T*>(p.X) + m * p.ldx + k;
     load8(x, n, p.vec, v);
-    if constexpr (GATED) {
-      float u[8];
-      load8(x + p.src_off, n, p.vec, u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = epi_act(v[i], p.gate_act) * u[i];
-    }
     const GroupScale gs = group_scale(half_warp_max(amax8(v)));
     const uint2 c = codes8(v, gs.mul);
     if (!on) continue;
@@ -123,9 +114,6 @@ int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
   p.K = a.K;
   p.Kb = (a.K + kBlock - 1) / kBlock;
   p.ldx = a.ldx;
-  p.src_off = a.src_off;
-  p.gate_act = a.gate_act;
-  p.n_rows = a.n_rows;
   p.pos = a.pos;
   p.copies = a.copies;
   p.q = a.q;
@@ -133,15 +121,14 @@ int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
   p.s = a.s;
   p.lds = a.lds;
   const int per16 = a.dt == MTC_F32 ? 4 : 8;
-  p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % per16 == 0 && (!a.gated || a.src_off % per16 == 0);
+  p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % per16 == 0;
   const long long blocks = ((long long)a.M * p.Kb + 15) / 16;
   const int sms = sm_count();
   MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
   const int grid = (int)(blocks < 8ll * sms ? blocks : 8ll * sms);
-  auto kernel = a.gated             ? quantize_kernel<float, true>
-                : a.dt == MTC_F32   ? quantize_kernel<float, false>
-                : a.dt == MTC_BF16  ? quantize_kernel<__nv_bfloat16, false>
-                                    : quantize_kernel<__half, false>;
+  auto kernel = a.dt == MTC_F32    ? quantize_kernel<float>
+                : a.dt == MTC_BF16 ? quantize_kernel<__nv_bfloat16>
+                                   : quantize_kernel<__half>;
   MTC_CHECK_CUDA(launch_chained(kernel, dim3(grid), dim3(256), 0, st, 1, p), who);
   return MTC_OK;
 }
@@ -259,7 +246,7 @@ extern "C" int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_ty
   a.rows = M;
   a.tile = d.tile;
   a.many = d.many;
-  a.slot_bound = a.slot_expect = (M + d.tile - 1) / d.tile;
+  a.slot_bound = (M + d.tile - 1) / d.tile;
   a.Y = Y;
   a.ydt = y_type;
   a.ldy = ldy;

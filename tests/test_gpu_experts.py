@@ -127,8 +127,9 @@ def forward(dev, T, E, k, D, I, dtype, activation="silu", ids=None, seed=0):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("T,E,k,D,I", [
     (1, 1, 1, 16, 1), (1, 64, 8, 256, 130), (3, 8, 2, 100, 60), (40, 16, 4, 300, 257),      # a few rows per expert
-    (90, 8, 1, 128, 128), (120, 16, 4, 260, 200), (300, 8, 4, 144, 96),                     # 16 to 96
+    (90, 8, 1, 128, 128), (120, 16, 4, 260, 200), (300, 8, 4, 144, 96),                     # tens
     (700, 4, 2, 200, 150), (1000, 3, 2, 384, 300),                                          # hundreds
+    (48, 128, 8, 512, 300), (250, 96, 8, 256, 700), (150, 32, 8, 256, 900),                 # several tiles per SM
 ])
 def test_experts(dev, T, E, k, D, I, dtype):
     forward(dev, T, E, k, D, I, TYPES[dtype], activation="gelu_tanh" if T % 2 else "silu", seed=T)

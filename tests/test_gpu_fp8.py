@@ -123,7 +123,8 @@ def test_gemm_matches_the_restatement(dev, M, K, N):
     assert torch.equal(y, fp8_gemm(x, m))  # the same bits every time
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 4096, 1024), (16, 14336, 512), (4, 4864, 896), (2100, 300, 4864), (1500, 1000, 3333)])
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 1024), (16, 14336, 512), (4, 4864, 896), (2100, 300, 4864), (1500, 1000, 3333),
+                                   (9, 1100, 40000), (40, 300, 40000), (100, 700, 40000)])
 def test_gemm_long_and_large(dev, M, K, N):
     from tensorpack_b200.kernels.fp8 import fp8_gemm
 
