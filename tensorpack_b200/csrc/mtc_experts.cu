@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Plan: rows (t, j) sorted by expert, stable, by one CTA
+// Plan: rows (t, j) sorted by expert, stable, a CTA per 1024 rows
 // ---------------------------------------------------------------------------
 struct PlanParams {
   const int32_t* ids;
@@ -166,6 +166,7 @@ struct PlanParams {
   int32_t* order;        // [R] row (t * k + j) at each sorted place
   int32_t* pos;          // [R] sorted place of each row, -1 for an id outside 0..E-1
   int32_t* slots;        // slot list
+  int32_t* counts;       // [CTAs][E] rows per expert of each CTA (more than one CTA)
 };
 
 constexpr int kPlanThreads = 1024;
@@ -196,9 +197,23 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int* total) {
   return r;
 }
 
-// Each warp owns a contiguous piece of the rows: it counts its experts, the
-// counts become places (experts in order, inside an expert the pieces in
-// order), and a second pass hands out the places in row order.
+// Rows per expert of every CTA's 1024 rows.
+__global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const PlanParams p) {
+  extern __shared__ int32_t hist[];
+  for (int i = threadIdx.x; i < p.E; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long r = (long long)blockIdx.x * kPlanThreads + threadIdx.x;
+  const int e = r < p.R ? p.ids[r] : -1;
+  if ((unsigned)e < (unsigned)p.E) atomicAdd(&hist[e], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.E; i += kPlanThreads) p.counts[(long long)blockIdx.x * p.E + i] = hist[i];
+}
+
+// Each warp owns 32 rows: it counts its experts, the counts of all warps and
+// CTAs become places (experts in order, inside an expert the rows in order),
+// and the rows take them.  The first CTA writes the slot list.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   extern __shared__ int32_t hist[];  // [32][E]
   __shared__ int warp_sums[33];
@@ -207,48 +222,50 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
-  const int piece = (((p.R + 31) >> 5) + 31) & ~31;
-  const int r0 = min((long long)warp * piece, (long long)p.R), r1 = min(r0 + piece, p.R);
+  const long long r = (long long)blockIdx.x * kPlanThreads + threadIdx.x;
+  const int id = r < p.R ? p.ids[r] : -1;
+  const bool ok = (unsigned)id < (unsigned)p.E;
+  const uint32_t same = __match_any_sync(0xffffffffu, ok ? id : -1);
+  const int rank = __popc(same & ((1u << lane) - 1u));
   int32_t* mine = hist + warp * p.E;
-  for (int r = r0 + lane; r < r1; r += 32) {
-    const int e = p.ids[r];
-    if ((unsigned)e < (unsigned)p.E) atomicAdd(&mine[e], 1);
-  }
+  if (ok && rank == 0) mine[id] = __popc(same);
   __syncthreads();
+  // thread e: rows of expert e in this CTA, in those before it, in all
   const int e = threadIdx.x;
-  int count = 0;
-  if (e < p.E)
+  int here = 0, before = 0, count = 0;
+  if (e < p.E) {
     for (int w = 0; w < 32; ++w) {
       const int c = hist[w * p.E + e];
-      hist[w * p.E + e] = count;
-      count += c;
+      hist[w * p.E + e] = here;
+      here += c;
     }
+    if (gridDim.x == 1) {
+      count = here;
+    } else {
+#pragma unroll 8
+      for (int b = 0; b < (int)gridDim.x; ++b) {
+        const int c = p.counts[(long long)b * p.E + e];
+        count += c;
+        before += b < (int)blockIdx.x ? c : 0;
+      }
+    }
+  }
   int total, n_slots;
   const int off = block_scan(count, warp_sums, &total);
-  const int ns = (count + p.size - 1) / p.size;
-  const int sl = block_scan(ns, warp_sums, &n_slots);
-  if (e < p.E) {
-    for (int w = 0; w < 32; ++w) hist[w * p.E + e] += off;
+  if (blockIdx.x == 0) {
+    const int ns = (count + p.size - 1) / p.size;
+    const int sl = block_scan(ns, warp_sums, &n_slots);
     for (int i = 0; i < ns; ++i)
       *reinterpret_cast<int4*>(p.slots + 4 + 4 * (sl + i)) = make_int4(e, off + i * p.size, off + count, 0);
+    if (threadIdx.x == 0) p.slots[0] = n_slots;
   }
-  if (threadIdx.x == 0) p.slots[0] = n_slots;
+  if (e < p.E)
+    for (int w = 0; w < 32; ++w) hist[w * p.E + e] += off + before;
   __syncthreads();
-  for (int rb = r0; rb < r1; rb += 32) {
-    const int r = rb + lane;
-    const int id = r < r1 ? p.ids[r] : -1;
-    const bool ok = (unsigned)id < (unsigned)p.E;
-    const uint32_t same = __match_any_sync(0xffffffffu, ok ? id : -1);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    int at = -1;
-    if (ok) at = mine[id] + rank;
-    __syncwarp();
-    if (ok && rank == 0) mine[id] += __popc(same);
-    __syncwarp();
-    if (r < r1) {
-      p.pos[r] = at;
-      if (ok) p.order[at] = r;
-    }
+  if (r < p.R) {
+    const int at = ok ? mine[id] + rank : -1;
+    p.pos[r] = at;
+    if (ok) p.order[at] = (int)r;
   }
 }
 
@@ -318,7 +335,8 @@ struct ExpertsPlan {
   int R, tile, slot_bound;
   bool raw, many;
   long long ldx, ldh, lds, ldo;
-  size_t order, pos, slots, xq, xs, hq, hs, out, bytes;
+  int plan_ctas;
+  size_t order, pos, slots, counts, xq, xs, hq, hs, out, bytes;
 };
 bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   const long long R = (long long)T * k;
@@ -345,6 +363,8 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   pl->order = take(4 * (size_t)R);
   pl->pos = take(4 * (size_t)R);
   pl->slots = take(16 * (size_t)(pl->slot_bound + 1));
+  pl->plan_ctas = (int)((R + kPlanThreads - 1) / kPlanThreads);
+  pl->counts = take(pl->plan_ctas > 1 ? 4 * (size_t)pl->plan_ctas * E : 4);
   pl->xq = pl->xs = 0;
   if (!pl->raw) {
     pl->xq = take((size_t)R * pl->ldx);
@@ -456,11 +476,14 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   int32_t* pos = reinterpret_cast<int32_t*>(base + pl.pos);
   int32_t* slots = reinterpret_cast<int32_t*>(base + pl.slots);
   {
-    PlanParams p = {ids, pl.R, E, pl.tile, order, pos, slots};
+    const PlanParams p = {ids, pl.R, E, pl.tile, order, pos, slots, reinterpret_cast<int32_t*>(base + pl.counts)};
     const size_t smem = (size_t)32 * E * 4;
-    if (smem > 48 * 1024)
-      MTC_CHECK_CUDA(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-    MTC_CHECK_CUDA(launch_chained(plan_kernel, dim3(1), dim3(kPlanThreads), smem, st, 1, p), who);
+    static std::atomic<uint64_t> ready{0};
+    MTC_CHECK_CUDA(allow_smem(plan_kernel, (size_t)32 * kMaxExperts * 4, ready), who);
+    if (pl.plan_ctas > 1)
+      MTC_CHECK_CUDA(launch_chained(plan_count_kernel, dim3(pl.plan_ctas), dim3(kPlanThreads), (size_t)E * 4, st, 1, p),
+                     who);
+    MTC_CHECK_CUDA(launch_chained(plan_kernel, dim3(pl.plan_ctas), dim3(kPlanThreads), smem, st, 1, p), who);
   }
   Product a;
   a.w[0] = gate;

@@ -43,13 +43,23 @@ __device__ __forceinline__ void flag(uint32_t* st, uint32_t bits) {
 // six more warps of the kernel quantize on the way (at most 16 rows per tile).
 enum { SRC_CODES = 0, SRC_F32 = 1, SRC_BF16 = 2, SRC_F16 = 3 };
 
+// Warps 0..3 scale, 4 issues TMA, the next 4 issue MMAs (for one accumulator
+// each: a thread needs some 0.3 us to wait for and issue the four MMAs of a
+// block and their commits, longer than the block's bytes take to arrive; 2
+// for wide tiles, whose sums want the registers), and 6 more quantize when
+// the kernel takes activations as they are.
+constexpr int kAccs = 4, kQuantWarps = 6;
+
+
 template <int BN, bool PAIR>
 struct FewCfg {
   static constexpr int kMats = PAIR ? 2 : 1;
   static constexpr uint32_t kBTile = BN * 128;
   static constexpr uint32_t kStage = kMats * kATile + kBTile;
   static constexpr int kCols = kMats * BN;              // TMEM columns of one accumulator
-  static constexpr int kAcc = 4;
+  static constexpr int kAcc = kAccs;                    // TMEM accumulators
+  static constexpr int kIssue = kCols >= 128 ? 2 : 4;   // issuing warps
+  static constexpr int kThreads = 32 * (5 + kIssue);    // without the quantizing warps
   static constexpr uint32_t kRed = 16 * 128 * 4 * kMats;  // staged sums of 16 tokens
   static constexpr uint32_t kRoom = 227 * 1024 - 1024 - 512 - 1024 - kRed;
   static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
@@ -61,9 +71,6 @@ struct FewCfg {
   static_assert(kCols * kAcc <= 512 && kSmem <= 227 * 1024, "TMEM and shared memory of one CTA");
   static_assert(kMats * BN * 128 * 4 <= kStages * kStage, "a cluster's partial sums fit the stages");
 };
-constexpr int kFewThreads = 192;      // 4 scaling warps, TMA warp, MMA warp
-constexpr int kQuantWarps = 6;        // more when the kernel quantizes its tokens itself
-
 struct FewParams {
   int K, nkb, N, Nb;                  // Nb: 128-feature tiles
   const float* sw[2];                 // scales of the matrix (or of gate and up)
@@ -120,6 +127,18 @@ __device__ __forceinline__ bool few_sync_or(bool x) {
   return r != 0;
 }
 
+// Four floats of the object at this offset in CTA `rank` of the cluster (the
+// loads of several ranks may be in flight together: not volatile, ordered by
+// the cluster barrier before them).
+__device__ __forceinline__ float4 load_cluster4(const float* p, int rank) {
+  float4 v;
+  asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(tc::mapa(p, rank))
+      : "memory");
+  return v;
+}
+
 // Staged values [i][128 features] of the tokens j0 + i * step, i < count, to
 // codes and scales: one half warp per token.  Called by the four scaling warps.
 __device__ __forceinline__ void quantize_staged(const FewParams& p, const float* h, int row0, int j0, int step,
@@ -146,7 +165,7 @@ __device__ __forceinline__ void quantize_staged(const FewParams& p, const float*
 // items slot + n_slots * feature tile in turn, so that neighbours in time
 // share weights, and the TMA warp runs ahead over their boundaries.
 template <int BN, int SRC, bool PAIR>
-__global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps, 1)
+__global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES ? 0 : 32 * kQuantWarps), 1)
     few_kernel(const __grid_constant__ CUtensorMap tw0, const __grid_constant__ CUtensorMap tw1,
                const __grid_constant__ CUtensorMap tx, const FewParams p) {
   using C = FewCfg<BN, PAIR>;
@@ -157,7 +176,7 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAcc;
   uint64_t* drain = acc_empty + C::kAcc;
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + 1);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + C::kAcc);
   uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
   float* red = reinterpret_cast<float*>(smem + C::kRedAt);
   float* sring = reinterpret_cast<float*>(smem + C::kScaleAt);
@@ -176,8 +195,8 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     for (int i = 0; i < C::kAcc; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 4);
+      mbar_init(&drain[i], 1);
     }
-    mbar_init(drain, 1);
     abort_flag[0] = 0;
     fence_barrier_init();
   }
@@ -231,35 +250,38 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
         flag(p.status, MTC_STATUS_TIMEOUT);
       }
     }
-  } else if (warp == 5) {
-    // ------------------------------------------------------------ MMA
+  } else if (warp >= 5 && warp < 5 + C::kIssue) {
+    // ------------------------------------------------------------ MMA: warp 5 + q issues the iterations q, q + kIssue, ...
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_e4m3_f32(128, BN);
-      uint32_t it = 0;
-      for (int w = cid; w < n_items && !abort_flag[0]; w += n_cid) {
-        for (int i = 0; i < n_it; ++i, ++it) {
-          const int s = it % C::kStages, b = it % C::kAcc;
-          if (!mbar_wait(&full[s], (it / C::kStages) & 1, p.timeout_ns) ||
-              (it >= C::kAcc && !mbar_wait(&acc_empty[b], ((it / C::kAcc) & 1) ^ 1, p.timeout_ns))) {
-            abort_flag[0] = 1;
-            break;
-          }
-          tc::fence_after();
-          const uint32_t a0 = smem_u32(smem + s * C::kStage), b0 = a0 + C::kMats * kATile;
-#pragma unroll
-          for (int m = 0; m < C::kMats; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_e4m3_ss(tmem + b * C::kCols + m * BN, tc::smem_desc_k_sw128(a0 + m * kATile + 32 * j),
-                          tc::smem_desc_k_sw128(b0 + 32 * j), idesc, j > 0);
-          tc::commit(&acc_full[b]);
-          tc::commit(&empty[s]);
+      const int q = warp - 5;
+      const int mine = cid < n_items ? (n_items - 1 - cid) / n_cid + 1 : 0;  // items of this CTA
+      const uint32_t total = (uint32_t)mine * n_it;
+      for (uint32_t it = q; it < total && !abort_flag[0]; it += C::kIssue) {
+        const int s = it % C::kStages, b = it % C::kAcc;
+        // The accumulator first: once it is free the sums up to it - kAcc
+        // have been read, so the stage's previous phase is over and the
+        // parity below means this one.
+        if ((it >= C::kAcc && !mbar_wait(&acc_empty[b], ((it / C::kAcc) & 1) ^ 1, p.timeout_ns)) ||
+            !mbar_wait(&full[s], (it / C::kStages) & 1, p.timeout_ns)) {
+          abort_flag[0] = 1;
+          break;
         }
+        tc::fence_after();
+        const uint32_t a0 = smem_u32(smem + s * C::kStage), b0 = a0 + C::kMats * kATile;
+#pragma unroll
+        for (int m = 0; m < C::kMats; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_e4m3_ss(tmem + b * C::kCols + m * BN, tc::smem_desc_k_sw128(a0 + m * kATile + 32 * j),
+                        tc::smem_desc_k_sw128(b0 + 32 * j), idesc, j > 0);
+        tc::commit(&acc_full[b]);
+        tc::commit(&empty[s]);
       }
       if (abort_flag[0]) {
         // no MMA may read shared memory or write TMEM after this CTA has left
-        tc::commit(drain);
-        (void)mbar_wait(drain, 0, 100000000ull);
+        tc::commit(&drain[q]);
+        (void)mbar_wait(&drain[q], 0, 100000000ull);
       }
     }
   } else if (warp < 4) {
@@ -371,9 +393,10 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     // complete; that must cover i - 2 kStages, or the parity it waits for
     // would be that of the phase before.
     static_assert(SRC == SRC_CODES || kQuantWarps <= C::kStages, "a quantizing warp may not lap the stages");
+    static_assert(C::kAcc <= C::kStages, "nor an issuing one");
     typedef typename SrcType<SRC>::T T;
     const int half = lane >> 4, l = lane & 15;
-    uint32_t it = 0, mine = warp - 6;
+    uint32_t it = 0, mine = warp - 5 - C::kIssue;
     bool ok = true;
     for (int w = cid; w < n_items && ok; w += n_cid) {
       const Slot slot = slot_at(p.slots, p.M, BN, w % n_slots);
@@ -462,7 +485,7 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     const bool on = cid < n_items;
     const Slot slot = on ? slot_at(p.slots, p.M, BN, cid % n_slots) : Slot{};
     const int ft = on ? cid / n_slots : 0, ntok = on ? min(BN, slot.end - slot.row0) : 0;
-    const int feat = 32 * warp + lane, f0 = 128 * ft, n = f0 + feat;
+    const int feat = 32 * warp + lane, f0 = 128 * ft;
     if (warp < 4 && on) {
 #pragma unroll
       for (int j = 0; j < C::kCols; ++j)
@@ -471,32 +494,52 @@ __global__ void __launch_bounds__(SRC == SRC_CODES ? kFewThreads : kFewThreads +
     __syncthreads();
     tc::cluster_sync();
     if (warp < 4 && on && !abort_flag[0]) {
-      const float bias = (!PAIR && p.bias && n < p.N) ? __ldg(p.bias + n) : 0.0f;
-      int count = 0;
+      // a warp per token, 4 features per lane, all ranks' loads in flight
+      const int f4 = 4 * lane, n4 = f0 + f4;
+      float bias[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bias[q] = (!PAIR && p.bias && n4 + q < p.N) ? __ldg(p.bias + n4 + q) : 0.0f;
+      const int count = rank < ntok ? (ntok - 1 - rank) / split + 1 : 0;
 #pragma unroll 1
-      for (int j = rank; j < ntok; j += split, ++count) {
-        float a[C::kMats];
+      for (int i = warp; i < count; i += 4) {
+        const int j = rank + i * split;
+        float4 x[C::kMats][8];
+#pragma unroll
+        for (int m = 0; m < C::kMats; ++m)
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (q < split) x[m][q] = load_cluster4(part + (m * BN + j) * 128 + f4, q);
+        float a[C::kMats][4];
 #pragma unroll
         for (int m = 0; m < C::kMats; ++m) {
-          a[m] = 0.0f;
-          for (int q = 0; q < split; ++q) {
-            float x;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                         : "=f"(x)
-                         : "r"(tc::mapa(part + (m * BN + j) * 128 + feat, q))
-                         : "memory");
-            a[m] += x;
-          }
+          a[m][0] = a[m][1] = a[m][2] = a[m][3] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (q < split) {
+              a[m][0] += x[m][q].x;
+              a[m][1] += x[m][q].y;
+              a[m][2] += x[m][q].z;
+              a[m][3] += x[m][q].w;
+            }
         }
         if constexpr (PAIR) {
-          red[count * 128 + feat] = n < p.N ? epi_act(a[0], p.act) * a[C::kMats - 1] : 0.0f;
-        } else if (n < p.N) {
-          const float y = a[0] + bias;
-          store1(p.Y, p.ydt, (slot.row0 + j) * p.ldy + n, p.act ? epi_act(y, p.act) : y);
+          float h[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) h[q] = n4 + q < p.N ? epi_act(a[0][q], p.act) * a[C::kMats - 1][q] : 0.0f;
+          *reinterpret_cast<float4*>(red + i * 128 + f4) = make_float4(h[0], h[1], h[2], h[3]);
+        } else {
+          const long long y = (slot.row0 + j) * p.ldy + n4;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (n4 + q < p.N) {
+              const float o = a[0][q] + bias[q];
+              store1(p.Y, p.ydt, y + q, p.act ? epi_act(o, p.act) : o);
+            }
         }
       }
       if constexpr (PAIR) {
-        if (!few_sync_or(false)) quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
+        few_sync();
+        quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
       }
     }
     tc::cluster_sync();  // no CTA leaves while another reads its partial sums
@@ -633,7 +676,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   uint64_t* acc_full = empty + kManyStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2]
   uint64_t* drain = acc_empty + 2;
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + 1);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(drain + 2);
   uint32_t* tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -651,8 +694,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], kManyWarps);
+      mbar_init(&drain[i], 1);
     }
-    mbar_init(drain, 1);
     abort_flag[0] = 0;
     fence_barrier_init();
   }
@@ -667,11 +710,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (warp == kManyWarps) {
       // ------------------------------------------------------------ TMA (lane 0) and scales (all lanes)
       uint32_t it = 0;
-      Slot next = slot_at(p.slots, p.M, 128, blockIdx.x % n_slots);  // one tile ahead
+      // Tiles in time: a dense product runs the token tiles of one feature
+      // tile together (all tokens stay in L2), a grouped one the feature
+      // tiles of one token tile (its expert's weights do).
+      auto slot_of = [&](int t) { return p.slots ? t / p.n_tiles : t % n_slots; };
+      Slot next = slot_at(p.slots, p.M, 128, slot_of(blockIdx.x));  // one tile ahead
       for (int t = blockIdx.x; t < n_work; t += gridDim.x) {
         const Slot slot = next;
-        if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, p.M, 128, (t + gridDim.x) % n_slots);
-        const int nt = t / n_slots, f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
+        if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, p.M, 128, slot_of(t + gridDim.x));
+        const int nt = p.slots ? t % p.n_tiles : t / n_slots, f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
         // lanes 0 and 1 fetch the features' scales, every lane those of the
         // rows lane, lane + 32, ...; a row past the end takes the last row's
         // scale (its values are never stored)
@@ -714,32 +761,32 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
         if (abort_flag[0]) flag(p.status, MTC_STATUS_TIMEOUT);
       }
-    } else if (warp == kManyWarps + 1 && lane == 0) {
-      // ---------------------------------------------------------- MMA
+    } else if (warp <= kManyWarps + 2 && lane == 0) {
+      // ---------------------------------------------------------- MMA: one warp per accumulator
       constexpr uint32_t idesc = idesc_e4m3_f32(128, 256);
-      uint32_t it = 0;
-      for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
-        for (int kb = 0; kb < p.nkb; ++kb, ++it) {
-          const int s = it % kManyStages, b = it & 1;
-          if (!mbar_wait(&full[s], (it / kManyStages) & 1, p.timeout_ns) ||
-              (it >= 2 && !mbar_wait(&acc_empty[b], ((it >> 1) & 1) ^ 1, p.timeout_ns))) {
-            abort_flag[0] = 1;
-            break;
-          }
-          tc::fence_after();
-          const uint32_t a0 = smem_u32(smem + s * kManyStage), b0 = a0 + kATile;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_e4m3_ss(tmem + b * 256, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
-                        j > 0);
-          tc::commit(&acc_full[b]);
-          tc::commit(&empty[s]);
+      const int b = warp - kManyWarps - 1;
+      const uint32_t total = (uint32_t)((n_work - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * p.nkb;
+      for (uint32_t it = b; it < total && !abort_flag[0]; it += 2) {
+        const int s = it % kManyStages;
+        // (the accumulator first: see few_kernel)
+        if ((it >= 2 && !mbar_wait(&acc_empty[b], ((it >> 1) & 1) ^ 1, p.timeout_ns)) ||
+            !mbar_wait(&full[s], (it / kManyStages) & 1, p.timeout_ns)) {
+          abort_flag[0] = 1;
+          break;
         }
+        tc::fence_after();
+        const uint32_t a0 = smem_u32(smem + s * kManyStage), b0 = a0 + kATile;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma_e4m3_ss(tmem + b * 256, tc::smem_desc_k_sw128(a0 + 32 * j), tc::smem_desc_k_sw128(b0 + 32 * j), idesc,
+                      j > 0);
+        tc::commit(&acc_full[b]);
+        tc::commit(&empty[s]);
       }
       if (abort_flag[0]) {
         // no MMA may read shared memory or write TMEM after this CTA has left
-        tc::commit(drain);
-        (void)mbar_wait(drain, 0, 100000000ull);
+        tc::commit(&drain[b]);
+        (void)mbar_wait(&drain[b], 0, 100000000ull);
       }
     }
   } else {
@@ -915,7 +962,7 @@ int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap
   static std::atomic<uint64_t> ready{0};
   constexpr size_t smem = FewCfg<BN, PAIR>::kSmem;
   MTC_CHECK_CUDA(allow_smem(few_kernel<BN, SRC, PAIR>, smem, ready), who);
-  constexpr int threads = SRC == SRC_CODES ? kFewThreads : kFewThreads + 32 * kQuantWarps;
+  constexpr int threads = FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES ? 0 : 32 * kQuantWarps);
   MTC_CHECK_CUDA(launch_chained(few_kernel<BN, SRC, PAIR>, dim3(grid), dim3(threads), smem, st, p.split, tw0, tw1, tx,
                                 p),
                  who);
