@@ -477,7 +477,7 @@ MTC_API int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type,
 /* Routing of T tokens to k of E experts (E <= 1024, k <= 32) from router
  * logits (T x E, row stride ld).  Scores: softmax over the experts, or
  * sigmoid.  The choice goes by score + bias (bias: E finite floats, or NULL)
- * in 64 bits.  With groups > 1 (at most 32, dividing E) only the experts of
+ * in 64 bits; without bias and groups by the logits, whose order that is.  With groups > 1 (at most 32, dividing E) only the experts of
  * the top_groups groups with the largest sum of their two best choices
  * compete.  ids: the k best, best first, ties to the lowest index; weights:
  * their scores (without bias), divided by their sum if renormalize, times

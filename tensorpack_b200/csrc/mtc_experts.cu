@@ -26,16 +26,94 @@ struct RouteParams {
   float* weights;
 };
 
-// A score that decides: 64-bit order, so that experts whose scores agree in
-// 32 bits are still told apart.  The unsigned order of the key is the order
-// of the value; key 1 is a masked (-inf or NaN) expert, key 0 one that may
-// not be chosen.
+// Unsigned order of the key = order of the value; key 1 is a masked (-inf or
+// NaN) expert, key 0 one that may not be chosen.
 __device__ __forceinline__ unsigned long long order_key(double c) {
   if (!(c > -INFINITY)) return 1ull;  // -inf, NaN
   const long long b = __double_as_longlong(c);
   return (unsigned long long)b ^ (b < 0 ? ~0ull : 0x8000000000000000ull);
 }
+__device__ __forceinline__ uint32_t order_key(float c) {
+  if (!(c > -INFINITY)) return 1u;
+  const uint32_t b = __float_as_uint(c);
+  return b ^ ((int)b < 0 ? ~0u : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k ^ ((int)k < 0 ? 0x80000000u : ~0u));
+}
 
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+  return x;
+}
+
+// Score of a logit: exp(z - max) (to be divided by the total), or
+// 1 / (1 + exp(-z)); a masked one has score 0.
+template <typename F>
+__device__ __forceinline__ F raw_score(float z, float zmax, bool sigmoid) {
+  if (z == -INFINITY) return (F)0;
+  if (sizeof(F) == 8) return sigmoid ? 1.0 / (1.0 + exp(-(double)z)) : exp((double)z - (double)zmax);
+  return sigmoid ? 1.0f / (1.0f + expf(-z)) : expf(z - zmax);
+}
+
+// Bits of the experts' groups that are kept, one per group at bit g * lanes,
+// and how far the worst kept group is ahead of the best dropped one.  `cs`:
+// the choices in shared memory.  `lanes` lanes (a power of two) find a
+// group's two best.
+template <typename F>
+__device__ __forceinline__ uint32_t keep_groups(const RouteParams& p, const F* cs, int lane, int lanes, F* gap) {
+  const int g = lane / lanes, sub = lane & (lanes - 1);
+  F g1 = -INFINITY, g2 = -INFINITY;
+  if (g < p.groups)
+    for (int i = sub; i < p.gsize; i += lanes) {
+      const F x = cs[g * p.gsize + i];
+      if (x > g1) {
+        g2 = g1;
+        g1 = x;
+      } else if (x > g2) {
+        g2 = x;
+      }
+    }
+  for (int d = 1; d < lanes; d <<= 1) {
+    const F o1 = __shfl_xor_sync(0xffffffffu, g1, d), o2 = __shfl_xor_sync(0xffffffffu, g2, d);
+    if (o1 > g1) {
+      g2 = g1 > o2 ? g1 : o2;
+      g1 = o1;
+    } else {
+      g2 = g2 > o1 ? g2 : o1;
+    }
+  }
+  const F gv = p.gsize > 1 ? g1 + g2 : g1;
+  int rank = 0;
+  for (int o = 0; o < p.groups; ++o) {
+    const F v = __shfl_sync(0xffffffffu, gv, o * lanes);
+    rank += v > gv || (v == gv && o < g);
+  }
+  const bool real = g < p.groups, kept = real && rank < p.top_groups;
+  // the two groups on either side of the border
+  const uint32_t last = __ballot_sync(0xffffffffu, real && sub == 0 && rank == p.top_groups - 1);
+  const uint32_t first = __ballot_sync(0xffffffffu, real && sub == 0 && rank == p.top_groups);
+  const F in = __shfl_sync(0xffffffffu, gv, __ffs(last) - 1), out = __shfl_sync(0xffffffffu, gv, __ffs(first) - 1);
+  *gap = in > out ? in - out : (F)0;
+  if (in == -INFINITY || out == -INFINITY) *gap = in == out ? (F)INFINITY : *gap;  // masked groups: by index
+  return __ballot_sync(0xffffffffu, kept && sub == 0);
+}
+
+// A warp per token.  The choice is made in 64 bits as defined, but reached in
+// 32 where that is certain: without bias and groups the order of the scores
+// is that of the logits; otherwise the fp32 choices are taken when every
+// decision (between neighbours of the k + 1 best, at the groups' border) has
+// a margin above the fp32 error, and computed again in 64 bits when one has
+// not (about one token in a hundred).
+//
+// Error of an fp32 choice s + b, with M = max(|s + b| + s): the rounding of
+// the sum is below 2^-24 M; a sigmoid's relative error below 6 * 2^-24; a
+// softmax score's below (16 + d) * 2^-24 for a logit d below the largest (the
+// difference, expf, the total, the division), where s d is below s log(1/s)
+// and so (16 + d) s below 22 M.  Twice that is below 2^-20 M and 2^-18 M.
+//
+// 64 bits for all: 29.3 us for 8192 x 256 with groups and bias.
 template <typename T, int NPL>
 __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   extern __shared__ double route_smem[];
@@ -46,82 +124,74 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   if (t >= p.T) return;
   const T* z = reinterpret_cast<const T*>(p.logits) + t * p.ld;
   float v[NPL];
-  float zmax = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
     const int e = 32 * i + lane;
-    float x = -INFINITY;
-    if (e < p.E) {
-      x = to_f32(z[e]);
-      if (x != x) x = -INFINITY;
-      x = fminf(x, 3.402823466e38f);
-    }
-    v[i] = x;
-    zmax = fmaxf(zmax, x);
+    v[i] = e < p.E ? to_f32(z[e]) : -INFINITY;
   }
-  for (int d = 16; d; d >>= 1) zmax = fmaxf(zmax, __shfl_xor_sync(0xffffffffu, zmax, d));
-  // score of a logit: exp(z - max) / total, or 1 / (1 + exp(-z)); a masked one has score 0
-  auto raw_score = [&](float x) -> double {
-    if (x == -INFINITY) return 0.0;
-    return p.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : exp((double)x - (double)zmax);
-  };
-  double total = 1.0;
-  unsigned long long key[NPL];
-  {
-    double c[NPL];
-    double sum = 0.0;
+  float zmax = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) {
+    if (v[i] != v[i]) v[i] = -INFINITY;
+    v[i] = fminf(v[i], 3.402823466e38f);
+    zmax = fmaxf(zmax, v[i]);
+  }
+  if (!p.sigmoid) zmax = warp_max(zmax);
+  const bool by_logit = !p.bias && p.groups == 1;
+  int lanes = 1;
+  while (2 * lanes * p.groups <= 32) lanes *= 2;
+
+  uint32_t key[NPL];
+  float margin = 0.0f;
+  bool sure = true;
+  if (by_logit) {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) key[i] = 32 * i + lane < p.E ? order_key(v[i]) : 0u;
+  } else {
+    float c[NPL], sum = 0.0f, most = 0.0f;
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      c[i] = raw_score(v[i]);
+      c[i] = raw_score<float>(v[i], zmax, p.sigmoid);
       sum += c[i];
     }
+    float inv = 1.0f;
     if (!p.sigmoid) {
+#pragma unroll
       for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      total = sum;
+      inv = 1.0f / sum;
     }
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int e = 32 * i + lane;
-      if (!p.sigmoid) c[i] = c[i] / total;
-      if (p.bias && e < p.E) c[i] += (double)p.bias[e];
+      const float sc = c[i] * inv;
+      c[i] = p.bias && e < p.E ? sc + p.bias[e] : sc;
       if (v[i] == -INFINITY) c[i] = -INFINITY;
+      else most = fmaxf(most, fabsf(c[i]) + sc);
     }
+    margin = warp_max(most) * (p.sigmoid ? 9.5367431640625e-7f : 3.814697265625e-6f);
     uint32_t keep = ~0u;
     if (p.groups > 1) {
-      double* cs = route_smem + warp * p.E;
+      float* cs = reinterpret_cast<float*>(route_smem + warp * p.E);
 #pragma unroll
       for (int i = 0; i < NPL; ++i)
         if (32 * i + lane < p.E) cs[32 * i + lane] = c[i];
       __syncwarp();
-      double g1 = -INFINITY, g2 = -INFINITY;
-      if (lane < p.groups)
-        for (int i = 0; i < p.gsize; ++i) {
-          const double x = cs[lane * p.gsize + i];
-          if (x > g1) {
-            g2 = g1;
-            g1 = x;
-          } else if (x > g2) {
-            g2 = x;
-          }
-        }
-      const double gv = p.gsize > 1 ? g1 + g2 : g1;
-      int rank = 0;
-      for (int g = 0; g < p.groups; ++g) {
-        const double o = __shfl_sync(0xffffffffu, gv, g);
-        rank += o > gv || (o == gv && g < lane);
-      }
-      keep = __ballot_sync(0xffffffffu, lane < p.groups && rank < p.top_groups);
+      float gap;
+      keep = keep_groups<float>(p, cs, lane, lanes, &gap);
+      sure = gap > 2.0f * margin;  // a group's value is the sum of two choices
+      __syncwarp();
     }
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int e = 32 * i + lane;
-      key[i] = 0ull;
-      if (e < p.E && (p.groups == 1 || (keep >> (e / p.gsize) & 1u))) key[i] = order_key(c[i]);
+      key[i] = e < p.E && (p.groups == 1 || (keep >> (e / p.gsize * lanes) & 1u)) ? order_key(c[i]) : 0u;
     }
   }
   int my_id = 0;
-  for (int j = 0; j < p.k; ++j) {
-    unsigned long long best = 0ull;
+  uint32_t before = 0u;
+  for (int j = 0; j <= p.k && sure; ++j) {
+    if (j == p.k && by_logit) break;
+    uint32_t best = 0u;
     int at = 0;
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
@@ -129,26 +199,78 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
         best = key[i];
         at = i;
       }
-    const uint32_t hi = (uint32_t)(best >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t lo = hi == mh ? (uint32_t)best : 0u, ml = __reduce_max_sync(0xffffffffu, lo);
-    const uint32_t mine = (hi == mh && lo == ml) ? (uint32_t)(32 * at + lane) : ~0u;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    if (!by_logit && j > 0 && before > 1u && top > 1u) sure = key_value(before) - key_value(top) > margin;
+    before = top;
+    const uint32_t mine = best == top ? (uint32_t)(32 * at + lane) : ~0u;
     const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
     if (mine == id) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i)
-        if (i == at) key[i] = 0ull;
+        if (i == at) key[i] = 0u;
     }
     if (lane == j) my_id = (int)id;
   }
+  if (!sure) {
+    double* cs = route_smem + warp * p.E;
+    double sum = 0.0;
+    for (int i = 0; i < NPL; ++i) {
+      float x = 32 * i + lane < p.E ? to_f32(z[32 * i + lane]) : -INFINITY;
+      if (x != x) x = -INFINITY;
+      x = fminf(x, 3.402823466e38f);
+      const double sc = raw_score<double>(x, zmax, p.sigmoid);
+      sum += sc;
+      if (32 * i + lane < p.E) cs[32 * i + lane] = x == -INFINITY ? (double)-INFINITY : sc;
+    }
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    for (int e = lane; e < p.E; e += 32) {
+      double c = cs[e];
+      if (c != -INFINITY) {
+        if (!p.sigmoid) c = c / sum;
+        if (p.bias) c += (double)p.bias[e];
+        cs[e] = c;
+      }
+    }
+    __syncwarp();
+    uint32_t keep = ~0u;
+    double gap;
+    if (p.groups > 1) keep = keep_groups<double>(p, cs, lane, lanes, &gap);
+    unsigned long long done = 0ull;  // this lane's experts that are taken, by i (at most 32)
+    for (int j = 0; j < p.k; ++j) {
+      unsigned long long best = 0ull;
+      int at = 0;
+      for (int i = 0; i < NPL; ++i) {
+        const int e = 32 * i + lane;
+        if (e >= p.E || (done >> i & 1ull) || !(p.groups == 1 || (keep >> (e / p.gsize * lanes) & 1u))) continue;
+        const unsigned long long o = order_key(cs[e]);
+        if (o > best) {
+          best = o;
+          at = i;
+        }
+      }
+      const uint32_t hi = (uint32_t)(best >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
+      const uint32_t lo = hi == mh ? (uint32_t)best : 0u, ml = __reduce_max_sync(0xffffffffu, lo);
+      const uint32_t mine = (hi == mh && lo == ml) ? (uint32_t)(32 * at + lane) : ~0u;
+      const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
+      if (mine == id) done |= 1ull << at;
+      if (lane == j) my_id = (int)id;
+    }
+  }
+  // the weights, from the scores of the chosen in 64 bits
   double w = 0.0;
   if (lane < p.k) {
     float x = to_f32(z[my_id]);
     if (x != x) x = -INFINITY;
-    w = raw_score(fminf(x, 3.402823466e38f));
+    w = raw_score<double>(fminf(x, 3.402823466e38f), zmax, p.sigmoid);
   }
-  double div = total;
+  double div = 1.0;
   if (p.renorm) {
     div = w;
+    for (int d = 16; d; d >>= 1) div += __shfl_xor_sync(0xffffffffu, div, d);
+  } else if (!p.sigmoid) {
+    div = 0.0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) div += raw_score<double>(v[i], zmax, false);
     for (int d = 16; d; d >>= 1) div += __shfl_xor_sync(0xffffffffu, div, d);
   }
   if (lane < p.k) {
@@ -275,7 +397,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
 struct CombineParams {
   const void* rows;
   long long ldr;
-  const int32_t* pos;
+  const int32_t* pos;    // or null: row j, for the ids of one token
+  const int32_t* ids;
+  int E;
   const float* weights;
   int T, k, D;
   void* Y;
@@ -285,43 +409,61 @@ struct CombineParams {
 
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
-  const int t = blockIdx.x;
+  const int parts = (p.D + 2047) >> 11, t = blockIdx.x / parts;
   __shared__ int at[kMaxTopK];
   __shared__ float w[kMaxTopK];
   griddep_wait();
   griddep_launch_dependents();
-  if (threadIdx.x < p.k) {
-    at[threadIdx.x] = p.pos[(long long)t * p.k + threadIdx.x];
-    w[threadIdx.x] = p.weights[(long long)t * p.k + threadIdx.x];
+  if (threadIdx.x < kMaxTopK) {
+    const int j = threadIdx.x;
+    int a = -1;
+    if (j < p.k) {
+      a = p.pos ? p.pos[(long long)t * p.k + j] : (unsigned)p.ids[j] < (unsigned)p.E ? j : -1;
+      w[j] = p.weights[(long long)t * p.k + j];
+    }
+    at[j] = a;
   }
   __syncthreads();
-  for (int d = 8 * threadIdx.x; d < p.D; d += 8 * 256) {
-    float a[8];
+  const int d = 8 * ((blockIdx.x - t * parts) * 256 + threadIdx.x);
+  if (d >= p.D) return;
+  float a[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = 0.0f;
-    for (int j = 0; j < p.k; ++j) {
-      if (at[j] < 0) continue;
-      float v[8];
-      load8(reinterpret_cast<const T*>(p.rows) + at[j] * p.ldr + d, p.D - d, true, v);
+  for (int i = 0; i < 8; ++i) a[i] = 0.0f;
+  // (rows are padded to 8 values, so the last vector may be read whole)
+  constexpr int kVec = sizeof(T) == 4 ? 2 : 1, kMore = sizeof(T) == 4 ? 4 : 8;
+  for (int j0 = 0; j0 < p.k; j0 += kMore) {
+    uint4 raw[kMore][kVec];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = fmaf(w[j], v[i], a[i]);
+    for (int j = 0; j < kMore; ++j) {
+      const int r = j0 + j < kMaxTopK ? at[j0 + j] : -1;
+      const T* row = reinterpret_cast<const T*>(p.rows) + r * p.ldr + d;
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) raw[j][q] = load16_if(reinterpret_cast<const uint4*>(row) + q, r >= 0);
     }
-    const long long y = t * p.ldy + d;
-    if (p.vec && d + 8 <= p.D) {
-      if (p.ydt == MTC_F32) {
-        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + y);
-        o[0] = make_float4(a[0], a[1], a[2], a[3]);
-        o[1] = make_float4(a[4], a[5], a[6], a[7]);
-      } else {
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.Y) + y) =
-            make_uint4(pack2(p.ydt, a[0], a[1]), pack2(p.ydt, a[2], a[3]), pack2(p.ydt, a[4], a[5]),
-                       pack2(p.ydt, a[6], a[7]));
+#pragma unroll
+    for (int j = 0; j < kMore; ++j)
+      if (j0 + j < p.k && at[j0 + j] >= 0) {
+        float v[8];
+        unpack8<T>(raw[j], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = fmaf(w[j0 + j], v[i], a[i]);
       }
+  }
+  const long long y = t * p.ldy + d;
+  if (p.vec && d + 8 <= p.D) {
+    if (p.ydt == MTC_F32) {
+      float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.Y) + y);
+      o[0] = make_float4(a[0], a[1], a[2], a[3]);
+      o[1] = make_float4(a[4], a[5], a[6], a[7]);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (d + i < p.D) store1(p.Y, p.ydt, y + i, a[i]);
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.Y) + y) =
+          make_uint4(pack2(p.ydt, a[0], a[1]), pack2(p.ydt, a[2], a[3]), pack2(p.ydt, a[4], a[5]),
+                     pack2(p.ydt, a[6], a[7]));
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d + i < p.D) store1(p.Y, p.ydt, y + i, a[i]);
   }
 }
 
@@ -330,10 +472,11 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How the experts' products run, from the mean number of rows of an expert:
 // up to 8, 16-row tiles whose tokens the first product quantizes itself; up
-// to 48, wider tiles of codes; above, the 128-token kernel.
+// to 48, wider tiles of codes; above, the 128-token kernel.  A single token
+// needs no plan: every row is a slot.
 struct ExpertsPlan {
   int R, tile, slot_bound;
-  bool raw, many;
+  bool direct, raw, many;
   long long ldx, ldh, lds, ldo;
   int plan_ctas;
   size_t order, pos, slots, counts, xq, xs, hq, hs, out, bytes;
@@ -343,12 +486,13 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   if (R > 0x7fff0000ll) return false;
   pl->R = (int)R;
   const double mean = (double)R / E;
-  pl->raw = mean <= 8.0;
-  pl->many = mean > 48.0;
+  pl->direct = T == 1;
+  pl->raw = pl->direct || mean <= 8.0;
+  pl->many = !pl->raw && mean > 48.0;
   pl->tile = pl->raw ? 16 : mean <= 24.0 ? 32 : pl->many ? 128 : 64;
   const long long used = R < E ? R : E;
   long long bound = R / pl->tile + used;
-  if (bound > R) bound = R;
+  if (bound > R || pl->direct) bound = R;
   pl->slot_bound = (int)bound;
   pl->ldx = (D + 15) & ~15ll;
   pl->ldh = (I + 15) & ~15ll;
@@ -379,8 +523,9 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
 
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t st) {
-  const int warps = p.groups > 1 && p.E > 512 ? 4 : 8;
-  const size_t smem = p.groups > 1 ? (size_t)warps * p.E * 8 : 0;
+  const bool by_logit = !p.bias && p.groups == 1;
+  const int warps = !by_logit && p.E > 512 ? 4 : 8;
+  const size_t smem = by_logit ? 0 : (size_t)warps * p.E * 8;
   auto go = [&](auto kernel) -> int {
     if (smem > 48 * 1024)
       MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
@@ -475,7 +620,7 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   int32_t* order = reinterpret_cast<int32_t*>(base + pl.order);
   int32_t* pos = reinterpret_cast<int32_t*>(base + pl.pos);
   int32_t* slots = reinterpret_cast<int32_t*>(base + pl.slots);
-  {
+  if (!pl.direct) {
     const PlanParams p = {ids, pl.R, E, pl.tile, order, pos, slots, reinterpret_cast<int32_t*>(base + pl.counts)};
     const size_t smem = (size_t)32 * E * 4;
     static std::atomic<uint64_t> ready{0};
@@ -488,7 +633,8 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   Product a;
   a.w[0] = gate;
   a.w[1] = up;
-  a.slots = slots;
+  a.slots = pl.direct ? ids : slots;
+  a.experts = pl.direct ? E : 0;
   a.slot_bound = pl.slot_bound;
   a.rows = pl.R;
   a.tile = pl.tile;
@@ -498,7 +644,7 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   Product b = a;
   b.w[0] = down;
   b.w[1] = nullptr;
-  b.early = true;  // the plan ran before the first product
+  b.early = true;  // the plan (or whatever wrote the ids) ran before the first product
   if (!pl.raw) {
     QuantRows q;
     q.X = X;
@@ -522,8 +668,9 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
     a.X = X;
     a.xdt = x_type;
     a.ldx = ldx;
-    a.order = order;
+    a.order = pl.direct ? nullptr : order;
     a.kdiv = k;
+    if (pl.direct) a.ldx = 0;  // every row is the one token
   }
   a.hq = base + pl.hq;
   a.ldh = pl.ldh;
@@ -540,11 +687,23 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   b.ldy = pl.ldo;
   rc = launch_product(b, st, who);
   if (rc != MTC_OK) return rc;
-  CombineParams c = {base + pl.out, pl.ldo, pos, weights, T, k, D, Y, ldy, y_type, 0};
+  CombineParams c = {};
+  c.rows = base + pl.out;
+  c.ldr = pl.ldo;
+  c.pos = pl.direct ? nullptr : pos;
+  c.ids = ids;
+  c.E = E;
+  c.weights = weights;
+  c.T = T;
+  c.k = k;
+  c.D = D;
+  c.Y = Y;
+  c.ldy = ldy;
+  c.ydt = y_type;
   c.vec = (reinterpret_cast<uintptr_t>(Y) & 15) == 0 && ldy % (y_type == MTC_F32 ? 4 : 8) == 0;
   auto kernel = y_type == MTC_F32    ? combine_kernel<float>
                 : y_type == MTC_BF16 ? combine_kernel<__nv_bfloat16>
                                      : combine_kernel<__half>;
-  MTC_CHECK_CUDA(launch_chained(kernel, dim3(T), dim3(256), 0, st, 1, c), who);
+  MTC_CHECK_CUDA(launch_chained(kernel, dim3((unsigned)((D + 2047) / 2048) * (unsigned)T), dim3(256), 0, st, 1, c), who);
   return MTC_OK;
 }

@@ -93,6 +93,44 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 
+// Starts bringing `bytes` (a multiple of 16) at the 16-byte aligned p into L2.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  if (bytes) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
+// 16 bytes at p, or zeros: one predicated load, so that several are in flight.
+__device__ __forceinline__ uint4 load16_if(const uint4* p, bool on) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.u32 q, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@q ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+// Eight values from one (16-bit types) or two (fp32) such vectors.
+template <typename T, int NV>
+__device__ __forceinline__ void unpack8(const uint4 (&raw)[NV], float (&v)[8]) {
+  static_assert(NV * 16 == 8 * sizeof(T), "eight values");
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[NV - 1].x, raw[NV - 1].y, raw[NV - 1].z,
+                         raw[NV - 1].w};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T lo, hi;
+      *reinterpret_cast<uint16_t*>(&lo) = (uint16_t)(w[i] & 0xffffu);
+      *reinterpret_cast<uint16_t*>(&hi) = (uint16_t)(w[i] >> 16);
+      v[2 * i] = to_f32(lo);
+      v[2 * i + 1] = to_f32(hi);
+    }
+  }
+}
+
 // Eight consecutive values at p as fp32; `n` of them exist (the others read
 // as zero).  `vec`: p is 16-byte aligned and n >= 8 may be read as vectors.
 template <typename T>
@@ -229,20 +267,28 @@ __device__ __forceinline__ void fma2(f32x2& acc, f32x2 v, f32x2 s) {
 // ---------------------------------------------------------------------------
 // Token tiles
 // ---------------------------------------------------------------------------
-// Slot list written by the plan kernel for a grouped product: word 0 is the
-// number of slots, slot i is {expert, first row, end row of the expert, 0} at
-// words 4 + 4 i.  (Read from L2: a product may read it before its predecessor
-// in the stream has ended.)  A dense product has no list: slot i covers rows
-// from i * size of the single matrix.
+// Slots of a grouped product: a list written by the plan kernel (word 0 is
+// their number, slot i is {expert, first row, end row of the expert, 0} at
+// words 4 + 4 i), or, for a single token (ids, experts > 0), one slot per row
+// with the row's expert, or none of its rows if that is no expert.  (Read
+// from L2: a product may read them before its predecessor in the stream has
+// ended.)  A dense product has neither: slot i covers rows from i * size of
+// the single matrix.
 struct Slot {
   int e, row0, end;
 };
-__device__ __forceinline__ int slot_count(const int32_t* slots, int M, int size) {
-  return slots ? __ldcg(slots) : (M + size - 1) / size;
+__device__ __forceinline__ int slot_count(const int32_t* slots, int experts, int M, int size) {
+  return experts ? M : slots ? __ldcg(slots) : (M + size - 1) / size;
 }
-__device__ __forceinline__ Slot slot_at(const int32_t* slots, int M, int size, int i) {
+__device__ __forceinline__ Slot slot_at(const int32_t* slots, int experts, int M, int size, int i) {
   Slot s;
-  if (slots) {
+  if (experts) {
+    const int e = __ldcg(slots + i);
+    const bool ok = (unsigned)e < (unsigned)experts;
+    s.e = ok ? e : 0;
+    s.row0 = i;
+    s.end = ok ? i + 1 : i;
+  } else if (slots) {
     const int4 v = __ldcg(reinterpret_cast<const int4*>(slots + 4 + 4 * i));
     s.e = v.x;
     s.row0 = v.y;

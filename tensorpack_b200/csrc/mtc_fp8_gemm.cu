@@ -22,6 +22,8 @@
 //    the same 128 of the up matrix; the output is act(gate) * up, quantized.
 #include <string.h>
 
+#include <type_traits>
+
 #include "mtc_fp8.cuh"
 #include "mtc_internal.h"
 #include "mtc_fp8_internal.h"
@@ -61,12 +63,14 @@ struct FewCfg {
   static constexpr int kIssue = kCols >= 128 ? 2 : 4;   // issuing warps
   static constexpr int kThreads = 32 * (5 + kIssue);    // without the quantizing warps
   static constexpr uint32_t kRed = 16 * 128 * 4 * kMats;  // staged sums of 16 tokens
-  static constexpr uint32_t kRoom = 227 * 1024 - 1024 - 512 - 1024 - kRed;
+  static constexpr uint32_t kMul = 4 * 2 * kCols * 4;   // per scaling warp, two buffers of scales
+  static constexpr uint32_t kRoom = 227 * 1024 - 1024 - 512 - 1024 - kRed - kMul;
   static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
   static constexpr int kRing = kStages + kAcc;          // slots of in-kernel token scales
   static constexpr uint32_t kBars = kStages * kStage;
   static constexpr uint32_t kRedAt = kBars + 512;
-  static constexpr uint32_t kScaleAt = kRedAt + kRed;
+  static constexpr uint32_t kMulAt = kRedAt + kRed;
+  static constexpr uint32_t kScaleAt = kMulAt + kMul;
   static constexpr size_t kSmem = 1024 + kScaleAt + (BN == 16 ? kRing * BN * 4 : 0);
   static_assert(kCols * kAcc <= 512 && kSmem <= 227 * 1024, "TMEM and shared memory of one CTA");
   static_assert(kMats * BN * 128 * 4 <= kStages * kStage, "a cluster's partial sums fit the stages");
@@ -74,7 +78,8 @@ struct FewCfg {
 struct FewParams {
   int K, nkb, N, Nb;                  // Nb: 128-feature tiles
   const float* sw[2];                 // scales of the matrix (or of gate and up)
-  const int32_t* slots;
+  const int32_t* slots;               // slot list, or ids of one token's rows (experts > 0)
+  int experts;
   int M;
   const float* sx;                    // SRC_CODES: token scales [nkb][lds]
   long long lds;
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
   if (!p.early) griddep_wait();
-  const int n_slots = slot_count(p.slots, p.M, BN), n_items = n_slots * p.Nb;
+  const int n_slots = slot_count(p.slots, p.experts, p.M, BN), n_items = n_slots * p.Nb;
   auto load_weights = [&](int s, const Slot& slot, int f0, int kb) {
     mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : C::kStage - C::kBTile);
     tc::tma_load_2d(smem + s * C::kStage, &tw0, kb * 128, slot.e * p.N + f0, &full[s]);
@@ -214,23 +219,23 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
   };
   if (p.early) {
     if (tid == 128 && cid < n_items) {
-      const Slot slot = slot_at(p.slots, p.M, BN, cid % n_slots);
+      const Slot slot = slot_at(p.slots, p.experts, p.M, BN, cid % n_slots);
       for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i, slot, cid / n_slots * 128, kb0 + i);
     }
     griddep_wait();
   }
   griddep_launch_dependents();
 
-  float acc[C::kCols];
+  f32x2 acc[C::kCols / 2];  // sums of two tokens each
   if (warp == 4) {
     // ------------------------------------------------------------ weights (and codes of the tokens) by TMA
     if (lane == 0) {
       uint32_t it = 0;
       Slot next = {};
-      if (cid < n_items) next = slot_at(p.slots, p.M, BN, cid % n_slots);  // one item ahead
+      if (cid < n_items) next = slot_at(p.slots, p.experts, p.M, BN, cid % n_slots);  // one item ahead
       for (int w = cid; w < n_items && !abort_flag[0]; w += n_cid) {
         const Slot slot = next;
-        if (w + n_cid < n_items) next = slot_at(p.slots, p.M, BN, (w + n_cid) % n_slots);
+        if (w + n_cid < n_items) next = slot_at(p.slots, p.experts, p.M, BN, (w + n_cid) % n_slots);
         const int f0 = w / n_slots * 128;
         for (int i = 0; i < n_it; ++i, ++it) {
           const int s = it % C::kStages;
@@ -288,15 +293,16 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
     // ------------------------------------------------------------ scale and add
     constexpr int kLanes = (BN + 31) / 32;  // tokens per lane
     const int feat = 32 * warp + lane;
+    float* mul = reinterpret_cast<float*>(smem + C::kMulAt) + warp * 2 * C::kCols;
     uint32_t it = 0;
     for (int w = cid; w < n_items; w += n_cid) {
-      const Slot slot = slot_at(p.slots, p.M, BN, w % n_slots);
+      const Slot slot = slot_at(p.slots, p.experts, p.M, BN, w % n_slots);
       const int ft = w / n_slots, ntok = min(BN, slot.end - slot.row0);
       const float* swp[C::kMats];
 #pragma unroll
       for (int m = 0; m < C::kMats; ++m) swp[m] = p.sw[m] + ((long long)slot.e * p.Nb + ft) * p.nkb + kb0;
 #pragma unroll
-      for (int j = 0; j < C::kCols; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < C::kCols / 2; ++j) acc[j] = 0ull;
       // The next block's scales, tokens lane, lane + 32, ...; multiplied
       // where they are used, so that nothing waits for the loads before that.
       float sn[kLanes], wn[C::kMats];
@@ -329,6 +335,14 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
         tc::fence_after();
         // the quantizing warps wrote this block's token scales before its MMA ran
         if constexpr (SRC != SRC_CODES) sc[0] = sring[(it % C::kRing) * BN + (lane & (BN - 1))];
+        // sx * sw of all tokens where every lane can read four at a time
+        float* mu = mul + (it & 1) * C::kCols;
+#pragma unroll
+        for (int m = 0; m < C::kMats; ++m)
+#pragma unroll
+          for (int c = 0; c < kLanes; ++c)
+            if (BN >= 32 || lane < BN) mu[m * BN + 32 * c + lane] = sc[c] * wc[m];
+        __syncwarp();
         const uint32_t ta = tmem + b * C::kCols + ((uint32_t)(32 * warp) << 16);
 #pragma unroll
         for (int c = 0; c < C::kCols / 16; ++c) {
@@ -340,12 +354,11 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[b]);
           }
-          const int m = 16 * c / BN, t0 = 16 * c - m * BN;
-          const float sm = sc[t0 / 32] * wc[m];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float s = __shfl_sync(0xffffffffu, sm, (t0 + j) & 31);
-            acc[16 * c + j] = fmaf(__uint_as_float(v[j]), s, acc[16 * c + j]);
+          for (int j = 0; j < 4; ++j) {
+            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(mu + 16 * c + 4 * j);
+            fma2(acc[8 * c + 2 * j], pair(v[4 * j], v[4 * j + 1]), s.x);
+            fma2(acc[8 * c + 2 * j + 1], pair(v[4 * j + 2], v[4 * j + 3]), s.y);
           }
         }
       }
@@ -364,9 +377,11 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
       for (int c = 0; c < BN / 16; ++c) {
         if (16 * c < ntok) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            red[j * 128 + feat] = acc[16 * c + j];
-            if constexpr (PAIR) red[(16 + j) * 128 + feat] = acc[BN + 16 * c + j];
+          for (int j = 0; j < 16 * C::kMats; j += 2) {
+            float x, y;
+            unpair(acc[(j < 16 ? 16 * c + j : BN + 16 * c + j - 16) / 2], x, y);
+            red[j * 128 + feat] = x;
+            red[(j + 1) * 128 + feat] = y;
           }
           const int count = min(16, ntok - 16 * c);
           if constexpr (PAIR) {
@@ -389,17 +404,20 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
   } else if constexpr (SRC != SRC_CODES) {
     // ------------------------------------------------------------ quantize the tokens: warp q takes iterations q, q + 6, ...
     static_assert(SRC == SRC_CODES || BN == 16, "in-kernel quantization serves 16 tokens");
-    // A warp at iteration i has seen the MMA of i - kQuantWarps - kStages
-    // complete; that must cover i - 2 kStages, or the parity it waits for
-    // would be that of the phase before.
-    static_assert(SRC == SRC_CODES || kQuantWarps <= C::kStages, "a quantizing warp may not lap the stages");
+    // At iteration i a warp waits for the MMA of i - kStages by the parity of
+    // the stage's barrier, which must not be a phase further back: the MMA of
+    // i - 2 kStages has to be known complete.  The warp's last wait was for
+    // the MMA of i - kQuantWarps - kStages, and a complete MMA means that all
+    // those kAcc and more before it are (the sums are read in order).
+    static_assert(SRC == SRC_CODES || C::kStages == kQuantWarps || C::kStages >= kQuantWarps + C::kAcc,
+                  "a quantizing warp may not lap the stages");
     static_assert(C::kAcc <= C::kStages, "nor an issuing one");
     typedef typename SrcType<SRC>::T T;
     const int half = lane >> 4, l = lane & 15;
     uint32_t it = 0, mine = warp - 5 - C::kIssue;
     bool ok = true;
     for (int w = cid; w < n_items && ok; w += n_cid) {
-      const Slot slot = slot_at(p.slots, p.M, BN, w % n_slots);
+      const Slot slot = slot_at(p.slots, p.experts, p.M, BN, w % n_slots);
       const int ntok = min(BN, slot.end - slot.row0);
       const uint32_t end = it + n_it;
       if (mine < end) {
@@ -409,49 +427,74 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
           at = slot.row0 + l;
           if (p.order) at = p.order[at] / p.kdiv;
           at *= p.ldx;
+          // The activations come into L2 ahead of the loads, which would
+          // each wait behind the weights in memory otherwise.
+          if (warp == 5 + C::kIssue && half == 0 && p.vec && w == cid) {
+            const int n = min(p.K, kb1 * 128) - kb0 * 128;
+            prefetch_l2(reinterpret_cast<const T*>(p.X) + at + kb0 * 128, (uint32_t)(n * sizeof(T)) & ~15u);
+          }
         }
         for (; mine < end; mine += kQuantWarps) {
           const int s = mine % C::kStages, k0 = (kb0 + (int)(mine - it)) * 128, k = k0 + 8 * l;
           uint8_t* tile = smem + s * C::kStage + C::kMats * kATile;
-          auto put = [&](int m, const float (&v)[8]) {
-            const GroupScale g = group_scale(half_warp_max(amax8(v)));
-            const uint2 c = codes8(v, g.mul);
-            // row m of the K-major SWIZZLE_128B tile: 16-byte chunk j sits at chunk j ^ (m % 8)
-            *reinterpret_cast<uint2*>(tile + m * 128 + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8) = c;
-            if (l == 0) sring[(mine % C::kRing) * BN + m] = g.scale;
+          // codes of row m, whose scale this lane or another one has stored:
+          // row m of the K-major SWIZZLE_128B tile, whose 16-byte chunk j sits
+          // at chunk j ^ (m % 8)
+          auto put = [&](int m, const float (&v)[8], float factor) {
+            *reinterpret_cast<uint2*>(tile + m * 128 + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8) = codes8(v, factor);
           };
+          float* my_scales = sring + (mine % C::kRing) * BN;
           auto stage_free = [&]() -> bool {
             return __all_sync(0xffffffffu, mine < C::kStages ||
                                                mbar_wait(&empty[s], ((mine / C::kStages) & 1) ^ 1, p.timeout_ns));
           };
-          if (p.vec && k0 + 128 <= p.K) {
-            // all loads of (half) a block in flight before the first value is used
-            constexpr int kVec = sizeof(T) == 4 ? 2 : 1, kRounds = 8 / kVec;
+          // All loads of ROUNDS row pairs in flight before the first value is
+          // used; the maxima of all rows reduced together, and lane r of a
+          // half warp divides for its row r alone.
+          constexpr int kVec = sizeof(T) == 4 ? 2 : 1;
+          auto rows = [&](auto rounds) {
+            constexpr int ROUNDS = decltype(rounds)::value;
+#pragma unroll 1
+            for (int r0 = 0; 2 * r0 < ntok; r0 += ROUNDS) {
+              uint4 raw[ROUNDS][kVec];
 #pragma unroll
-            for (int r0 = 0; r0 < 8; r0 += kRounds) {
-              if (2 * r0 < ntok) {
-                uint4 raw[kRounds][kVec];
+              for (int r = 0; r < ROUNDS; ++r) {
+                const int m = 2 * (r0 + r) + half;
+                const T* row = reinterpret_cast<const T*>(p.X) + __shfl_sync(0xffffffffu, at, m) + k;
 #pragma unroll
-                for (int r = 0; r < kRounds; ++r) {
-                  const int m = 2 * (r0 + r) + half;
-                  const long long row = __shfl_sync(0xffffffffu, at, m);
+                for (int q = 0; q < kVec; ++q) raw[r][q] = load16_if(reinterpret_cast<const uint4*>(row) + q, m < ntok);
+              }
+              uint32_t am[ROUNDS];
 #pragma unroll
-                  for (int q = 0; q < kVec; ++q)
-                    raw[r][q] = m < ntok ? *(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.X) + row + k) + q)
-                                         : make_uint4(0u, 0u, 0u, 0u);
-                }
-                if (r0 == 0 && !stage_free()) ok = false;
+              for (int r = 0; r < ROUNDS; ++r) {
+                float v[8];
+                unpack8<T>(raw[r], v);
+                am[r] = amax8(v);
+              }
 #pragma unroll
-                for (int r = 0; r < kRounds; ++r) {
-                  const int m = 2 * (r0 + r);
-                  if (m < ntok) {
-                    float v[8];
-                    load8(reinterpret_cast<const T*>(raw[r]), 8, true, v);
-                    put(m + half, v);
-                  }
-                }
+              for (int d = 8; d; d >>= 1)
+#pragma unroll
+                for (int r = 0; r < ROUNDS; ++r) am[r] = max(am[r], __shfl_xor_sync(0xffffffffu, am[r], d));
+              uint32_t my_am = am[0];
+#pragma unroll
+              for (int r = 1; r < ROUNDS; ++r) my_am = (l & (ROUNDS - 1)) == r ? am[r] : my_am;
+              const GroupScale g = group_scale(my_am);
+              if (r0 == 0 && !stage_free()) ok = false;
+              if (l < ROUNDS) my_scales[2 * (r0 + l) + half] = g.scale;
+#pragma unroll
+              for (int r = 0; r < ROUNDS; ++r) {
+                const float factor = __shfl_sync(0xffffffffu, g.mul, r, 16);
+                float v[8];
+                unpack8<T>(raw[r], v);
+                put(2 * (r0 + r) + half, v, factor);
               }
             }
+          };
+          if (ntok <= 0) {
+            if (!stage_free()) ok = false;  // a row without an expert: nothing reads the codes
+          } else if (p.vec && k0 + 128 <= p.K) {
+            if (ntok <= 2) rows(std::integral_constant<int, 1>());
+            else rows(std::integral_constant<int, 4 / kVec>());
           } else {
             if (!stage_free()) ok = false;
 #pragma unroll 1
@@ -459,7 +502,9 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
               const long long row = __shfl_sync(0xffffffffu, at, m);
               float v[8];
               load8(reinterpret_cast<const T*>(p.X) + row + k, m < ntok ? p.K - k : 0, false, v);
-              put(m, v);
+              const GroupScale g = group_scale(half_warp_max(amax8(v)));
+              put(m, v, g.mul);
+              if (l == 0) my_scales[m] = g.scale;
             }
           }
           if (!ok) {
@@ -483,25 +528,32 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
     // the partial sums added in rank order.
     float* part = reinterpret_cast<float*>(smem);
     const bool on = cid < n_items;
-    const Slot slot = on ? slot_at(p.slots, p.M, BN, cid % n_slots) : Slot{};
+    const Slot slot = on ? slot_at(p.slots, p.experts, p.M, BN, cid % n_slots) : Slot{};
     const int ft = on ? cid / n_slots : 0, ntok = on ? min(BN, slot.end - slot.row0) : 0;
     const int feat = 32 * warp + lane, f0 = 128 * ft;
     if (warp < 4 && on) {
 #pragma unroll
-      for (int j = 0; j < C::kCols; ++j)
-        if ((j & (BN - 1)) < ntok) part[j * 128 + feat] = acc[j];
+      for (int j = 0; j < C::kCols; j += 2)
+        if ((j & (BN - 1)) < ntok) {
+          float x, y;
+          unpair(acc[j / 2], x, y);
+          part[j * 128 + feat] = x;
+          part[(j + 1) * 128 + feat] = y;
+        }
     }
     __syncthreads();
     tc::cluster_sync();
-    if (warp < 4 && on && !abort_flag[0]) {
-      // a warp per token, 4 features per lane, all ranks' loads in flight
+    if ((!PAIR || warp < 4) && on && !abort_flag[0]) {
+      // a warp (of all, or of those that quantize) per token, 4 features per
+      // lane, all ranks' loads in flight
+      const int n_warps = PAIR ? 4 : (int)(blockDim.x >> 5);
       const int f4 = 4 * lane, n4 = f0 + f4;
       float bias[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) bias[q] = (!PAIR && p.bias && n4 + q < p.N) ? __ldg(p.bias + n4 + q) : 0.0f;
       const int count = rank < ntok ? (ntok - 1 - rank) / split + 1 : 0;
 #pragma unroll 1
-      for (int i = warp; i < count; i += 4) {
+      for (int i = warp; i < count; i += n_warps) {
         const int j = rank + i * split;
         float4 x[C::kMats][8];
 #pragma unroll
@@ -682,7 +734,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_wait();
   griddep_launch_dependents();
-  const int n_slots = slot_count(p.slots, p.M, 128);
+  const int n_slots = slot_count(p.slots, 0, p.M, 128);
   const int n_work = n_slots * p.n_tiles;
   if ((int)blockIdx.x >= n_work) return;
 
@@ -714,10 +766,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // tile together (all tokens stay in L2), a grouped one the feature
       // tiles of one token tile (its expert's weights do).
       auto slot_of = [&](int t) { return p.slots ? t / p.n_tiles : t % n_slots; };
-      Slot next = slot_at(p.slots, p.M, 128, slot_of(blockIdx.x));  // one tile ahead
+      Slot next = slot_at(p.slots, 0, p.M, 128, slot_of(blockIdx.x));  // one tile ahead
       for (int t = blockIdx.x; t < n_work; t += gridDim.x) {
         const Slot slot = next;
-        if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, p.M, 128, slot_of(t + gridDim.x));
+        if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, 0, p.M, 128, slot_of(t + gridDim.x));
         const int nt = p.slots ? t % p.n_tiles : t / n_slots, f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
         // lanes 0 and 1 fetch the features' scales, every lane those of the
         // rows lane, lane + 32, ...; a row past the end takes the last row's
@@ -1119,6 +1171,7 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   p.sw[0] = w->scales;
   p.sw[1] = a.w[1] ? a.w[1]->scales : w->scales;
   p.slots = a.slots;
+  p.experts = a.experts;
   p.M = a.rows;
   p.sx = a.sx;
   p.lds = a.lds;

@@ -17,6 +17,7 @@ namespace fp8 {
 struct Product {
   const mtc_fp8_matrix* w[2] = {nullptr, nullptr};  // w[1]: the up matrix of a gate / up pair
   const int32_t* slots = nullptr;                   // device slot list, or null for a dense product
+  int experts = 0;                                  // > 0: slots are the expert ids of one token's rows
   int slot_bound = 0;                               // slots of the launch at most
   int rows = 0;                                     // rows of the token operand
   int tile = 128;                                   // rows per slot

@@ -80,6 +80,8 @@ def route(logits, k, score="softmax", bias=None, n_groups=1, top_groups=1, renor
     else:
         s = torch.where(masked, torch.zeros_like(z), 1 / (1 + torch.exp(-z)))
     c = s if bias is None else s + bias.double()
+    if bias is None and n_groups == 1:
+        c = z  # the order of the scores, also where they meet in 64 bits
     c = torch.where(masked, torch.full_like(c, -math.inf), c)
     T, E = c.shape
     dropped = torch.zeros_like(masked)

@@ -268,3 +268,24 @@ def test_refusals(dev):
         ExpertsFP8(lambda v: v, gate, up, down, 2)(x)
     with pytest.raises(ValueError, match="fit"):
         ExpertsFP8(lambda v: v, gate, up, gate, 2)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_choices_next_to_a_border(dev, score):
+    """Choices closer than fp32 tells apart, at the last place and at the
+    groups' border: decided in 64 bits."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    base = torch.randn(200, 1, device=dev, generator=g).expand(-1, 64)
+    z = base + 2e-7 * torch.randn(200, 64, device=dev, generator=g)
+    b = 1e-8 * torch.randn(64, device=dev, generator=g)
+    same_routing(z, 8, score=score)
+    same_routing(z, 8, score=score, bias=b)
+    same_routing(z, 8, score=score, bias=b, n_groups=8, top_groups=3)
+    same_routing(z, 6, score=score, n_groups=4, top_groups=2, renormalize=False)
+    same_routing(torch.zeros(5, 64, device=dev), 8, score=score, bias=b, n_groups=8, top_groups=2)
+
+
+def test_one_token_with_rows_of_no_expert(dev):
+    ids = torch.tensor([[3, -1, 7, 3, 8, 2 ** 30]], dtype=torch.int32, device=dev)
+    forward(dev, 1, 8, 6, 200, 130, torch.float32, ids=ids)
+    forward(dev, 1, 8, 6, 200, 130, torch.bfloat16, ids=torch.full_like(ids, -5))
