@@ -21,6 +21,8 @@ struct RouteParams {
   int T, E, k, sigmoid;
   const float* bias;
   int groups, gsize, top_groups, renorm;
+  uint32_t by_group;     // e / gsize = e * by_group >> 20 for e < 1024
+  int lanes;             // lanes that look at a group (a power of two)
   double scale;
   int32_t* ids;
   float* weights;
@@ -54,7 +56,7 @@ template <typename F>
 __device__ __forceinline__ F raw_score(float z, float zmax, bool sigmoid) {
   if (z == -INFINITY) return (F)0;
   if (sizeof(F) == 8) return sigmoid ? 1.0 / (1.0 + exp(-(double)z)) : exp((double)z - (double)zmax);
-  return sigmoid ? 1.0f / (1.0f + expf(-z)) : expf(z - zmax);
+  return sigmoid ? __fdividef(1.0f, 1.0f + __expf(-z)) : __expf(z - zmax);
 }
 
 // Bits of the experts' groups that are kept, one per group at bit g * lanes,
@@ -108,10 +110,12 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteParams& p, const F* c
 // not (about one token in a hundred).
 //
 // Error of an fp32 choice s + b, with M = max(|s + b| + s): the rounding of
-// the sum is below 2^-24 M; a sigmoid's relative error below 6 * 2^-24; a
-// softmax score's below (16 + d) * 2^-24 for a logit d below the largest (the
-// difference, expf, the total, the division), where s d is below s log(1/s)
-// and so (16 + d) s below 22 M.  Twice that is below 2^-20 M and 2^-18 M.
+// the sum is below 2^-24 M.  __expf(x) is off by 2 ulp and |x| 2^-24, the
+// division by 2 ulp.  A sigmoid's error is below ((4 + |z|)(1 - s) + 5) s
+// 2^-24, where |z| s (1 - s) < 0.3; a softmax score's below (20 + 2 d) s 2^-24
+// for a logit d below the largest (the difference, its exponential, the
+// total, the division), where s d < s log(1/s) and so 2 s d < 5 M.  Twice
+// that is below 2^-19 M and 2^-17 M.
 //
 // 64 bits for all: 29.3 us for 8192 x 256 with groups and bias.
 template <typename T, int NPL>
@@ -138,8 +142,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   }
   if (!p.sigmoid) zmax = warp_max(zmax);
   const bool by_logit = !p.bias && p.groups == 1;
-  int lanes = 1;
-  while (2 * lanes * p.groups <= 32) lanes *= 2;
+  const int lanes = p.lanes;
 
   uint32_t key[NPL];
   float margin = 0.0f;
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
       if (v[i] == -INFINITY) c[i] = -INFINITY;
       else most = fmaxf(most, fabsf(c[i]) + sc);
     }
-    margin = warp_max(most) * (p.sigmoid ? 9.5367431640625e-7f : 3.814697265625e-6f);
+    margin = warp_max(most) * (p.sigmoid ? 1.9073486328125e-6f : 7.62939453125e-6f);
     uint32_t keep = ~0u;
     if (p.groups > 1) {
       float* cs = reinterpret_cast<float*>(route_smem + warp * p.E);
@@ -184,32 +187,43 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int e = 32 * i + lane;
-      key[i] = e < p.E && (p.groups == 1 || (keep >> (e / p.gsize * lanes) & 1u)) ? order_key(c[i]) : 0u;
+      key[i] = e < p.E && (p.groups == 1 || (keep >> ((e * p.by_group >> 20) * lanes) & 1u)) ? order_key(c[i]) : 0u;
     }
   }
-  int my_id = 0;
-  uint32_t before = 0u;
-  for (int j = 0; j <= p.k && sure; ++j) {
-    if (j == p.k && by_logit) break;
-    uint32_t best = 0u;
-    int at = 0;
+  // k (+ 1, for the margin of the last place) rounds: every lane knows its
+  // best key, the winner looks for its next one
+  int my_id = 0, at = 0;
+  uint32_t before = 0u, best = 0u;
 #pragma unroll
-    for (int i = 0; i < NPL; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
-      }
+  for (int i = 0; i < NPL; ++i)
+    if (key[i] > best) {
+      best = key[i];
+      at = i;
+    }
+  const int rounds = by_logit ? p.k : p.k + 1;
+#pragma unroll 1
+  for (int j = 0; j < rounds; ++j) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    if (!by_logit && j > 0 && before > 1u && top > 1u) sure = key_value(before) - key_value(top) > margin;
-    before = top;
+    if (!by_logit) {
+      if (j > 0 && before > 1u && top > 1u && !(key_value(before) - key_value(top) > margin)) sure = false;
+      if (!sure || j == p.k) break;
+      before = top;
+    }
     const uint32_t mine = best == top ? (uint32_t)(32 * at + lane) : ~0u;
     const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
-    if (mine == id) {
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (i == at) key[i] = 0u;
-    }
     if (lane == j) my_id = (int)id;
+    if (mine == id) {
+      const int gone = at;
+      best = 0u;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        if (i == gone) key[i] = 0u;
+        if (key[i] > best) {
+          best = key[i];
+          at = i;
+        }
+      }
+    }
   }
   if (!sure) {
     double* cs = route_smem + warp * p.E;
@@ -241,7 +255,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
       int at = 0;
       for (int i = 0; i < NPL; ++i) {
         const int e = 32 * i + lane;
-        if (e >= p.E || (done >> i & 1ull) || !(p.groups == 1 || (keep >> (e / p.gsize * lanes) & 1u))) continue;
+        if (e >= p.E || (done >> i & 1ull) || !(p.groups == 1 || (keep >> ((e * p.by_group >> 20) * lanes) & 1u))) continue;
         const unsigned long long o = order_key(cs[e]);
         if (o > best) {
           best = o;
@@ -573,6 +587,9 @@ extern "C" int mtc_route_experts(const void* logits, int32_t type, int32_t T, in
   p.bias = bias;
   p.groups = groups == top_groups ? 1 : groups;  // every group kept: no limit
   p.gsize = E / groups;
+  p.by_group = ((1u << 20) + p.gsize - 1) / p.gsize;
+  p.lanes = 1;
+  while (2 * p.lanes * groups <= 32) p.lanes *= 2;
   p.top_groups = top_groups;
   p.renorm = renormalize != 0;
   p.scale = (double)scale;
