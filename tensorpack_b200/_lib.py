@@ -146,6 +146,8 @@ _lib = None
 def load(path: str = LIB_PATH):
     """Load (once) and return the ctypes library with prototypes attached."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

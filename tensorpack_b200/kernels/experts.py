@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .fp8 import _TYPES, FP8Experts, _check_output, _current_device, _ld, _raw_stream, _rows
+from .fp8 import _TYPES, FP8Experts, _check_output, _current_device, _empty, _raw_stream, _rows
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
@@ -54,14 +54,16 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
             return route_experts(logits, top_k, score=score, bias=bias, n_groups=n_groups, top_groups=top_groups,
                                  renormalize=renormalize, scale=scale)
     if bias is not None:
-        bias = torch.as_tensor(bias, dtype=torch.float32, device=dev).reshape(-1).contiguous()
-        if bias.numel() != E:
-            raise ValueError(f"route_experts: bias has {bias.numel()} values, there are {E} experts")
-    ids = logits.new_empty((T, top_k), dtype=torch.int32)
-    weights = logits.new_empty((T, top_k), dtype=torch.float32)
+        if not (isinstance(bias, torch.Tensor) and bias.dtype == torch.float32 and bias.device == dev
+                and bias.dim() == 1 and bias.is_contiguous()):
+            bias = torch.as_tensor(bias, dtype=torch.float32, device=dev).reshape(-1).contiguous()
+        if bias.shape[0] != E:
+            raise ValueError(f"route_experts: bias has {bias.shape[0]} values, there are {E} experts")
+    ids = _empty((T, top_k), (top_k, 1), dtype=torch.int32, device=dev)
+    weights = _empty((T, top_k), (top_k, 1), dtype=torch.float32, device=dev)
     if T:
         rc = _lib.load().mtc_route_experts(
-            logits.data_ptr(), _TYPES[logits.dtype], T, E, _ld(logits), top_k, _lib.SCORES[score],
+            logits.data_ptr(), _TYPES[logits.dtype], T, E, logits.stride(0) if T > 1 else E, top_k, _lib.SCORES[score],
             None if bias is None else bias.data_ptr(), n_groups, top_groups, bool(renormalize), scale, ids.data_ptr(),
             weights.data_ptr(), _raw_stream(dev.index))
         if rc:
@@ -85,54 +87,57 @@ def experts_forward(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, g
     for m in (gate, up, down):
         if not isinstance(m, FP8Experts) or len(m.shape) != 3:
             raise TypeError("experts_forward: gate, up and down must be FP8Experts")
-    if _current_device() != X.device.index:
-        with torch.cuda.device(X.device):
+    dev = X.device
+    index = dev.index
+    if _current_device() != index:
+        with torch.cuda.device(dev):
             return experts_forward(X, ids, weights, gate, up, down, activation=activation, Y=Y, out_dtype=out_dtype)
     T, D = X.shape
     E, K, I = gate.shape
-    dev = X.device
     assert D == K, f"Shape mismatch: {tuple(X.shape)} vs {gate.shape}"
-    if up.shape != (E, D, I) or down.shape != (E, I, D):
+    if up.shape != gate.shape or down.shape != (E, I, D):
         raise ValueError(f"experts_forward: gate {gate.shape}, up {up.shape} and down {down.shape} do not fit")
     if E > MAX_EXPERTS:
         raise ValueError(f"experts_forward: {E} experts, at most {MAX_EXPERTS}")
-    if any(m.device != dev for m in (gate, up, down)) or ids.device != dev or weights.device != dev:
+    if gate.device != dev or up.device != dev or down.device != dev or ids.device != dev or weights.device != dev:
         raise ValueError(f"experts_forward: all operands must be on {dev}")
-    if ids.dim() != 2 or ids.shape[0] != T or ids.shape != weights.shape or not 1 <= ids.shape[1] <= MAX_TOP_K:
-        raise ValueError(f"experts_forward: ids {tuple(ids.shape)} and weights {tuple(weights.shape)} for {T} tokens "
+    shape = ids.shape
+    if len(shape) != 2 or shape[0] != T or shape != weights.shape or not 1 <= shape[1] <= MAX_TOP_K:
+        raise ValueError(f"experts_forward: ids {tuple(shape)} and weights {tuple(weights.shape)} for {T} tokens "
                          f"(1..{MAX_TOP_K} experts each)")
     if ids.dtype != torch.int32:
         if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
             raise ValueError(f"experts_forward: ids of type {ids.dtype}")
         # (an id that does not fit 32 bits is no expert either)
-        ids = torch.where((ids >= 0) & (ids < E), ids, torch.full_like(ids, -1) if ids.dtype.is_signed else E).to(
-            torch.int32)
-    if activation not in _lib.ACTIVATIONS:
+        ids = ids.to(torch.int64)
+        ids = torch.where((ids >= 0) & (ids < E), ids, torch.full_like(ids, -1)).to(torch.int32)
+    act = _lib.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"unknown activation {activation!r} (one of relu, silu, gelu_tanh)")
     if weights.dtype != torch.float32:
         weights = weights.to(torch.float32)
     ids, weights = ids.contiguous(), weights.contiguous()
-    k = ids.shape[1]
+    k = shape[1]
     if Y is None:
-        if out_dtype is None:
-            out_dtype = torch.float32
-        elif out_dtype not in _TYPES:
-            raise ValueError(f"experts_forward: output type {out_dtype} (one of float32, bfloat16, float16)")
-        Y, ldy = X.new_empty((T, D), dtype=out_dtype), D
+        y_type = _TYPES.get(out_dtype)
+        if y_type is None:
+            if out_dtype is not None:
+                raise ValueError(f"experts_forward: output type {out_dtype} (one of float32, bfloat16, float16)")
+            out_dtype, y_type = torch.float32, _lib.F32
+        Y, ldy = _empty((T, D), (D, 1), dtype=out_dtype, device=dev), D
     else:
         _check_output(Y, (T, D), out_dtype, dev, (X, ids, weights), "experts_forward")
-        ldy = Y.stride(0) if T > 1 else D
+        y_type, ldy = _TYPES[Y.dtype], Y.stride(0) if T > 1 else D
     if T:
         lib = _lib.load()
-        y_type = _TYPES[Y.dtype]
         need = lib.mtc_experts_workspace_bytes(gate._ref, T, k, y_type)
         if not need:
             raise ValueError(f"experts_forward: too many rows ({T} x {k})")
-        ws = X.new_empty(need, dtype=torch.uint8)
+        ws = _empty((need,), (1,), dtype=torch.uint8, device=dev)
         rc = lib.mtc_experts_forward(
-            gate._ref, up._ref, down._ref, X.data_ptr(), _TYPES[X.dtype], T, _ld(X), ids.data_ptr(),
-            weights.data_ptr(), k, _lib.ACTIVATIONS[activation], Y.data_ptr(), y_type, ldy, ws.data_ptr(), need,
-            gate._status_ptr, _raw_stream(dev.index))
+            gate._ref, up._ref, down._ref, X.data_ptr(), _TYPES[X.dtype], T, X.stride(0) if T > 1 else D,
+            ids.data_ptr(), weights.data_ptr(), k, act, Y.data_ptr(), y_type, ldy, ws.data_ptr(), need,
+            gate._status_ptr, _raw_stream(index))
         if rc:
             _lib.check(rc, "experts")
     return Y

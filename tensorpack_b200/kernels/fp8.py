@@ -37,6 +37,8 @@ _CODES = torch.float8_e4m3fn
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = torch.cuda.current_device
+# (the cheapest of torch's allocations: 1.5 us against 2 to 2.4 for empty and new_empty)
+_empty = torch.empty_strided
 
 
 def _cuda_device(device=None) -> torch.device:
@@ -255,14 +257,14 @@ def fp8_quantize(X: torch.Tensor):
     if K < 1:
         raise ValueError("fp8_quantize: rows without values")
     ld, kb = -(-K // 16) * 16, -(-K // BLOCK)
-    codes = X.new_empty((M, ld), dtype=_CODES)
-    scales = X.new_empty((kb, M), dtype=torch.float32)
+    codes = _empty((M, ld), (ld, 1), dtype=_CODES, device=dev)
+    scales = _empty((M, kb), (1, M), dtype=torch.float32, device=dev)
     if M:
-        rc = _lib.load().mtc_fp8_quantize(X.data_ptr(), _TYPES[X.dtype], M, K, _ld(X), codes.data_ptr(), ld,
-                                          scales.data_ptr(), M, _raw_stream(dev.index))
+        rc = _lib.load().mtc_fp8_quantize(X.data_ptr(), _TYPES[X.dtype], M, K, X.stride(0) if M > 1 else K,
+                                          codes.data_ptr(), ld, scales.data_ptr(), M, _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "fp8 quantize")
-    return codes[:, :K] if ld != K else codes, scales.T
+    return codes if ld == K else codes[:, :K], scales
 
 
 def fp8_gemm(X, W: FP8Matrix, bias=None, activation: Optional[str] = None, Y=None, *, out_dtype=None):
@@ -284,10 +286,12 @@ def fp8_gemm(X, W: FP8Matrix, bias=None, activation: Optional[str] = None, Y=Non
     X = _rows(X, "fp8_gemm")
     if X.device != dev:
         raise ValueError(f"fp8_gemm: activations on {X.device}, weights on {dev}")
-    if _current_device() != dev.index:
+    index = dev.index
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return fp8_gemm(X, W, bias, activation, Y, out_dtype=out_dtype)
-    (M, K), (K2, N) = X.shape, W.shape
+    M, K = X.shape
+    K2, N = W.shape
     assert K == K2, f"Shape mismatch: {tuple(X.shape)} vs {W.shape}"
     ep = None
     if bias is not None:
@@ -296,25 +300,28 @@ def fp8_gemm(X, W: FP8Matrix, bias=None, activation: Optional[str] = None, Y=Non
             bias = torch.as_tensor(bias, dtype=torch.float32, device=dev).reshape(-1).contiguous()
         if bias.shape[0] != N:
             raise ValueError(f"bias has {bias.shape[0]} values, the output {N} columns")
-    if bias is not None or activation is not None:
         ep = _ep(epilogue(bias, activation))
+    elif activation is not None:
+        ep = _ep(epilogue(None, activation))
     if Y is None:
-        if out_dtype is None:
-            out_dtype = torch.float32
-        elif out_dtype not in _TYPES:
-            raise ValueError(f"fp8_gemm: output type {out_dtype} (one of float32, bfloat16, float16)")
-        Y, ldy = X.new_empty((M, N), dtype=out_dtype), N
+        y_type = _TYPES.get(out_dtype)
+        if y_type is None:
+            if out_dtype is not None:
+                raise ValueError(f"fp8_gemm: output type {out_dtype} (one of float32, bfloat16, float16)")
+            out_dtype, y_type = torch.float32, _lib.F32
+        Y, ldy = _empty((M, N), (N, 1), dtype=out_dtype, device=dev), N
     else:
         _check_output(Y, (M, N), out_dtype, dev, (X,) if bias is None else (X, bias), "fp8_gemm")
-        ldy = Y.stride(0) if M > 1 else N
+        y_type, ldy = _TYPES[Y.dtype], Y.stride(0) if M > 1 else N
     if M:
         lib = _lib.load()
-        ws, need = None, 0
+        at, need = None, 0
         if M > RAW_MAX_M:
             need = lib.mtc_fp8_gemm_workspace_bytes(W._ref, M)
-            ws = X.new_empty(need, dtype=torch.uint8)
-        rc = lib.mtc_fp8_gemm(W._ref, X.data_ptr(), _TYPES[X.dtype], M, _ld(X), Y.data_ptr(), _TYPES[Y.dtype], ldy,
-                              None if ws is None else ws.data_ptr(), need, W._status_ptr, ep, _raw_stream(dev.index))
+            ws = _empty((need,), (1,), dtype=torch.uint8, device=dev)
+            at = ws.data_ptr()
+        rc = lib.mtc_fp8_gemm(W._ref, X.data_ptr(), _TYPES[X.dtype], M, X.stride(0) if M > 1 else K, Y.data_ptr(),
+                              y_type, ldy, at, need, W._status_ptr, ep, _raw_stream(index))
         if rc:
             _lib.check(rc, "fp8 gemm")
     return Y
