@@ -457,8 +457,8 @@ MTC_API int mtc_fp8_pack(const float* W, int32_t K, int32_t N, int64_t ldw, uint
 MTC_API int mtc_fp8_unpack(const mtc_fp8_matrix* w, int32_t e, float* out, int64_t ldo, void* stream);
 
 /* Activations X (M x K, type MTC_F32 / BF16 / F16, row stride ldx) to codes
- * (M rows of ldq bytes, ldq a multiple of 16; bytes from K to ldq are
- * written as zero) and scales (scales[b * lds + m] for inputs 128 b .. 128 b
+ * (M rows of ldq bytes, ldq a multiple of 16; bytes from K on are left as
+ * they are) and scales (scales[b * lds + m] for inputs 128 b .. 128 b
  * + 127 of row m), by the rule of mtc_fp8_pack per row and 128 inputs. */
 MTC_API int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_t K, int64_t ldx, uint8_t* codes,
                              int64_t ldq, float* scales, int64_t lds, void* stream);

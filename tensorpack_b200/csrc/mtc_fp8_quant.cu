@@ -19,6 +19,16 @@ struct QuantParams {
   long long lds;
 };
 
+// Eight codes of a row of which `left` values exist (VEC: all or none).
+template <bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* q, const uint2& c, int left) {
+  if (left >= 8) {
+    *reinterpret_cast<uint2*>(q) = c;
+  } else if (!VEC) {
+    for (int i = 0; i < left; ++i) q[i] = (uint8_t)((i < 4 ? c.x >> (8 * i) : c.y >> (8 * i - 32)) & 0xffu);
+  }
+}
+
 // One half warp per group of 128 inputs, 8 values per lane, U groups at a
 // time: their loads are in flight together, their maxima reduced together, and
 // lane u of the half warp divides for group u alone.  Bound by memory:
@@ -80,17 +90,16 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
     for (int u = 0; u < U; ++u) {
       const uint2 c = codes8(v[u], __shfl_sync(0xffffffffu, gs.mul, u, 16));
       if (mm[u] < 0) continue;
-      // (k is a multiple of 8 and ldq of 16, so a lane's 8 codes stay inside the row)
       const int k = bb[u] * kBlock + 8 * l;
       if (p.pos) {
         for (int j = 0; j < p.copies; ++j) {
           const int r = p.pos[(long long)mm[u] * p.copies + j];
           if (r < 0) continue;
-          if (k < p.ldq) *reinterpret_cast<uint2*>(p.q + (long long)r * p.ldq + k) = c;
+          store_codes<VEC>(p.q + (long long)r * p.ldq + k, c, p.K - k);
           if (l == u) p.s[(long long)bb[u] * p.lds + r] = gs.scale;
         }
       } else {
-        if (k < p.ldq) *reinterpret_cast<uint2*>(p.q + (long long)mm[u] * p.ldq + k) = c;
+        store_codes<VEC>(p.q + (long long)mm[u] * p.ldq + k, c, p.K - k);
         if (l == u) p.s[(long long)bb[u] * p.lds + mm[u]] = gs.scale;
       }
     }

@@ -257,14 +257,14 @@ def fp8_quantize(X: torch.Tensor):
     if K < 1:
         raise ValueError("fp8_quantize: rows without values")
     ld, kb = -(-K // 16) * 16, -(-K // BLOCK)
-    codes = _empty((M, ld), (ld, 1), dtype=_CODES, device=dev)
+    codes = _empty((M, K), (ld, 1), dtype=_CODES, device=dev)
     scales = _empty((M, kb), (1, M), dtype=torch.float32, device=dev)
     if M:
         rc = _lib.load().mtc_fp8_quantize(X.data_ptr(), _TYPES[X.dtype], M, K, X.stride(0) if M > 1 else K,
                                           codes.data_ptr(), ld, scales.data_ptr(), M, _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "fp8 quantize")
-    return codes if ld == K else codes[:, :K], scales
+    return codes, scales
 
 
 def fp8_gemm(X, W: FP8Matrix, bias=None, activation: Optional[str] = None, Y=None, *, out_dtype=None):
