@@ -32,12 +32,12 @@ struct RouteParams {
 // NaN) expert, key 0 one that may not be chosen.
 __device__ __forceinline__ unsigned long long order_key(double c) {
   if (!(c > -INFINITY)) return 1ull;  // -inf, NaN
-  const long long b = __double_as_longlong(c);
+  const long long b = __double_as_longlong(c + 0.0);  // (-0 is 0)
   return (unsigned long long)b ^ (b < 0 ? ~0ull : 0x8000000000000000ull);
 }
 __device__ __forceinline__ uint32_t order_key(float c) {
   if (!(c > -INFINITY)) return 1u;
-  const uint32_t b = __float_as_uint(c);
+  const uint32_t b = __float_as_uint(c + 0.0f);
   return b ^ ((int)b < 0 ? ~0u : 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
@@ -102,12 +102,30 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteParams& p, const F* c
   return __ballot_sync(0xffffffffu, kept && sub == 0);
 }
 
-// A warp per token.  The choice is made in 64 bits as defined, but reached in
-// 32 where that is certain: without bias and groups the order of the scores
-// is that of the logits; otherwise the fp32 choices are taken when every
-// decision (between neighbours of the k + 1 best, at the groups' border) has
-// a margin above the fp32 error, and computed again in 64 bits when one has
-// not (about one token in a hundred).
+// Descending order by a network of compare-exchanges (Batcher's odd-even
+// merge sort).
+template <int N>
+__device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+    for (int q = p; q >= 1; q >>= 1)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b);
+            k[i + j + q] = min(a, b);
+          }
+}
+
+// A warp per token.  The choice is made in 64 bits as defined (without bias
+// and groups by the logits), but reached in 32 where that is certain: the
+// fp32 choices are taken when every decision (between neighbours of the k + 1
+// best, at the groups' border) has a margin above the error, and made again
+// in 64 bits when one has not (about one token in a hundred).
 //
 // Error of an fp32 choice s + b, with M = max(|s + b| + s): the rounding of
 // the sum is below 2^-24 M.  __expf(x) is off by 2 ulp and |x| 2^-24, the
@@ -117,9 +135,11 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteParams& p, const F* c
 // total, the division), where s d < s log(1/s) and so 2 s d < 5 M.  Twice
 // that is below 2^-19 M and 2^-17 M.
 //
-// 64 bits for all: 29.3 us for 8192 x 256 with groups and bias.
+// 8192 x 256 with groups and bias: 22.3 us (24.7 in 64 bits for all, which
+// also has twice the registers), bound by instruction issue; 24.8 without the
+// limit on registers that lets 48 warps share an SM.
 template <typename T, int NPL>
-__global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(256, NPL <= 8 ? 6 : 1) route_kernel(const RouteParams p) {
   extern __shared__ double route_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * (blockDim.x >> 5) + warp;
@@ -144,34 +164,47 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   const bool by_logit = !p.bias && p.groups == 1;
   const int lanes = p.lanes;
 
+  // Keys in 32 bits whose last bits hold the lane's index of the expert, so
+  // that a lane sorts values and indices at once.  What these bits hide goes
+  // into the margin.
+  constexpr uint32_t kLow = NPL - 1;
   uint32_t key[NPL];
-  float margin = 0.0f;
+  float margin;
   bool sure = true;
-  if (by_logit) {
+  {
+    float c[NPL], most = 0.0f;
+    if (by_logit) {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) key[i] = 32 * i + lane < p.E ? order_key(v[i]) : 0u;
-  } else {
-    float c[NPL], sum = 0.0f, most = 0.0f;
+      for (int i = 0; i < NPL; ++i) {
+        c[i] = v[i];
+        if (v[i] != -INFINITY) most = fmaxf(most, fabsf(v[i]));
+      }
+    } else {
+      float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      c[i] = raw_score<float>(v[i], zmax, p.sigmoid);
-      sum += c[i];
+      for (int i = 0; i < NPL; ++i) {
+        c[i] = raw_score<float>(v[i], zmax, p.sigmoid);
+        sum += c[i];
+      }
+      float inv = 1.0f;
+      if (!p.sigmoid) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        inv = __fdividef(1.0f, sum);
+      }
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        const int e = 32 * i + lane;
+        const float sc = c[i] * inv;
+        c[i] = p.bias && e < p.E ? sc + p.bias[e] : sc;
+        if (v[i] == -INFINITY) c[i] = -INFINITY;
+        else most = fmaxf(most, fabsf(c[i]) + sc);
+      }
     }
-    float inv = 1.0f;
-    if (!p.sigmoid) {
-#pragma unroll
-      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      inv = 1.0f / sum;
-    }
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      const int e = 32 * i + lane;
-      const float sc = c[i] * inv;
-      c[i] = p.bias && e < p.E ? sc + p.bias[e] : sc;
-      if (v[i] == -INFINITY) c[i] = -INFINITY;
-      else most = fmaxf(most, fabsf(c[i]) + sc);
-    }
-    margin = warp_max(most) * (p.sigmoid ? 1.9073486328125e-6f : 7.62939453125e-6f);
+    most = warp_max(most);
+    // (the hidden bits: below NPL ulp of each)
+    margin = most * ((by_logit ? 0.0f : p.sigmoid ? 1.9073486328125e-6f : 7.62939453125e-6f) +
+                     2.0f * NPL * 1.1920928955078125e-7f);
     uint32_t keep = ~0u;
     if (p.groups > 1) {
       float* cs = reinterpret_cast<float*>(route_smem + warp * p.E);
@@ -187,86 +220,84 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int e = 32 * i + lane;
-      key[i] = e < p.E && (p.groups == 1 || (keep >> ((e * p.by_group >> 20) * lanes) & 1u)) ? order_key(c[i]) : 0u;
+      const uint32_t o = (order_key(c[i]) & ~kLow) | (kLow - i);  // a tie goes to the lowest index
+      key[i] = e < p.E && (p.groups == 1 || (keep >> ((e * p.by_group >> 20) * lanes) & 1u)) ? o : 0u;
     }
   }
-  // k (+ 1, for the margin of the last place) rounds: every lane knows its
-  // best key, the winner looks for its next one
-  int my_id = 0, at = 0;
-  uint32_t before = 0u, best = 0u;
-#pragma unroll
-  for (int i = 0; i < NPL; ++i)
-    if (key[i] > best) {
-      best = key[i];
-      at = i;
-    }
-  const int rounds = by_logit ? p.k : p.k + 1;
+  sort_descending(key);
+  // k + 1 rounds (the last for the margin of the last place): the best of the
+  // lanes' first keys; its lane moves its others up
+  int my_id = 0;
+  uint32_t before = 0u;
 #pragma unroll 1
-  for (int j = 0; j < rounds; ++j) {
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    if (!by_logit) {
-      if (j > 0 && before > 1u && top > 1u && !(key_value(before) - key_value(top) > margin)) sure = false;
-      if (!sure || j == p.k) break;
-      before = top;
-    }
-    const uint32_t mine = best == top ? (uint32_t)(32 * at + lane) : ~0u;
-    const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
-    if (lane == j) my_id = (int)id;
-    if (mine == id) {
-      const int gone = at;
-      best = 0u;
+  for (int j = 0; j <= p.k; ++j) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
+    if (j > 0 && top > 2 * kLow + 1 && !(key_value(before & ~kLow) - key_value(top & ~kLow) > margin)) sure = false;
+    if (j < p.k && top <= 2 * kLow + 1) sure = false;  // only masked experts are left: by index
+    if (!sure || j == p.k) break;
+    before = top;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == top)) - 1;
+    if (lane == j) my_id = (int)(32 * (kLow - (top & kLow))) + owner;
+    if (lane == owner) {
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        if (i == gone) key[i] = 0u;
-        if (key[i] > best) {
-          best = key[i];
-          at = i;
-        }
-      }
+      for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
+      key[NPL - 1] = 0u;
     }
   }
   if (!sure) {
-    double* cs = route_smem + warp * p.E;
-    double sum = 0.0;
+    // all of it in 64 bits, in registers (a warp that comes here is the one
+    // the others' end waits for)
+    unsigned long long wide[NPL];
+    double c[NPL], sum = 0.0;
+#pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      float x = 32 * i + lane < p.E ? to_f32(z[32 * i + lane]) : -INFINITY;
-      if (x != x) x = -INFINITY;
-      x = fminf(x, 3.402823466e38f);
-      const double sc = raw_score<double>(x, zmax, p.sigmoid);
-      sum += sc;
-      if (32 * i + lane < p.E) cs[32 * i + lane] = x == -INFINITY ? (double)-INFINITY : sc;
+      c[i] = by_logit ? (double)v[i] : raw_score<double>(v[i], zmax, p.sigmoid);
+      sum += c[i];
     }
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    for (int e = lane; e < p.E; e += 32) {
-      double c = cs[e];
-      if (c != -INFINITY) {
-        if (!p.sigmoid) c = c / sum;
-        if (p.bias) c += (double)p.bias[e];
-        cs[e] = c;
+    if (!by_logit) {
+      if (!p.sigmoid) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      }
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        if (!p.sigmoid) c[i] = c[i] / sum;
+        if (p.bias && 32 * i + lane < p.E) c[i] += (double)p.bias[32 * i + lane];
+        if (v[i] == -INFINITY) c[i] = -INFINITY;
       }
     }
-    __syncwarp();
     uint32_t keep = ~0u;
-    double gap;
-    if (p.groups > 1) keep = keep_groups<double>(p, cs, lane, lanes, &gap);
-    unsigned long long done = 0ull;  // this lane's experts that are taken, by i (at most 32)
+    if (p.groups > 1) {
+      double* cs = route_smem + warp * p.E;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i)
+        if (32 * i + lane < p.E) cs[32 * i + lane] = c[i];
+      __syncwarp();
+      double gap;
+      keep = keep_groups<double>(p, cs, lane, lanes, &gap);
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const int e = 32 * i + lane;
+      wide[i] = e < p.E && (p.groups == 1 || (keep >> ((e * p.by_group >> 20) * lanes) & 1u)) ? order_key(c[i]) : 0ull;
+    }
+#pragma unroll 1
     for (int j = 0; j < p.k; ++j) {
       unsigned long long best = 0ull;
       int at = 0;
-      for (int i = 0; i < NPL; ++i) {
-        const int e = 32 * i + lane;
-        if (e >= p.E || (done >> i & 1ull) || !(p.groups == 1 || (keep >> ((e * p.by_group >> 20) * lanes) & 1u))) continue;
-        const unsigned long long o = order_key(cs[e]);
-        if (o > best) {
-          best = o;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i)
+        if (wide[i] > best) {
+          best = wide[i];
           at = i;
         }
-      }
       const uint32_t hi = (uint32_t)(best >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
       const uint32_t lo = hi == mh ? (uint32_t)best : 0u, ml = __reduce_max_sync(0xffffffffu, lo);
       const uint32_t mine = (hi == mh && lo == ml) ? (uint32_t)(32 * at + lane) : ~0u;
       const uint32_t id = __reduce_min_sync(0xffffffffu, mine);
-      if (mine == id) done |= 1ull << at;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i)
+        if (mine == id && i == at) wide[i] = 0ull;
       if (lane == j) my_id = (int)id;
     }
   }
@@ -537,9 +568,8 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
 
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t st) {
-  const bool by_logit = !p.bias && p.groups == 1;
-  const int warps = !by_logit && p.E > 512 ? 4 : 8;
-  const size_t smem = by_logit ? 0 : (size_t)warps * p.E * 8;
+  const int warps = p.E > 512 ? 4 : 8;
+  const size_t smem = (size_t)warps * p.E * 8;
   auto go = [&](auto kernel) -> int {
     if (smem > 48 * 1024)
       MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),

@@ -283,6 +283,9 @@ def test_choices_next_to_a_border(dev, score):
     same_routing(z, 8, score=score, bias=b, n_groups=8, top_groups=3)
     same_routing(z, 6, score=score, n_groups=4, top_groups=2, renormalize=False)
     same_routing(torch.zeros(5, 64, device=dev), 8, score=score, bias=b, n_groups=8, top_groups=2)
+    signs = torch.where(torch.randn(20, 64, device=dev, generator=g) < 0, -0.0, 0.0)
+    same_routing(signs, 8, score=score)
+    same_routing(signs, 8, score=score, n_groups=8, top_groups=2)
 
 
 def test_one_token_with_rows_of_no_expert(dev):
