@@ -74,21 +74,6 @@ __device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {
   return m;
 }
 
-// Element types of activations and outputs (mtc_dtype of the C ABI).
-template <int DT>
-struct Elem;
-template <>
-struct Elem<MTC_F32> {
-  typedef float T;
-};
-template <>
-struct Elem<MTC_BF16> {
-  typedef __nv_bfloat16 T;
-};
-template <>
-struct Elem<MTC_F16> {
-  typedef __half T;
-};
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }

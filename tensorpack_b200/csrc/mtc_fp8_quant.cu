@@ -32,11 +32,12 @@ __device__ __forceinline__ void store_codes(uint8_t* q, const uint2& c, int left
 // One half warp per group of 128 inputs, 8 values per lane, U groups at a
 // time: their loads are in flight together, their maxima reduced together, and
 // lane u of the half warp divides for group u alone.  Bound by memory:
-// 4096 x 14336 fp32 took 64.3 us one group at a time with every lane dividing
-// (4.6 TB/s).
-template <typename T, bool VEC>
+// 4096 x 14336 fp32 takes 49.9 us (5.9 TB/s; 64.3 us one group at a time with
+// every lane dividing).  U = 1 when a half warp has one group at most:
+// 333 x 4864 fp16 and the product after it take 17.0 us, 19.2 with U = 4.
+template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
-  constexpr int U = sizeof(T) == 4 ? 2 : 4, kVec = sizeof(T) == 4 ? 2 : 1;
+  constexpr int kVec = sizeof(T) == 4 ? 2 : 1;
   const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
   griddep_wait();
   griddep_launch_dependents();
@@ -175,13 +176,21 @@ int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
   p.lds = a.lds;
   // whole vectors: rows that start on 16 bytes and hold a multiple of 8 values
   const bool vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % (a.dt == MTC_F32 ? 4 : 8) == 0 && a.K % 8 == 0;
-  const long long blocks = ((long long)a.M * p.Kb + 15) / 16;
   const int sms = sm_count();
   MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
-  const int grid = (int)(blocks < 8ll * sms ? blocks : 8ll * sms);
-  auto kernel = a.dt == MTC_F32    ? (vec ? quantize_kernel<float, true> : quantize_kernel<float, false>)
-                : a.dt == MTC_BF16 ? (vec ? quantize_kernel<__nv_bfloat16, true> : quantize_kernel<__nv_bfloat16, false>)
-                                   : (vec ? quantize_kernel<__half, true> : quantize_kernel<__half, false>);
+  // 8 CTAs of 256 threads per SM hold all that fits; more groups than their
+  // half warps are taken several at a time
+  const long long blocks = ((long long)a.M * p.Kb + 15) / 16;
+  const bool many = blocks > 8ll * sms;
+  const int grid = (int)(many ? 8ll * sms : blocks);
+  void (*kernel)(QuantParams);
+#define MTC_PICK(T, U) \
+  (vec ? (many ? quantize_kernel<T, true, U> : quantize_kernel<T, true, 1>) \
+       : (many ? quantize_kernel<T, false, U> : quantize_kernel<T, false, 1>))
+  if (a.dt == MTC_F32) kernel = MTC_PICK(float, 2);
+  else if (a.dt == MTC_BF16) kernel = MTC_PICK(__nv_bfloat16, 4);
+  else kernel = MTC_PICK(__half, 4);
+#undef MTC_PICK
   MTC_CHECK_CUDA(launch_chained(kernel, dim3(grid), dim3(256), 0, st, 1, p), who);
   return MTC_OK;
 }
