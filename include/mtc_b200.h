@@ -466,9 +466,11 @@ MTC_API int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_t K
 /* Y = act(Xq @ W + bias) for one matrix (E = 1): X is quantized as by
  * mtc_fp8_quantize, products of codes are exact, sums are fp32 (128 inputs on
  * the tensor cores, the scaled sums of the blocks in order), Y is rounded
- * once to its type.  Up to 16 rows need no workspace (the kernel quantizes
+ * once to its type.  Up to 8 rows need no workspace (the kernel quantizes
  * them itself); `ws` is 256-byte aligned, its size from
- * mtc_fp8_gemm_workspace_bytes on the same device.  Same inputs, same bits. */
+ * mtc_fp8_gemm_workspace_bytes.  `status` (one word on the device, or NULL)
+ * gets MTC_STATUS_TIMEOUT when a pipeline wait ran out.  Same inputs, same
+ * bits. */
 MTC_API size_t mtc_fp8_gemm_workspace_bytes(const mtc_fp8_matrix* w, int32_t M);
 MTC_API int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type, int32_t M, int64_t ldx, void* Y,
                          int32_t y_type, int64_t ldy, void* ws, size_t ws_bytes, uint32_t* status,
@@ -477,9 +479,9 @@ MTC_API int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type,
 /* Routing of T tokens to k of E experts (E <= 1024, k <= 32) from router
  * logits (T x E, row stride ld).  Scores: softmax over the experts, or
  * sigmoid.  The choice goes by score + bias (bias: E finite floats, or NULL)
- * in 64 bits; without bias and groups by the logits, whose order that is.  With groups > 1 (at most 32, dividing E) only the experts of
- * the top_groups groups with the largest sum of their two best choices
- * compete.  ids: the k best, best first, ties to the lowest index; weights:
+ * in 64 bits; without bias and groups by the logits, whose order that is.
+ * With groups > 1 (at most 32, dividing E) only the experts of the top_groups
+ * groups with the largest sum of their two best choices compete.  ids: the k best, best first, ties to the lowest index; weights:
  * their scores (without bias), divided by their sum if renormalize, times
  * scale.  A logit of -inf or NaN is a masked expert: score 0, chosen only
  * when no other is left; +inf counts as the largest finite number.  A row

@@ -516,9 +516,16 @@ bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16;
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How the experts' products run, from the mean number of rows of an expert:
-// up to 8, 16-row tiles whose tokens the first product quantizes itself; up
-// to 48, wider tiles of codes; above, the 128-token kernel.  A single token
-// needs no plan: every row is a slot.
+// up to 12, 16-row tiles whose tokens the first product quantizes itself; up
+// to 20, 32-row tiles of codes; above, the 128-token kernel.  Device times
+// of the three at a mean of m rows:
+//    64 experts, 2048 x 1024:   m = 12  93 / 102 / 119 us   m = 16  107 / 107 / 120
+//                               m = 20 131 / 117 / 125      m = 24  142 / 127 / 125
+//   128 experts, 2048 x 768:    m = 8  121 / 134 / 165      m = 16  161 / 152 / 168
+//     8 experts, 4096 x 14336:  m = 8  264 / 276 / 277      m = 16  334 / 296 / 281
+//   256 experts, 1024 x 512:    m = 8   99 / 106 / 132      m = 24  182 / 151 / 140
+// A single token needs no plan: every row is a slot (20.2 us a call with 8 of
+// 64 experts, 25.7 with a plan).
 struct ExpertsPlan {
   int R, tile, slot_bound;
   bool direct, raw, many;
@@ -528,13 +535,13 @@ struct ExpertsPlan {
 };
 bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   const long long R = (long long)T * k;
-  if (R > 0x7fff0000ll) return false;
+  if (R > kMaxRows || (long long)T * ((D + 2047) / 2048) > kMaxRows) return false;
   pl->R = (int)R;
   const double mean = (double)R / E;
   pl->direct = T == 1;
-  pl->raw = pl->direct || mean <= 8.0;
-  pl->many = !pl->raw && mean > 48.0;
-  pl->tile = pl->raw ? 16 : mean <= 24.0 ? 32 : pl->many ? 128 : 64;
+  pl->raw = pl->direct || mean <= 12.0;
+  pl->many = !pl->raw && mean > 20.0;
+  pl->tile = pl->raw ? 16 : pl->many ? 128 : 32;
   const long long used = R < E ? R : E;
   long long bound = R / pl->tile + used;
   if (bound > R || pl->direct) bound = R;
@@ -569,11 +576,8 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t st) {
   const int warps = p.E > 512 ? 4 : 8;
-  const size_t smem = (size_t)warps * p.E * 8;
+  const size_t smem = (size_t)warps * p.E * 8;  // the choices, where groups compare them: 32 KB at most
   auto go = [&](auto kernel) -> int {
-    if (smem > 48 * 1024)
-      MTC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                     "mtc_route_experts");
     MTC_CHECK_CUDA(launch_chained(kernel, dim3((p.T + warps - 1) / warps), dim3(32 * warps), smem, st, 1, p),
                    "mtc_route_experts");
     return MTC_OK;
@@ -600,7 +604,7 @@ extern "C" int mtc_route_experts(const void* logits, int32_t type, int32_t T, in
   MTC_REQUIRE(logits && ids && weights, "mtc_route_experts: null pointer");
   MTC_REQUIRE(dtype_ok(type), "mtc_route_experts: unknown element type %d", type);
   MTC_REQUIRE(score == MTC_SCORE_SOFTMAX || score == MTC_SCORE_SIGMOID, "mtc_route_experts: unknown score %d", score);
-  MTC_REQUIRE(T >= 0 && E >= 1 && E <= kMaxExperts && ld >= E, "mtc_route_experts: bad shape (T=%d, E=%d, ld=%lld)", T,
+  MTC_REQUIRE(T >= 0 && T <= kMaxRows && E >= 1 && E <= kMaxExperts && ld >= E, "mtc_route_experts: bad shape (T=%d, E=%d, ld=%lld)", T,
               E, (long long)ld);
   MTC_REQUIRE(groups >= 1 && groups <= kMaxGroups && E % groups == 0 && top_groups >= 1 && top_groups <= groups,
               "mtc_route_experts: %d experts in %d groups, %d of them kept", E, groups, top_groups);

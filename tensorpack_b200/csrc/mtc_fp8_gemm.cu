@@ -1026,6 +1026,7 @@ int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap
   return MTC_OK;
 }
 
+// Tiles that gate / up pairs come in, too.
 template <int BN, int SRC>
 int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid,
                bool pair, cudaStream_t st, const char* who) {
@@ -1090,6 +1091,7 @@ int encode_codes_map(CUtensorMap* map, const uint8_t* codes, long long ld, long 
 int check_matrix(const mtc_fp8_matrix* w, const char* who) {
   MTC_REQUIRE(w && w->codes && w->scales, "%s: null matrix", who);
   MTC_REQUIRE(w->K >= 1 && w->N >= 1 && w->E >= 1, "%s: bad matrix shape %d x (%d, %d)", who, w->E, w->K, w->N);
+  MTC_REQUIRE(w->K <= kMaxRows && w->N <= kMaxRows, "%s: more than 2^31 inputs or outputs", who);
   MTC_REQUIRE(w->ldk >= w->K && (w->ldk & 15) == 0, "%s: row stride %lld of the codes is not a multiple of 16 >= K",
               who, (long long)w->ldk);
   MTC_REQUIRE((reinterpret_cast<uintptr_t>(w->codes) & 15) == 0, "%s: codes not 16-byte aligned", who);
@@ -1114,6 +1116,7 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   const int sms = sm_count();
   MTC_REQUIRE(sms > 0, "%s: no CUDA device", who);
   if (a.slot_bound <= 0) return MTC_OK;
+  MTC_REQUIRE((long long)a.slot_bound * Nb <= kMaxRows, "%s: more than 2^31 tiles", who);
   CUtensorMap tw[2], tx;
   for (int i = 0; i < n_mats; ++i) {
     const mtc_fp8_matrix* m = a.w[i];
@@ -1211,13 +1214,13 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   const int grid = split > 1 ? (int)bound * split : (int)(bound < sms ? bound : sms);
   const bool pair = n_mats == 2;
   if (a.xq) {
+    // (pairs in tiles of 16 bring activations, those in tiles of 32 codes)
+    if (a.tile == 32) return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
+    MTC_REQUIRE(!pair, "%s: a gate / up pair in tiles of %d rows", who, a.tile);
     switch (a.tile) {
-      case 16: return launch_few<16, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
-      case 32: return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
-      case 64: return launch_few<64, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
-      default:
-        MTC_REQUIRE(!pair, "%s: a gate / up pair in tiles of %d rows", who, a.tile);
-        return launch_few<128, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
+      case 16: return launch_few<16, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
+      case 64: return launch_few<64, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
+      default: return launch_few<128, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
     }
   }
   p.X = a.X;

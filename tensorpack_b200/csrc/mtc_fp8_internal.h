@@ -45,6 +45,10 @@ struct Product {
   uint32_t* status = nullptr;
 };
 
+// Rows of an operand, and tiles of a product, at most: indexes of rows, of
+// tiles and of the blocks behind the last one stay below 2^31.
+constexpr long long kMaxRows = 0x7fff0000ll;
+
 int check_matrix(const mtc_fp8_matrix* w, const char* who);
 int sm_count();
 

@@ -198,9 +198,17 @@ int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
 namespace {
 bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16; }
 
-// Rows of one token tile of a dense product: the kernel for few rows up to
-// 128 of them, in tiles that waste at most half of the MMA; above, the
-// 128 x 256 tiles, once there are enough of them to occupy the SMs.
+// How a dense product runs.  Times on the device, weights from memory.
+//  * Up to 8 rows the product quantizes the activations itself: 13.7 us at
+//    8 x 4096 x 14336 against 15.1 with the quantizer before it (its codes
+//    are loaded like the weights); 17.8 against 15.6 with 10 rows.
+//  * The kernel for few rows takes them in tiles that waste at most half of
+//    the MMA.  From 65 rows on the 128 x 256 tiles take over where the few
+//    kernel could not split its inputs any more, that is, where its 128 x 128
+//    tiles fill more than half of the SMs: 26 against 48 us at
+//    129 x 4096 x 14336, 18.0 / 18.7 at 256 x 2048 x 8192 (128 tiles), but
+//    24.4 / 18.4 at 200 x 4096 x 4096 (64), 13.3 / 12.3 at 700 x 1024 x 1536
+//    (72) and 43 / 14.7 at 333 x 4864 x 901 (24).
 struct DensePlan {
   int tile;
   bool many, raw;
@@ -209,10 +217,9 @@ struct DensePlan {
 };
 DensePlan dense_plan(int M, int K, int N, int sms) {
   DensePlan d;
-  const long long many_tiles = (long long)((M + 127) / 128) * ((N + 255) / 256);
-  d.many = M > 128 && many_tiles >= sms;
-  d.tile = d.many || M > 64 ? 128 : M > 32 ? 64 : M > 16 ? 32 : 16;
-  d.raw = M <= 16;
+  d.many = M > 64 && 2ll * ((M + 127) / 128) * ((N + 127) / 128) > sms;
+  d.tile = M > 64 ? 128 : M > 32 ? 64 : M > 16 ? 32 : 16;
+  d.raw = M <= 8;
   d.ldq = (K + 15) & ~15ll;
   d.lds = (M + 3) & ~3ll;
   d.q_bytes = d.raw ? 0 : (((size_t)M * d.ldq + 255) & ~(size_t)255);
@@ -258,7 +265,7 @@ extern "C" int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_
   clear_error();
   MTC_REQUIRE(X && codes && scales, "mtc_fp8_quantize: null pointer");
   MTC_REQUIRE(dtype_ok(x_type), "mtc_fp8_quantize: unknown element type %d", x_type);
-  MTC_REQUIRE(M >= 0 && K >= 1 && ldx >= K, "mtc_fp8_quantize: bad shape (M=%d, K=%d, ldx=%lld)", M, K,
+  MTC_REQUIRE(M >= 0 && M <= kMaxRows && K >= 1 && K <= kMaxRows && ldx >= K, "mtc_fp8_quantize: bad shape (M=%d, K=%d, ldx=%lld)", M, K,
               (long long)ldx);
   MTC_REQUIRE(ldq >= K && (ldq & 15) == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && lds >= M,
               "mtc_fp8_quantize: codes need rows of a multiple of 16 bytes >= K and 16-byte alignment");
@@ -276,9 +283,8 @@ extern "C" int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_
 }
 
 extern "C" size_t mtc_fp8_gemm_workspace_bytes(const mtc_fp8_matrix* w, int32_t M) {
-  if (!w || M < 1 || w->K < 1) return 0;
-  const int sms = sm_count();
-  return dense_plan(M, w->K, w->N, sms > 0 ? sms : 1).bytes;
+  if (!w || M < 1 || M > kMaxRows || w->K < 1) return 0;
+  return dense_plan(M, w->K, w->N, 1).bytes;  // (the number of SMs does not enter it)
 }
 
 extern "C" int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type, int32_t M, int64_t ldx, void* Y,
@@ -290,7 +296,7 @@ extern "C" int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_ty
   MTC_REQUIRE(w->E == 1, "mtc_fp8_gemm: %d stacked matrices", w->E);
   MTC_REQUIRE(X && Y, "mtc_fp8_gemm: null pointer");
   MTC_REQUIRE(dtype_ok(x_type) && dtype_ok(y_type), "mtc_fp8_gemm: unknown element type");
-  MTC_REQUIRE(M >= 1 && ldx >= w->K && ldy >= w->N, "mtc_fp8_gemm: bad shape (M=%d, ldx=%lld, ldy=%lld)", M,
+  MTC_REQUIRE(M >= 1 && M <= kMaxRows && ldx >= w->K && ldy >= w->N, "mtc_fp8_gemm: bad shape (M=%d, ldx=%lld, ldy=%lld)", M,
               (long long)ldx, (long long)ldy);
   EpiArg epa;
   rc = read_epilogue(ep, &epa, "mtc_fp8_gemm");

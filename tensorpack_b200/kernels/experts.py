@@ -30,7 +30,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     Scores are the softmax over the experts or the sigmoid of the logits.
     The experts are chosen by score + ``bias`` (E finite floats, to balance
     their load), compared in 64 bits (without bias and groups by the logits,
-    whose order that is), best first, ties to the lowest index.  With ``n_groups`` > 1 only the experts of the ``top_groups`` groups (equal
+    whose order that is), best first, ties to the lowest index.  With
+    ``n_groups`` > 1 only the experts of the ``top_groups`` groups (equal
     consecutive parts of the E experts) with the largest sum of their two best
     choices compete.  The weights are the scores without the bias, divided by
     their sum if ``renormalize``, times ``scale``.

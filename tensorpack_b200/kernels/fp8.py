@@ -27,7 +27,7 @@ from .. import _lib
 from .device import _ep, epilogue
 
 BLOCK = 128            # inputs (and outputs) that share a scale
-RAW_MAX_M = 16         # largest M whose activations the product quantizes itself (no workspace)
+RAW_MAX_M = 8          # largest M whose activations the product quantizes itself (no workspace)
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _CODES = torch.float8_e4m3fn
 
@@ -70,10 +70,6 @@ def _rows(X: torch.Tensor, what: str) -> torch.Tensor:
     if (X.shape[1] > 1 and X.stride(1) != 1) or (X.shape[0] > 1 and X.stride(0) < X.shape[1]):
         X = X.contiguous()
     return X
-
-
-def _ld(X: torch.Tensor) -> int:
-    return X.stride(0) if X.shape[0] > 1 else X.shape[1]
 
 
 def _span(t: torch.Tensor):

@@ -33,7 +33,7 @@ def gemm(lib, w, x_type=0, M=1, ldx=256, y_type=0, ldy=128, X=P, Y=P, ep=None):
 @pytest.mark.parametrize("kw,text", [
     (dict(codes=None), b"null"), (dict(scales=None), b"null"), (dict(K=0), b"shape"), (dict(N=-1), b"shape"),
     (dict(E=0), b"shape"), (dict(ldk=250), b"stride"), (dict(ldk=240), b"stride"), (dict(codes=4104), b"aligned"),
-    (dict(E=1 << 20, N=1 << 20), b"2^31"),
+    (dict(E=1 << 20, N=1 << 20), b"2^31"), (dict(K=2 ** 31 - 1, ldk=2 ** 31), b"2^31"),
 ])
 def test_bad_matrices_are_refused(lib, kw, text):
     assert gemm(lib, matrix(**kw)) == _lib.MTC_ERR_INVALID
@@ -42,7 +42,7 @@ def test_bad_matrices_are_refused(lib, kw, text):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(X=None), b"null"), (dict(Y=None), b"null"), (dict(x_type=3), b"type"), (dict(y_type=-1), b"type"),
-    (dict(M=0), b"shape"), (dict(ldx=255), b"shape"), (dict(ldy=127), b"shape"),
+    (dict(M=0), b"shape"), (dict(M=2 ** 31 - 1), b"shape"), (dict(ldx=255), b"shape"), (dict(ldy=127), b"shape"),
 ])
 def test_bad_products_are_refused(lib, kw, text):
     assert gemm(lib, matrix(), **kw) == _lib.MTC_ERR_INVALID
@@ -59,7 +59,8 @@ def test_dense_product_takes_one_matrix_and_a_known_activation(lib):
 def test_bad_quantize_arguments_are_refused(lib):
     ok = dict(X=P, t=0, M=2, K=100, ldx=100, q=P, ldq=112, s=P, lds=2)
     for bad in (dict(X=None), dict(t=5), dict(K=0), dict(ldx=99), dict(q=None), dict(ldq=100), dict(ldq=96),
-                dict(q=P + 8), dict(s=None), dict(lds=1), dict(M=-1)):
+                dict(q=P + 8), dict(s=None), dict(lds=1), dict(M=-1), dict(M=2 ** 31 - 1, lds=2 ** 31),
+                dict(K=2 ** 31 - 1, ldx=2 ** 31, ldq=2 ** 31)):
         a = {**ok, **bad}
         assert lib.mtc_fp8_quantize(a["X"], a["t"], a["M"], a["K"], a["ldx"], a["q"], a["ldq"], a["s"], a["lds"],
                                     None) == _lib.MTC_ERR_INVALID, bad
@@ -70,7 +71,7 @@ def test_bad_quantize_arguments_are_refused(lib):
 @pytest.mark.parametrize("kw", [
     dict(logits=None), dict(t=4), dict(E=0), dict(E=1025), dict(ld=7), dict(k=0), dict(k=9), dict(score=2),
     dict(groups=3), dict(groups=4, top=0), dict(groups=4, top=5), dict(groups=4, top=1, k=3), dict(E=64, ld=64, k=33),
-    dict(E=66, ld=66, groups=33, top=1, k=1), dict(ids=None), dict(T=-1),
+    dict(E=66, ld=66, groups=33, top=1, k=1), dict(ids=None), dict(T=-1), dict(T=2 ** 31 - 1),
 ])
 def test_bad_routing_is_refused(lib, kw):
     a = {**dict(logits=P, t=0, T=2, E=8, ld=8, k=2, score=0, groups=1, top=1, ids=P), **kw}
@@ -93,6 +94,8 @@ def test_bad_expert_products_are_refused(lib):
                dict(T=1 << 30, k=32)):
         assert call(**kw) == _lib.MTC_ERR_INVALID, kw
     assert lib.mtc_experts_workspace_bytes(ctypes.byref(gate), 1 << 30, 32, 0) == 0
+    wide = matrix(E=1, K=1 << 20, N=128, ldk=1 << 20)  # 512 parts of 2048 columns per token
+    assert lib.mtc_experts_workspace_bytes(ctypes.byref(wide), 1 << 22, 1, 0) == 0
     assert lib.mtc_experts_workspace_bytes(None, 1, 1, 0) == 0
 
 

@@ -135,6 +135,18 @@ def test_experts(dev, T, E, k, D, I, dtype):
     forward(dev, T, E, k, D, I, TYPES[dtype], activation="gelu_tanh" if T % 2 else "silu", seed=T)
 
 
+@pytest.mark.parametrize("rows", [11, 12, 13, 20, 21, 48, 49])
+def test_experts_on_both_sides_of_their_variants(dev, rows):
+    """`rows` rows per expert on average, all tokens and only some of them
+    at real experts."""
+    E, k = 6, 2
+    T = -(-rows * E // k)
+    _, ids, _, _, _ = forward(dev, T, E, k, 272, 264, torch.float32, seed=rows)
+    ids = ids.clone()
+    ids[::3] = -1
+    forward(dev, T, E, k, 272, 264, torch.bfloat16, ids=ids, seed=rows)
+
+
 @pytest.mark.parametrize("T", [1, 30, 300, 1500])
 def test_uneven_experts(dev, T):
     """All tokens at one expert, experts without tokens, the same expert

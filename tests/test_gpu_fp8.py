@@ -136,6 +136,22 @@ def test_gemm_long_and_large(dev, M, K, N):
     close(y, ref, mag, K, torch.float32)
 
 
+@pytest.mark.parametrize("M,K,N", [(7, 1300, 900), (8, 1300, 900), (9, 1300, 900), (10, 300, 40000), (64, 300, 20000),
+                                   (65, 700, 9700), (65, 700, 9400), (128, 300, 9500), (129, 264, 4700), (129, 264, 4900),
+                                   (200, 1000, 4900), (257, 129, 6400)])
+def test_gemm_on_both_sides_of_its_variants(dev, M, K, N):
+    from tensorpack_b200.kernels.fp8 import fp8_gemm
+
+    m, b = weights(K, N, N, dev), normal((N,), 9, dev)
+    for t in (torch.float32, torch.float16):
+        x = normal((M, K), M + K, dev, t)
+        y = fp8_gemm(x, m, b, "silu")
+        torch.cuda.synchronize()
+        m.check_status()
+        ref, mag = R.gemm(x, m.codes, m.scales[0], b, "silu")
+        close(y, ref, mag, K, torch.float32)
+
+
 @pytest.mark.parametrize("xt", list(TYPES))
 @pytest.mark.parametrize("yt", list(TYPES))
 @pytest.mark.parametrize("M,N", [(3, 200), (50, 200), (1300, 4000)])
