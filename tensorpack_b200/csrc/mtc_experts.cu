@@ -547,9 +547,9 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   if (bound > R || pl->direct) bound = R;
   pl->slot_bound = (int)bound;
   pl->ldx = (D + 15) & ~15ll;
-  pl->ldh = (I + 15) & ~15ll;
+  pl->ldh = (I + 31) & ~31ll;
   pl->lds = (R + 3) & ~3ll;
-  pl->ldo = (D + 7) & ~7ll;
+  pl->ldo = (D + 15) & ~15ll;
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t here = at;

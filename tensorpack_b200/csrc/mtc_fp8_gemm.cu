@@ -613,12 +613,10 @@ constexpr int kManyStages = 4;
 constexpr uint32_t kManyStage = 3 * kATile;
 constexpr int kManyWarps = 8;                         // scaling warps: 2 column halves x 4 lane quadrants
 constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup with the TMA and the MMA warp
-// Staging of the output, per warp 32 rows of 64 bytes; the row stride of 5
-// 16-byte units keeps 16-byte accesses free of bank conflicts.  (More stages
-// beat more staging: with 3 stages and whole rows staged for asynchronous
-// copies the loads' latency showed, 281 against 2xx us.)
-constexpr int kRowLd = 80;
-constexpr uint32_t kStaging = 32 * kRowLd;
+// A row of each scaling thread, for values that cannot leave as vectors (the
+// stride of 5 16-byte units keeps 16-byte accesses free of bank conflicts).
+constexpr int kRowLd = 20;
+constexpr uint32_t kStaging = kManyWarps * 32 * kRowLd * 4;
 // Scales of an iteration: sx of 128 rows, sw of the two scale blocks of the
 // features, and the tile {first row, end row, feature tile}, in a ring that
 // the TMA warp fills together with a stage (4-byte asynchronous copies: rows
@@ -628,7 +626,7 @@ constexpr uint32_t kStaging = 32 * kRowLd;
 // overwritten early.
 constexpr int kScaleSlots = 8, kScaleLd = 132;
 static_assert(kScaleSlots > kManyStages + 2, "a scale slot must outlive its reader");
-constexpr uint32_t kManyScales = kManyStages * kManyStage + kManyWarps * kStaging;
+constexpr uint32_t kManyScales = kManyStages * kManyStage + kStaging;
 constexpr uint32_t kManyTiles = kManyScales + kScaleSlots * kScaleLd * 4;
 constexpr uint32_t kManyBars = kManyTiles + kScaleSlots * 16;
 constexpr size_t kManySmem = 1024 + kManyBars + 256;
@@ -646,7 +644,7 @@ struct ManyParams {
   const float* sx;
   long long lds;
   void* Y;
-  int ydt, y_bytes, vec;
+  int ydt, vec;                       // vec: rows of Y start on 32 bytes
   long long ldy;
   const float* bias;
   float one;                          // 1
@@ -658,9 +656,8 @@ struct ManyParams {
   unsigned long long timeout_ns;
 };
 
-// Barriers of the two warps that share rows (64 threads); the second form
-// tells both whether either of them passed true.
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+// Barrier of the two warps that share rows (64 threads), which tells both
+// whether either of them passed true.
 __device__ __forceinline__ bool pair_sync_or(int id, bool x) {
   uint32_t r;
   asm volatile(
@@ -674,26 +671,11 @@ __device__ __forceinline__ bool pair_sync_or(int id, bool x) {
   return r != 0;
 }
 
-// The warp's staged rows (64 bytes each) to row pieces: 4 lanes per row, 16
-// bytes per lane.  `left` bytes of every piece exist, rows from `rows` on do
-// not.  Called by whole warps.
-__device__ __forceinline__ void store_rows(uint8_t* dst, long long ld, const uint8_t* stg, int lane, int left, int rows) {
-  __syncwarp();
-  const int sub = 16 * (lane & 3);
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int rr = 8 * r + (lane >> 2);
-    if (rr < rows && sub < left) {
-      const uint8_t* src = stg + rr * kRowLd + sub;
-      uint8_t* d = dst + rr * ld + sub;
-      if (sub + 16 <= left) {
-        *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(src);
-      } else {
-        for (int i = 0; i < left - sub; i += 2) *reinterpret_cast<uint16_t*>(d + i) = *reinterpret_cast<const uint16_t*>(src + i);
-      }
-    }
-  }
-  __syncwarp();
+// 32 bytes at a 32-byte aligned address (a whole sector from one thread).
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // What becomes of the sums: stored as they are, after bias and activation
@@ -707,7 +689,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   constexpr bool GATED = MODE >= kGated;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* staging = smem + kManyStages * kManyStage;
+  float* staging = reinterpret_cast<float*>(smem + kManyStages * kManyStage);
   float* scales = reinterpret_cast<float*>(smem + kManyScales);  // [kScaleSlots][kScaleLd]
   int4* tiles = reinterpret_cast<int4*>(smem + kManyTiles);      // [kScaleSlots]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kManyBars);
@@ -832,13 +814,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // ------------------------------------------------------------ scale and add, then store
     regs_inc<kScaleRegs>();
     const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
-    uint8_t* my_row = staging + warp * kStaging + lane * kRowLd;
+    float* my_row = staging + (warp * 32 + lane) * kRowLd;
     const int my_scale = 32 * quad + lane;
-    // TMEM columns of the sums 0..63 and 64..127 (an up warp takes its halves
-    // the other way round: see below)
-    const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16) + 128 * hf;
-    const uint32_t tm_a = lanes + (GATED ? 64 * hf : 0), tm_b = lanes + (GATED ? 64 * (hf ^ 1) : 64);
+    // TMEM columns of the sums 0..63 and 64..127: 128 features, or 64 of the
+    // gate and the same 64 of the up matrix
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16);
+    const uint32_t tm_a = lanes + (GATED ? 64 : 128) * hf, tm_b = tm_a + (GATED ? 128 : 64);
     uint32_t it = 0;
+    int turn = 0;
     bool stop = false;
     for (int t = blockIdx.x; t < n_work && !stop; t += gridDim.x) {
       f32x2 acc[64];
@@ -856,8 +839,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tc::fence_after();
         // the TMA warp wrote this block's scales before its MMA ran
         const float* slot = scales + (it % kScaleSlots) * kScaleLd;
-        const float sc1 = slot[my_scale] * slot[128 + hf];
-        const f32x2 sc = pair(sc1, sc1);
+        const float sa = slot[my_scale] * slot[128 + (GATED ? 0 : hf)];
+        const float sb = GATED ? slot[my_scale] * slot[129] : sa;
+        const f32x2 sc_a = pair(sa, sa), sc_b = pair(sb, sb);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           uint32_t v[16];
@@ -869,132 +853,102 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (lane == 0) mbar_arrive(&acc_empty[b]);
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[2 * j], v[2 * j + 1]), sc);
+          for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[2 * j], v[2 * j + 1]), c < 4 ? sc_a : sc_b);
         }
       }
       const int4 tile = tiles[(it - 1) % kScaleSlots];
       const int nt = tile.z, m0 = tile.x + 32 * quad;
-      const int n0 = GATED ? nt * 128 : nt * 256 + 128 * hf;  // first feature of this warp
-      const int rows = ok ? tile.y - m0 : 0;                  // rows of this warp that exist (more than 32: all)
-      // Sums that are stored leave through a multiplication by p.one (= 1):
-      // stored directly, the compiler lays them out for the stores and moves
-      // every one of them in the main loop (466 against 415 thousand cycles
-      // at 4096 x 4096 x 14336).
-      auto sums4 = [&](int q, float (&o)[4]) {
-        unpair(acc[2 * q], o[0], o[1]);
-        unpair(acc[2 * q + 1], o[2], o[3]);
-      };
+      const int n0 = GATED ? nt * 128 + 64 * hf : nt * 256 + 128 * hf;  // first feature of this warp
+      const int left = p.N - n0;                                        // features of this warp that exist
+      const bool mine = ok && m0 + lane < tile.y;                       // this thread's row exists
       if constexpr (GATED) {
-        // The gate warp and the up warp of the same rows each finish half of
-        // the columns: sums 0..63 stay, 64..127 go to the other warp through
-        // the staged rows, 16 at a time.  The gate warp keeps columns 0..63,
-        // the up warp 64..127.
-        const uint8_t* other = staging + (warp ^ 4) * kStaging + lane * kRowLd;
-        const int n = n0 + 64 * hf, left = p.N - n;
         uint32_t am = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int j = 0; j < 32; ++j) {
+          float g[2], u[2];
+          unpair(acc[j], g[0], g[1]);
+          unpair(acc[32 + j], u[0], u[1]);
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            float o[4];
-            sums4(16 + 4 * c + j / 2, o);
-            *reinterpret_cast<float4*>(my_row + 8 * j) =
-                make_float4(o[0] * p.one, o[1] * p.one, o[2] * p.one, o[3] * p.one);
+          for (int q = 0; q < 2; ++q) {
+            g[q] = 2 * j + q < left ? act_fast<MODE - kGated>(g[q]) * u[q] : 0.0f;
+            am = max(am, abs_bits(g[q]));
           }
-          pair_sync(1 + quad);
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float4 o4 = *reinterpret_cast<const float4*>(other + 8 * j);
-            const float o[4] = {o4.x, o4.y, o4.z, o4.w};
-            float h[4];
-            sums4(4 * c + j / 2, h);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float g = hf ? o[q] : h[q], u = hf ? h[q] : o[q];
-              h[q] = 16 * c + 2 * j + q < left ? act_fast<MODE - kGated>(g) * u : 0.0f;
-              am = max(am, abs_bits(h[q]));
-            }
-            acc[8 * c + j] = pair(h[0], h[1]);
-            acc[8 * c + j + 1] = pair(h[2], h[3]);
-          }
-          pair_sync(1 + quad);
+          acc[j] = pair(g[0], g[1]);
         }
-        // the scale covers both warps' columns; both stop at the same tile
-        *reinterpret_cast<uint32_t*>(my_row + 64) = am;
+        // The scale covers the columns of two warps.  (A slot of this
+        // exchange is written again two tiles later, after a barrier that the
+        // other warp reaches once it has read it.)  Both stop at the same tile.
+        turn ^= 1;
+        reinterpret_cast<uint32_t*>(my_row)[turn] = am;
         stop = pair_sync_or(1 + quad, !ok);
-        am = max(am, *reinterpret_cast<const uint32_t*>(other + 64));
+        am = max(am, reinterpret_cast<const uint32_t*>(staging + ((warp ^ 4) * 32 + lane) * kRowLd)[turn]);
         const GroupScale gs = group_scale(am);
-        if (hf == 0 && lane < rows) p.hs[(long long)nt * p.hs_ld + m0 + lane] = gs.scale;
+        if (mine) {
+          if (hf == 0) p.hs[(long long)nt * p.hs_ld + m0 + lane] = gs.scale;
+          uint8_t* dst = p.hq + (long long)(m0 + lane) * p.ldh + n0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[4];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float h[4];
-            unpair(acc[8 * c + 2 * j], h[0], h[1]);
-            unpair(acc[8 * c + 2 * j + 1], h[2], h[3]);
-            w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
+            for (int j = 0; j < 8; ++j) {
+              float h[4];
+              unpair(acc[16 * c + 2 * j], h[0], h[1]);
+              unpair(acc[16 * c + 2 * j + 1], h[2], h[3]);
+              w[j] = gs.mul == 0.0f ? 0u : codes2(h[0], h[1], gs.mul) | codes2(h[2], h[3], gs.mul) << 16;
+            }
+            // (n0 and ldh are multiples of 32; codes past N are zero)
+            if (n0 + 32 * c < p.ldh) store32(dst + 32 * c, w);
           }
-          *reinterpret_cast<uint4*>(my_row + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        // (n and ldh are multiples of 16; codes past N are zero)
-        store_rows(p.hq + (long long)m0 * p.ldh + n, p.ldh, staging + warp * kStaging, lane, (int)min(64ll, p.ldh - n), rows);
-        // (the other warp reads this row's maximum before it can reach the
-        // next tile's barriers, and only those let this warp write it again)
       } else if (!ok) {
         stop = true;
-      } else {
-        const int left = p.N - n0;  // features of this warp that exist
+      } else if (mine) {
         const float* bias = p.bias ? p.bias + n0 : nullptr;
-        auto out4 = [&](int q, float (&o)[4]) {
-          sums4(q, o);
-          if constexpr (MODE >= kEpilogue) {
+        const long long y0 = (long long)(m0 + lane) * p.ldy + n0;
+        uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + y0 * (p.ydt == MTC_F32 ? 4 : 2);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (bias && 4 * q + j < left) o[j] += __ldg(bias + 4 * q + j);
-              o[j] = act_fast<MODE - kEpilogue>(o[j]);
-            }
-          }
-        };
-        uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + ((long long)m0 * p.ldy + n0) * p.y_bytes;
-        const long long ldy = p.ldy * p.y_bytes;
-        if (p.ydt == MTC_F32 || !p.vec) {
-          // 16 columns at a time; an output whose rows do not start on 16
-          // bytes takes them one value at a time
+        for (int c = 0; c < 8; ++c) {
+          float o[16];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int j = 0; j < 16; j += 2) {
+            unpair(acc[8 * c + j / 2], o[j], o[j + 1]);
+            if constexpr (MODE >= kEpilogue) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float o[4];
-              out4(4 * c + j, o);
-              *reinterpret_cast<float4*>(my_row + 16 * j) =
-                  make_float4(o[0] * p.one, o[1] * p.one, o[2] * p.one, o[3] * p.one);
-            }
-            if (p.vec) {
-              store_rows(y + 64 * c, ldy, staging + warp * kStaging, lane, 4 * (left - 16 * c), rows);
-            } else if (lane < rows) {
-#pragma unroll 1
-              for (int j = 0; j < min(16, left - 16 * c); ++j)
-                store1(y + lane * ldy, p.ydt, 16 * c + j, reinterpret_cast<const float*>(my_row)[j]);
-            }
-          }
-        } else {
-          // 16-bit outputs, 32 columns at a time
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
-#pragma unroll
-              for (int j = 0; j < 4; j += 2) {
-                float o[4];
-                out4(8 * c + 2 * i + j / 2, o);
-                w[j] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[0], o[1]) : pack2(MTC_F16, o[0], o[1]);
-                w[j + 1] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[2], o[3]) : pack2(MTC_F16, o[2], o[3]);
+              for (int q = j; q < j + 2; ++q) {
+                if (bias && 16 * c + q < left) o[q] += __ldg(bias + 16 * c + q);
+                o[q] = act_fast<MODE - kEpilogue>(o[q]);
               }
-              *reinterpret_cast<uint4*>(my_row + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            store_rows(y + 64 * c, ldy, staging + warp * kStaging, lane, 2 * (left - 32 * c), rows);
+          }
+          if (p.vec && 16 * c + 16 <= left) {
+            if (p.ydt != MTC_F32) {
+              uint32_t w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                w[j] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[2 * j], o[2 * j + 1]) : pack2(MTC_F16, o[2 * j], o[2 * j + 1]);
+              store32(y + 32 * c, w);
+            } else {
+              // Sums leave through a multiplication by p.one (= 1): stored
+              // directly, the compiler lays them out for the stores and moves
+              // every one of them in the main loop (466 against 415 thousand
+              // cycles at 4096 x 4096 x 14336).
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[8 * h + j] * p.one);
+                store32(y + 64 * c + 32 * h, w);
+              }
+            }
+          } else if (16 * c < left) {
+            // the last columns, or rows that do not start on 32 bytes: one
+            // value at a time, from shared memory to have the code once
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(my_row + j) =
+                  make_float4(o[j] * p.one, o[j + 1] * p.one, o[j + 2] * p.one, o[j + 3] * p.one);
+#pragma unroll 1
+            for (int j = 0; j < min(16, left - 16 * c); ++j) store1(p.Y, p.ydt, y0 + 16 * c + j, my_row[j]);
           }
         }
       }
@@ -1147,9 +1101,8 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
     p.lds = a.lds;
     p.Y = a.Y;
     p.ydt = a.ydt;
-    p.y_bytes = a.ydt == MTC_F32 ? 4 : 2;
     p.ldy = a.ldy;
-    p.vec = (reinterpret_cast<uintptr_t>(a.Y) & 15) == 0 && (a.ldy & (a.ydt == MTC_F32 ? 3 : 7)) == 0;
+    p.vec = (reinterpret_cast<uintptr_t>(a.Y) & 31) == 0 && (a.ldy & (a.ydt == MTC_F32 ? 7 : 15)) == 0;
     p.bias = a.bias;
     p.one = 1.0f;
     p.hq = a.hq;
