@@ -557,18 +557,18 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
 #pragma unroll 1
       for (int i = warp; i < count; i += n_warps) {
         const int j = rank + i * split;
-        float4 x[C::kMats][8];
+        float4 x[C::kMats][kMaxCluster];
 #pragma unroll
         for (int m = 0; m < C::kMats; ++m)
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
+          for (int q = 0; q < kMaxCluster; ++q)
             if (q < split) x[m][q] = load_cluster4(part + (m * BN + j) * 128 + f4, q);
         float a[C::kMats][4];
 #pragma unroll
         for (int m = 0; m < C::kMats; ++m) {
           a[m][0] = a[m][1] = a[m][2] = a[m][3] = 0.0f;
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
+          for (int q = 0; q < kMaxCluster; ++q)
             if (q < split) {
               a[m][0] += x[m][q].x;
               a[m][1] += x[m][q].y;
@@ -728,18 +728,52 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (warp >= kManyWarps) {
     regs_dec<kIssueRegs>();
+    // Tiles in time: a dense product runs the token tiles of one feature tile
+    // together (all tokens stay in L2), a grouped one the feature tiles of one
+    // token tile (its expert's weights do).
+    auto slot_of = [&](int t) { return p.slots ? t / p.n_tiles : t % n_slots; };
+    auto feature_tile = [&](int t) { return p.slots ? t % p.n_tiles : t / n_slots; };
+    // the stage of iteration `it`, once the MMA that read it before is over
+    auto stage_free = [&](uint32_t it) {
+      return it < kManyStages || mbar_wait(&empty[it % kManyStages], ((it / kManyStages) & 1) ^ 1, p.timeout_ns);
+    };
     if (warp == kManyWarps) {
-      // ------------------------------------------------------------ TMA (lane 0) and scales (all lanes)
+      // ------------------------------------------------------------ codes by TMA
+      if (lane == 0) {
+        uint32_t it = 0;
+        Slot next = slot_at(p.slots, 0, p.M, 128, slot_of(blockIdx.x));  // one tile ahead
+        for (int t = blockIdx.x; t < n_work && !abort_flag[0]; t += gridDim.x) {
+          const Slot slot = next;
+          if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, 0, p.M, 128, slot_of(t + gridDim.x));
+          const int f0 = slot.e * p.N + feature_tile(t) * (GATED ? 128 : 256);
+          for (int kb = 0; kb < p.nkb; ++kb, ++it) {
+            if (!stage_free(it)) {
+              abort_flag[0] = 1;
+              break;
+            }
+            const int s = it % kManyStages;
+            uint8_t* st = smem + s * kManyStage;
+            mbar_expect_tx(&full[s], kManyStage);
+            tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
+            tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
+            tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
+          }
+        }
+        if (abort_flag[0]) {
+          // nothing of this CTA may be in flight when it leaves
+          for (uint32_t j = it > kManyStages ? it - kManyStages : 0; j < it; ++j)
+            (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
+          flag(p.status, MTC_STATUS_TIMEOUT);
+        }
+      }
+    } else if (warp == kManyWarps + 3) {
+      // ------------------------------------------------------------ scales and tiles
       uint32_t it = 0;
-      // Tiles in time: a dense product runs the token tiles of one feature
-      // tile together (all tokens stay in L2), a grouped one the feature
-      // tiles of one token tile (its expert's weights do).
-      auto slot_of = [&](int t) { return p.slots ? t / p.n_tiles : t % n_slots; };
-      Slot next = slot_at(p.slots, 0, p.M, 128, slot_of(blockIdx.x));  // one tile ahead
+      Slot next = slot_at(p.slots, 0, p.M, 128, slot_of(blockIdx.x));
       for (int t = blockIdx.x; t < n_work; t += gridDim.x) {
         const Slot slot = next;
         if (t + (int)gridDim.x < n_work) next = slot_at(p.slots, 0, p.M, 128, slot_of(t + gridDim.x));
-        const int nt = p.slots ? t % p.n_tiles : t / n_slots, f0 = slot.e * p.N + nt * (GATED ? 128 : 256);
+        const int nt = feature_tile(t);
         // lanes 0 and 1 fetch the features' scales, every lane those of the
         // rows lane, lane + 32, ...; a row past the end takes the last row's
         // scale (its values are never stored)
@@ -751,19 +785,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int j = 0; j < 4; ++j) sx[j] = p.sx + min(slot.row0 + lane + 32 * j, slot.end - 1);
         bool ok = true;
         for (int kb = 0; kb < p.nkb; ++kb, ++it) {
-          const int s = it % kManyStages;
-          if (!__all_sync(0xffffffffu, it < kManyStages || mbar_wait(&empty[s], ((it / kManyStages) & 1) ^ 1, p.timeout_ns))) {
+          if (!__all_sync(0xffffffffu, stage_free(it))) {
             ok = false;
             break;
           }
-          if (lane == 0) {
-            uint8_t* st = smem + s * kManyStage;
-            tiles[it % kScaleSlots] = make_int4(slot.row0, slot.end, nt, 0);
-            mbar_expect_tx(&full[s], kManyStage);
-            tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
-            tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
-            tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
-          }
+          if (lane == 0) tiles[it % kScaleSlots] = make_int4(slot.row0, slot.end, nt, 0);
           float* sc = scales + (it % kScaleSlots) * kScaleLd;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -771,17 +797,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             sx[j] += p.lds;
           }
           if (lane < 2) copy4_async(sc + 128 + lane, sw + kb);
-          copy4_arrive(&full[s]);
+          copy4_arrive(&full[it % kManyStages]);
         }
         if (!ok && lane == 0) abort_flag[0] = 1;
         if (__any_sync(0xffffffffu, !ok || abort_flag[0])) break;
       }
-      if (lane == 0) {
-        // nothing of this CTA may be in flight when it leaves
-        for (uint32_t j = it > kManyStages ? it - kManyStages : 0; j < it; ++j)
-          (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
-        if (abort_flag[0]) flag(p.status, MTC_STATUS_TIMEOUT);
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp <= kManyWarps + 2 && lane == 0) {
       // ---------------------------------------------------------- MMA: one warp per accumulator
       constexpr uint32_t idesc = idesc_e4m3_f32(128, 256);
@@ -967,13 +988,26 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
+// `bound` items at most.  While they leave SMs idle their inputs are split
+// over clusters of up to 8 CTAs (one SM streams at most about twice its share
+// of the memory bandwidth): over as many as keep all items on the device at
+// once and give every CTA at least four blocks of 128 inputs.
+// 1 x 14336 x 4096, 32 items: 14.7 us split by 4, 31.3 whole; 1 x 8192 x 2048,
+// 16 items: 8.2 us; split by 8, which does not fit at once, 13.6.
+// 1 x 896 x 128: 4.6 us whole, 5.2 split by 2.  A split launch has one
+// cluster per item.
 template <int BN, int SRC, bool PAIR>
-int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid,
-               cudaStream_t st, const char* who) {
+int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, FewParams& p, long long bound,
+               int sms, cudaStream_t st, const char* who) {
   static std::atomic<uint64_t> ready{0};
+  static ClusterCounts clusters;
   constexpr size_t smem = FewCfg<BN, PAIR>::kSmem;
   MTC_CHECK_CUDA(allow_smem(few_kernel<BN, SRC, PAIR>, smem, ready), who);
   constexpr int threads = FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES ? 0 : 32 * kQuantWarps);
+  p.split = 1;
+  for (int s = 2; s <= kMaxCluster && bound * s <= sms && p.nkb >= 4 * s; ++s)
+    if (bound <= resident_clusters(few_kernel<BN, SRC, PAIR>, threads, smem, s, clusters)) p.split = s;
+  const int grid = p.split > 1 ? (int)bound * p.split : (int)(bound < sms ? bound : sms);
   MTC_CHECK_CUDA(launch_chained(few_kernel<BN, SRC, PAIR>, dim3(grid), dim3(threads), smem, st, p.split, tw0, tw1, tx,
                                 p),
                  who);
@@ -982,10 +1016,10 @@ int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap
 
 // Tiles that gate / up pairs come in, too.
 template <int BN, int SRC>
-int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, const FewParams& p, int grid,
-               bool pair, cudaStream_t st, const char* who) {
-  return pair ? launch_few<BN, SRC, true>(tw0, tw1, tx, p, grid, st, who)
-              : launch_few<BN, SRC, false>(tw0, tw1, tx, p, grid, st, who);
+int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, FewParams& p, long long bound,
+               int sms, bool pair, cudaStream_t st, const char* who) {
+  return pair ? launch_few<BN, SRC, true>(tw0, tw1, tx, p, bound, sms, st, who)
+              : launch_few<BN, SRC, false>(tw0, tw1, tx, p, bound, sms, st, who);
 }
 
 template <int MODE>
@@ -1156,32 +1190,24 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   p.early = a.early;
   p.status = a.status;
   p.timeout_ns = wait_limit_ns();
-  // Split the inputs over a cluster while the items would leave more than
-  // half of the SMs idle and every CTA keeps at least four blocks of 128
-  // inputs.  (One SM streams at most about twice its share of the memory
-  // bandwidth.)  A split launch has one cluster per item.
   const long long bound = (long long)Nb * a.slot_bound;
-  int split = 1;
-  while (split < 8 && bound * split * 2 <= sms && nkb >= 8 * split) split *= 2;
-  p.split = split;
-  const int grid = split > 1 ? (int)bound * split : (int)(bound < sms ? bound : sms);
   const bool pair = n_mats == 2;
   if (a.xq) {
     // (pairs in tiles of 16 bring activations, those in tiles of 32 codes)
-    if (a.tile == 32) return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, grid, pair, st, who);
+    if (a.tile == 32) return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, bound, sms, pair, st, who);
     MTC_REQUIRE(!pair, "%s: a gate / up pair in tiles of %d rows", who, a.tile);
     switch (a.tile) {
-      case 16: return launch_few<16, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
-      case 64: return launch_few<64, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
-      default: return launch_few<128, SRC_CODES, false>(tw[0], tw[1], tx, p, grid, st, who);
+      case 16: return launch_few<16, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
+      case 64: return launch_few<64, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
+      default: return launch_few<128, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
     }
   }
   p.X = a.X;
   p.ldx = a.ldx;
   p.vec = (reinterpret_cast<uintptr_t>(a.X) & 15) == 0 && a.ldx % (a.xdt == MTC_F32 ? 4 : 8) == 0;
-  if (a.xdt == MTC_F32) return launch_few<16, SRC_F32>(tw[0], tw[1], tx, p, grid, pair, st, who);
-  if (a.xdt == MTC_BF16) return launch_few<16, SRC_BF16>(tw[0], tw[1], tx, p, grid, pair, st, who);
-  return launch_few<16, SRC_F16>(tw[0], tw[1], tx, p, grid, pair, st, who);
+  if (a.xdt == MTC_F32) return launch_few<16, SRC_F32>(tw[0], tw[1], tx, p, bound, sms, pair, st, who);
+  if (a.xdt == MTC_BF16) return launch_few<16, SRC_BF16>(tw[0], tw[1], tx, p, bound, sms, pair, st, who);
+  return launch_few<16, SRC_F16>(tw[0], tw[1], tx, p, bound, sms, pair, st, who);
 }
 
 }  // namespace fp8

@@ -91,6 +91,35 @@ cudaError_t allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done)
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
+
+// How many clusters of `cluster` CTAs the device holds at once, one CTA per
+// SM: fewer than its SMs allow by number (15 of 8, 33 of 4 on 148 SMs), since
+// a cluster stays inside one GPC.  Asked once per device; 0 if unknown.
+constexpr int kMaxCluster = 8;
+typedef std::atomic<int> ClusterCounts[64][kMaxCluster + 1];
+template <typename Kernel>
+int resident_clusters(Kernel kernel, int threads, size_t smem, int cluster, ClusterCounts& known) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  if ((n = known[dev][cluster].load(std::memory_order_relaxed)) > 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  known[dev][cluster].store(n, std::memory_order_relaxed);
+  return n;
+}
 int launch_product(const Product& a, cudaStream_t st, const char* who);
 
 // Rows of activations to codes and scales; with `pos` row m goes to the rows

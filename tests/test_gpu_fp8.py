@@ -152,6 +152,21 @@ def test_gemm_on_both_sides_of_its_variants(dev, M, K, N):
         close(y, ref, mag, K, torch.float32)
 
 
+@pytest.mark.parametrize("M", [1, 12, 40, 70])
+@pytest.mark.parametrize("K,N", [(5000, 2000), (5000, 2100), (3600, 2500), (3600, 2800), (3600, 3600), (3600, 4200),
+                                 (3600, 4500), (3600, 5800), (1000, 6100)])
+def test_gemm_split_over_clusters_of_any_size(dev, M, K, N):
+    from tensorpack_b200.kernels.fp8 import fp8_gemm
+
+    x, m, b = normal((M, K), M + K, dev), weights(K, N, N, dev), normal((N,), 9, dev)
+    y = fp8_gemm(x, m, b, "relu")
+    torch.cuda.synchronize()
+    m.check_status()
+    ref, mag = R.gemm(x, m.codes, m.scales[0], b, "relu")
+    close(y, ref, mag, K, torch.float32)
+    assert torch.equal(y, fp8_gemm(x, m, b, "relu"))
+
+
 @pytest.mark.parametrize("xt", list(TYPES))
 @pytest.mark.parametrize("yt", list(TYPES))
 @pytest.mark.parametrize("M,N", [(3, 200), (50, 200), (1300, 4000)])
