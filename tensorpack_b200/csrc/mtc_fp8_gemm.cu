@@ -9,17 +9,22 @@
 //    features are the M side of the MMA (TMEM lane = feature), so one token
 //    costs 16 columns instead of 128 rows, and a warp's stores are
 //    consecutive features.  Bound by the weight bytes: a persistent CTA per
-//    SM streams its features' codes once through a TMA ring of 200 KB.  When
-//    there are few tiles a cluster of up to 8 CTAs splits the inputs and adds
-//    its partial sums through distributed shared memory in rank order: no
-//    workspace, no atomics, the same result every time.  PAIR: the gate and
-//    up matrices of a gated product side by side; the output is
-//    act(gate) * up, quantized.
+//    SM streams its features' codes once through a TMA ring (1 x 4096 x 14336
+//    13.4 us, 4.4 TB/s with some 3 us of start-up; 16 x 14336 x 4096 17.1 us
+//    with the quantizer).  When there are few tiles a cluster of up to 8 CTAs
+//    splits the inputs and adds its partial sums through distributed shared
+//    memory in rank order: no workspace, no atomics, the same result every
+//    time.  PAIR: the gate and up matrices of a gated product side by side;
+//    the output is act(gate) * up, quantized.
 //  * many_kernel<MODE>: 128 tokens x 256 features (TMEM lane = token), one
 //    persistent CTA per SM, two 256-column accumulators that alternate
-//    between the MMA and eight warps that scale and add.  Bound by the
-//    tensor cores.  kGated: the 256 features are 128 of the gate matrix and
-//    the same 128 of the up matrix; the output is act(gate) * up, quantized.
+//    between the MMA and eight warps that scale and add.  4096 x 4096 x 14336
+//    takes 245 us with the quantizer, 1.96 PFLOP/s: 208 us with the scaling
+//    taken out, 176 us with the MMAs taken out, 150 us with both (loads and
+//    stores alone), so each of them waits for another.  After some 50 ms the
+//    power limit lowers the clock (1965 to 1540 MHz) and it takes 285 us.
+//    kGated: the 256 features are 128 of the gate matrix and the same 128 of
+//    the up matrix; the output is act(gate) * up, quantized.
 #include <string.h>
 
 #include <type_traits>
@@ -612,15 +617,15 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
 constexpr int kManyStages = 4;
 constexpr uint32_t kManyStage = 3 * kATile;
 constexpr int kManyWarps = 8;                         // scaling warps: 2 column halves x 4 lane quadrants
-constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup with the TMA and the MMA warp
+constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup: codes, 2 for MMAs, scales
 // A row of each scaling thread, for values that cannot leave as vectors (the
 // stride of 5 16-byte units keeps 16-byte accesses free of bank conflicts).
 constexpr int kRowLd = 20;
 constexpr uint32_t kStaging = kManyWarps * 32 * kRowLd * 4;
 // Scales of an iteration: sx of 128 rows, sw of the two scale blocks of the
 // features, and the tile {first row, end row, feature tile}, in a ring that
-// the TMA warp fills together with a stage (4-byte asynchronous copies: rows
-// start anywhere, and no copy waits for a load).  It writes iteration i after
+// a warp of its own fills together with a stage (4-byte asynchronous copies:
+// rows start anywhere, and no copy waits for a load).  It writes iteration i after
 // the MMA of i - kManyStages has completed, which was issued after the sums
 // of i - kManyStages - 2 were read: more slots than kManyStages + 2 are never
 // overwritten early.
@@ -858,23 +863,26 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           break;
         }
         tc::fence_after();
-        // the TMA warp wrote this block's scales before its MMA ran
+        // this block's scales were written before its MMA ran
         const float* slot = scales + (it % kScaleSlots) * kScaleLd;
         const float sa = slot[my_scale] * slot[128 + (GATED ? 0 : hf)];
         const float sb = GATED ? slot[my_scale] * slot[129] : sa;
         const f32x2 sc_a = pair(sa, sa), sc_b = pair(sb, sb);
+        // (the next columns are loaded while these are added)
+        uint32_t v[2][16];
+        tmem_ld16(tm_a + b * 256, v[0]);
+        tmem_wait16(v[0]);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          uint32_t v[16];
-          tmem_ld16((c < 4 ? tm_a : tm_b) + b * 256 + 16 * (c & 3), v);
-          tmem_wait16(v);
-          if (c == 7) {
+          if (c < 7) tmem_ld16((c < 3 ? tm_a : tm_b) + b * 256 + 16 * ((c + 1) & 3), v[(c + 1) & 1]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[c & 1][2 * j], v[c & 1][2 * j + 1]), c < 4 ? sc_a : sc_b);
+          if (c < 7) tmem_wait16(v[(c + 1) & 1]);
+          if (c == 6) {
             tc::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[b]);
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) fma2(acc[8 * c + j], pair(v[2 * j], v[2 * j + 1]), c < 4 ? sc_a : sc_b);
         }
       }
       const int4 tile = tiles[(it - 1) % kScaleSlots];
