@@ -158,17 +158,38 @@ __device__ __forceinline__ uint32_t pack2(int dt, float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Activations with the hardware exponential and division (a few ulp; the
-// relative error of exp grows with |x|, but the result is then next to 0 or
-// x), short enough to be unrolled over a thread's sums: the many-row kernel's
-// epilogue.  GELU (tanh form) as x / (1 + exp(-2 u)), since
-// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)).
+// 2^x and 1 / x by the special function unit (2^-22 relative, 1 ulp);
+// denormal results are zero, which saves their handling and, next to the 1
+// below, changes nothing.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The larger of a and |b|, NaN if one of them is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+
+// Activations in a few instructions, to be unrolled over a thread's sums: the
+// many-row kernel's epilogue.  (The relative error of the exponential grows
+// with |x|, but the result is then next to 0 or x.)  SiLU is x / (1 +
+// 2^(-x log2 e)); GELU (tanh form) x / (1 + exp(-2 u)) with u = sqrt(2 / pi)
+// (x + 0.044715 x^3), since (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)).
 template <int ACT>
 __device__ __forceinline__ float act_fast(float x) {
+  constexpr float kLog2e = 1.4426950408889634f, kTwoRoot = 1.5957691216057308f;  // log2 e, 2 sqrt(2 / pi)
   if constexpr (ACT == MTC_ACT_RELU) return x < 0.0f ? 0.0f : x;
-  else if constexpr (ACT == MTC_ACT_SILU) return __fdividef(x, 1.0f + __expf(-x));
+  else if constexpr (ACT == MTC_ACT_SILU) return x * rcp_fast(1.0f + exp2_fast(-kLog2e * x));
   else if constexpr (ACT == MTC_ACT_GELU_TANH)
-    return __fdividef(x, 1.0f + __expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+    return x * rcp_fast(1.0f + exp2_fast(-x * fmaf(kLog2e * kTwoRoot * 0.044715f, x * x, kLog2e * kTwoRoot)));
   else return x;
 }
 

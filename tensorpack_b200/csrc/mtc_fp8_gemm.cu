@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int left = p.N - n0;                                        // features of this warp that exist
       const bool mine = ok && m0 + lane < tile.y;                       // this thread's row exists
       if constexpr (GATED) {
-        uint32_t am = 0;
+        float largest = 0.0f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           float g[2], u[2];
@@ -899,11 +899,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           unpair(acc[32 + j], u[0], u[1]);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            g[q] = 2 * j + q < left ? act_fast<MODE - kGated>(g[q]) * u[q] : 0.0f;
-            am = max(am, abs_bits(g[q]));
+            g[q] = act_fast<MODE - kGated>(g[q]) * u[q];
+            if (left < 64 && 2 * j + q >= left) g[q] = 0.0f;  // (a matrix may end in these columns)
+            largest = max_abs(largest, g[q]);
           }
           acc[j] = pair(g[0], g[1]);
         }
+        uint32_t am = __float_as_uint(largest);
         // The scale covers the columns of two warps.  (A slot of this
         // exchange is written again two tiles later, after a barrier that the
         // other warp reaches once it has read it.)  Both stop at the same tile.
