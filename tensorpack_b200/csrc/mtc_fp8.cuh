@@ -116,6 +116,24 @@ __device__ __forceinline__ void unpack8(const uint4 (&raw)[NV], float (&v)[8]) {
   }
 }
 
+// Bits of the largest |value| among those, as fp32.  (The order of 16-bit
+// values without their sign is that of their bits, too: two at a time.)
+template <typename T, int NV>
+__device__ __forceinline__ uint32_t amax_raw(const uint4 (&raw)[NV]) {
+  if constexpr (sizeof(T) == 4) {
+    float v[8];
+    unpack8<T>(raw, v);
+    return amax8(v);
+  } else {
+    const uint4 r = raw[0];
+    const uint32_t m = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+    const uint16_t top = (uint16_t)max(m & 0xffffu, m >> 16);
+    T x;
+    *reinterpret_cast<uint16_t*>(&x) = top;
+    return __float_as_uint(to_f32(x));
+  }
+}
+
 // Eight consecutive values at p as fp32; `n` of them exist (the others read
 // as zero).  `vec`: p is 16-byte aligned and n >= 8 may be read as vectors.
 template <typename T>

@@ -891,6 +891,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int left = p.N - n0;                                        // features of this warp that exist
       const bool mine = ok && m0 + lane < tile.y;                       // this thread's row exists
       if constexpr (GATED) {
+        if (left < 64) {
+          // the matrix ends in these columns: act(0) * 0 behind them
+#pragma unroll
+          for (int j = 0; j < 64; ++j) {
+            float x, y;
+            unpair(acc[j], x, y);
+            acc[j] = pair(2 * (j & 31) < left ? x : 0.0f, 2 * (j & 31) + 1 < left ? y : 0.0f);
+          }
+        }
         float largest = 0.0f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
@@ -900,7 +909,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             g[q] = act_fast<MODE - kGated>(g[q]) * u[q];
-            if (left < 64 && 2 * j + q >= left) g[q] = 0.0f;  // (a matrix may end in these columns)
             largest = max_abs(largest, g[q]);
           }
           acc[j] = pair(g[0], g[1]);

@@ -33,7 +33,8 @@ __device__ __forceinline__ void store_codes(uint8_t* q, const uint2& c, int left
 // time: their loads are in flight together, their maxima reduced together, and
 // lane u of the half warp divides for group u alone.  Bound by memory:
 // 4096 x 14336 fp32 takes 49.9 us (5.9 TB/s; 64.3 us one group at a time with
-// every lane dividing).  U = 1 when a half warp has one group at most:
+// every lane dividing); bf16 39.3 us, bound by instruction issue (43.0 with
+// the maxima of 16-bit values one at a time).  U = 1 when a half warp has one group at most:
 // 333 x 4864 fp16 and the product after it take 17.0 us, 19.2 with U = 4.
 template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
@@ -76,8 +77,12 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
     uint32_t am[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (VEC) unpack8<T>(raw[u], v[u]);
-      am[u] = amax8(v[u]);
+      if (VEC && U > 1) {
+        am[u] = amax_raw<T>(raw[u]);
+      } else {
+        if (VEC) unpack8<T>(raw[u], v[u]);
+        am[u] = amax8(v[u]);
+      }
     }
 #pragma unroll
     for (int d = 8; d; d >>= 1)
@@ -89,6 +94,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
     const GroupScale gs = group_scale(mine);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (VEC && U > 1) unpack8<T>(raw[u], v[u]);
       const uint2 c = codes8(v[u], __shfl_sync(0xffffffffu, gs.mul, u, 16));
       if (mm[u] < 0) continue;
       const int k = bb[u] * kBlock + 8 * l;
