@@ -397,19 +397,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   int32_t* mine = hist + warp * p.E;
   if (ok && rank == 0) mine[id] = __popc(same);
   __syncthreads();
-  // thread e: rows of expert e in this CTA, in those before it, in all
+  // thread e: rows of expert e by warp, in the CTAs before this one, in all
   const int e = threadIdx.x;
-  int here = 0, before = 0, count = 0;
+  int rows[32], before = 0, count = 0;
   if (e < p.E) {
-    for (int w = 0; w < 32; ++w) {
-      const int c = hist[w * p.E + e];
-      hist[w * p.E + e] = here;
-      here += c;
-    }
+#pragma unroll
+    for (int w = 0; w < 32; ++w) rows[w] = hist[w * p.E + e];
     if (gridDim.x == 1) {
-      count = here;
+#pragma unroll
+      for (int w = 0; w < 32; ++w) count += rows[w];
     } else {
-#pragma unroll 8
+#pragma unroll 16
       for (int b = 0; b < (int)gridDim.x; ++b) {
         const int c = p.counts[(long long)b * p.E + e];
         count += c;
@@ -426,8 +424,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       *reinterpret_cast<int4*>(p.slots + 4 + 4 * (sl + i)) = make_int4(e, off + i * p.size, off + count, 0);
     if (threadIdx.x == 0) p.slots[0] = n_slots;
   }
-  if (e < p.E)
-    for (int w = 0; w < 32; ++w) hist[w * p.E + e] += off + before;
+  if (e < p.E) {
+    int at = off + before;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      hist[w * p.E + e] = at;
+      at += rows[w];
+    }
+  }
   __syncthreads();
   if (r < p.R) {
     const int at = ok ? mine[id] + rank : -1;

@@ -57,7 +57,6 @@ enum { SRC_CODES = 0, SRC_F32 = 1, SRC_BF16 = 2, SRC_F16 = 3 };
 // the kernel takes activations as they are.
 constexpr int kAccs = 4, kQuantWarps = 6;
 
-
 template <int BN, bool PAIR>
 struct FewCfg {
   static constexpr int kMats = PAIR ? 2 : 1;

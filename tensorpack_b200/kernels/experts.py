@@ -6,7 +6,9 @@ weights; ``experts_forward`` runs the chosen experts, whose matrices are
 
     y_t = sum_j weights[t, j] * (act(x_t @ gate_e) * (x_t @ up_e)) @ down_e,   e = ids[t, j]
 
-Both enqueue their kernels on the current stream and do not synchronise.
+Both enqueue their kernels on the current stream and do not synchronise.  A
+wait that ran out in a kernel is reported by ``gate.check_status()``.
+Inference only: results carry no gradient.
 """
 
 from __future__ import annotations
@@ -127,7 +129,9 @@ def experts_forward(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, g
             out_dtype, y_type = torch.float32, _lib.F32
         Y, ldy = _empty((T, D), (D, 1), dtype=out_dtype, device=dev), D
     else:
-        _check_output(Y, (T, D), out_dtype, dev, (X, ids, weights), "experts_forward")
+        _check_output(Y, (T, D), out_dtype, dev, (X, ids, weights) + tuple(t for m in (gate, up, down)
+                                                                           for t in (m._store, m.scales)),
+                      "experts_forward")
         y_type, ldy = _TYPES[Y.dtype], Y.stride(0) if T > 1 else D
     if T:
         lib = _lib.load()

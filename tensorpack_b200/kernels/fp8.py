@@ -12,7 +12,8 @@ as amax = max(max|x|, 2^-100), scale = amax / 448, code = e4m3(x * (448 /
 amax)), every step rounded to nearest even in fp32.  A group that holds an
 infinity or a NaN gets a NaN scale, so what is computed from it is NaN.
 
-There is no CPU fallback: without CUDA these raise.
+There is no CPU fallback: without CUDA these raise.  Inference only: results
+carry no gradient.
 """
 
 from __future__ import annotations
@@ -307,7 +308,8 @@ def fp8_gemm(X, W: FP8Matrix, bias=None, activation: Optional[str] = None, Y=Non
             out_dtype, y_type = torch.float32, _lib.F32
         Y, ldy = _empty((M, N), (N, 1), dtype=out_dtype, device=dev), N
     else:
-        _check_output(Y, (M, N), out_dtype, dev, (X,) if bias is None else (X, bias), "fp8_gemm")
+        _check_output(Y, (M, N), out_dtype, dev, (X, W._store, W.scales) if bias is None else
+                      (X, W._store, W.scales, bias), "fp8_gemm")
         y_type, ldy = _TYPES[Y.dtype], Y.stride(0) if M > 1 else N
     if M:
         lib = _lib.load()

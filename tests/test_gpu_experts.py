@@ -13,6 +13,9 @@ may hold a few such values: 5e-2 of its own norm tells it from another row.
 """
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -304,3 +307,56 @@ def test_one_token_with_rows_of_no_expert(dev):
     ids = torch.tensor([[3, -1, 7, 3, 8, 2 ** 30]], dtype=torch.int32, device=dev)
     forward(dev, 1, 8, 6, 200, 130, torch.float32, ids=ids)
     forward(dev, 1, 8, 6, 200, 130, torch.bfloat16, ids=torch.full_like(ids, -5))
+
+
+FIRST_CALLS = """
+import torch
+from tensorpack_b200.kernels import experts, fp8
+dev = torch.device("cuda")
+g = torch.Generator(device=dev).manual_seed(1)
+w = fp8.FP8Matrix.from_tensor(torch.randn(2048, 512, device=dev, generator=g))
+mats = [fp8.FP8Experts.from_tensor(torch.randn(4, a, b, device=dev, generator=g)) for a, b in
+        ((512, 128), (512, 128), (128, 512))]
+def run(x):
+    y = fp8.fp8_gemm(x, w, activation="silu")
+    ids, weights = experts.route_experts(y[:, :4], 2)
+    return experts.experts_forward(y, ids, weights, *mats)
+xs = [torch.randn(n, 2048, device=dev, generator=g) for n in (1, 5, 30, 300)]
+s = torch.cuda.Stream()
+graphs, outs = [], []
+for x in xs:   # every kernel's first launch is a captured one
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        outs.append(run(x))
+    graphs.append(graph)
+for _ in range(3):
+    for graph in graphs:
+        graph.replay()
+torch.cuda.synchronize()
+w.check_status()
+for x, y in zip(xs, outs):
+    assert y.isfinite().all() and y.abs().max() > 0 and torch.equal(y, run(x))
+"""
+
+
+def test_first_calls_inside_a_capture(dev):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_an_output_on_top_of_the_weights_is_refused(dev):
+    from tensorpack_b200.kernels.experts import experts_forward
+    from tensorpack_b200.kernels.fp8 import FP8Matrix, fp8_gemm
+
+    codes = torch.zeros(128, 256, dtype=torch.uint8, device=dev)
+    m = FP8Matrix.from_codes(codes, torch.ones(1, 2, device=dev))
+    x = torch.ones(3, 256, device=dev)
+    with pytest.raises(ValueError, match="overlaps"):
+        fp8_gemm(x, m, Y=codes.view(-1).view(torch.float32)[:3 * 128].view(3, 128))
+    E, D, I = 2, 128, 128
+    mats = stack(E, D, I, 1, dev), stack(E, D, I, 2, dev), stack(E, I, D, 3, dev)
+    ids = torch.zeros(3, 1, dtype=torch.int32, device=dev)
+    y = mats[2]._store.view(-1).view(torch.float32)[:3 * D].view(3, D)
+    with pytest.raises(ValueError, match="overlaps"):
+        experts_forward(x[:, :D], ids, ids.float(), *mats, Y=y)
