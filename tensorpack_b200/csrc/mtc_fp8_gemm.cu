@@ -619,7 +619,7 @@ constexpr int kManyWarps = 8;                         // scaling warps: 2 column
 constexpr int kManyThreads = 32 * (kManyWarps + 4);   // + a warpgroup: codes, 2 for MMAs, scales
 // A row of each scaling thread, for values that cannot leave as vectors (the
 // stride of 5 16-byte units keeps 16-byte accesses free of bank conflicts):
-// 4000 x 1024 x 3001 bf16 takes 43.5 us, 95.6 with every thread storing
+// 4000 x 1024 x 3001 bf16 takes 42.2 us, 95.6 with every thread storing
 // its own row.
 constexpr int kRowLd = 20;
 constexpr uint32_t kStaging = kManyWarps * 32 * kRowLd * 4;
@@ -634,7 +634,8 @@ constexpr int kScaleSlots = 8, kScaleLd = 132;
 static_assert(kScaleSlots > kManyStages + 2, "a scale slot must outlive its reader");
 constexpr uint32_t kManyScales = kManyStages * kManyStage + kStaging;
 constexpr uint32_t kManyTiles = kManyScales + kScaleSlots * kScaleLd * 4;
-constexpr uint32_t kManyBars = kManyTiles + kScaleSlots * 16;
+constexpr uint32_t kManyBias = kManyTiles + kScaleSlots * 16;  // 128 values per scaling warp
+constexpr uint32_t kManyBars = kManyBias + kManyWarps * 128 * 4;
 constexpr size_t kManySmem = 1024 + kManyBars + 256;
 static_assert(kManySmem <= 227 * 1024, "shared memory of one CTA");
 // Registers: 384 threads are launched with 168 each; the scaling warps (128
@@ -842,6 +843,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     regs_inc<kScaleRegs>();
     const int quad = warp & 3, hf = warp >> 2;  // TMEM lanes 32 quad .., columns 128 hf ..
     float* my_row = staging + (warp * 32 + lane) * kRowLd;
+    float* bias = reinterpret_cast<float*>(smem + kManyBias) + 128 * warp;
     const int my_scale = 32 * quad + lane;
     // TMEM columns of the sums 0..63 and 64..127: 128 features, or 64 of the
     // gate and the same 64 of the up matrix
@@ -943,21 +945,31 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       } else if (!ok) {
         stop = true;
       } else {
-        const float* bias = p.bias ? p.bias + n0 : nullptr;
+        if constexpr (MODE >= kEpilogue) {
+          // the warp's 128 values of the bias, then read four at a time
+          float4 f;
+          f.x = p.bias && 4 * lane < left ? __ldg(p.bias + n0 + 4 * lane) : 0.0f;
+          f.y = p.bias && 4 * lane + 1 < left ? __ldg(p.bias + n0 + 4 * lane + 1) : 0.0f;
+          f.z = p.bias && 4 * lane + 2 < left ? __ldg(p.bias + n0 + 4 * lane + 2) : 0.0f;
+          f.w = p.bias && 4 * lane + 3 < left ? __ldg(p.bias + n0 + 4 * lane + 3) : 0.0f;
+          *reinterpret_cast<float4*>(bias + 4 * lane) = f;
+          __syncwarp();
+        }
         const long long y0 = (long long)(m0 + lane) * p.ldy + n0;
         uint8_t* y = reinterpret_cast<uint8_t*>(p.Y) + y0 * (p.ydt == MTC_F32 ? 4 : 2);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           float o[16];
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
+          for (int j = 0; j < 16; j += 4) {
             unpair(acc[8 * c + j / 2], o[j], o[j + 1]);
+            unpair(acc[8 * c + j / 2 + 1], o[j + 2], o[j + 3]);
             if constexpr (MODE >= kEpilogue) {
-#pragma unroll
-              for (int q = j; q < j + 2; ++q) {
-                if (bias && 16 * c + q < left) o[q] += __ldg(bias + 16 * c + q);
-                o[q] = act_fast<MODE - kEpilogue>(o[q]);
-              }
+              const float4 f = *reinterpret_cast<const float4*>(bias + 16 * c + j);
+              o[j] = act_fast<MODE - kEpilogue>(o[j] + f.x);
+              o[j + 1] = act_fast<MODE - kEpilogue>(o[j + 1] + f.y);
+              o[j + 2] = act_fast<MODE - kEpilogue>(o[j + 2] + f.z);
+              o[j + 3] = act_fast<MODE - kEpilogue>(o[j + 3] + f.w);
             }
           }
           if (p.vec && 16 * c + 16 <= left) {
@@ -989,7 +1001,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                   make_float4(o[j] * p.one, o[j + 1] * p.one, o[j + 2] * p.one, o[j + 3] * p.one);
             __syncwarp();
             const int col = lane & 15;
-#pragma unroll 4
+#pragma unroll
             for (int r = lane >> 4; r < 32; r += 2)
               if (m0 + r < tile.y && 16 * c + col < left)
                 store1(p.Y, p.ydt, (long long)(m0 + r) * p.ldy + n0 + 16 * c + col, (my_row - lane * kRowLd)[r * kRowLd + col]);
