@@ -182,6 +182,23 @@ def test_types_bias_and_activations(dev, xt, yt, M, N):
         close(y, ref, mag, K, TYPES[yt])
 
 
+@pytest.mark.parametrize("yt", list(TYPES))
+@pytest.mark.parametrize("N", [4872, 4881, 4865, 4991])
+def test_aligned_rows_with_a_ragged_end(dev, yt, N):
+    """Rows that start on 32 bytes and end inside a vector: what lies behind
+    them in the larger tensor stays."""
+    from tensorpack_b200.kernels.fp8 import fp8_gemm
+
+    M, K, t = 300, 260, TYPES[yt]
+    x, m, b = normal((M, K), 3, dev), weights(K, N, 4, dev), normal((N,), 5, dev)
+    hold = torch.full((M + 1, 5008), 7.0, device=dev, dtype=t)
+    for bias, act in ((None, None), (b, "gelu_tanh")):
+        y = fp8_gemm(x, m, bias, act, Y=hold[:M, :N])
+        ref, mag = R.gemm(x, m.codes, m.scales[0], bias, act)
+        close(y, ref, mag, K, t)
+        assert (hold[M] == 7).all() and (hold[:, N:] == 7).all()
+
+
 @pytest.mark.parametrize("M", [2, 40, 1300])
 def test_operands_that_are_views(dev, M):
     """Rows with a stride, rows that start off 16 bytes, an output inside a
