@@ -495,10 +495,11 @@ MTC_API int mtc_route_experts(const void* logits, int32_t type, int32_t T, int32
  * (act(x_t Wg) * (x_t Wu)) Wd with the matrices of expert ids[t][j]; gate and
  * up are E x (K = D, N = I), down is E x (K = I, N = D).  x_t and the gated
  * values are quantized as by mtc_fp8_quantize; the gated values are fp32
- * before that, the experts' outputs are rounded to Y's type, weighted and
- * added in fp32 in the order of j, and rounded once more.  An id outside
+ * before that, the experts' outputs are fp32, weighted and added in fp32 in
+ * the order of j, and the sum is rounded once to Y's type.  An id outside
  * 0..E-1 is no expert and adds nothing.  `ws` is 256-byte aligned, its size
- * from mtc_experts_workspace_bytes.  Y must not overlap X. */
+ * from mtc_experts_workspace_bytes (the same for every y_type).  Y must not
+ * overlap X. */
 MTC_API size_t mtc_experts_workspace_bytes(const mtc_fp8_matrix* gate, int32_t T, int32_t k, int32_t y_type);
 MTC_API int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_matrix* up, const mtc_fp8_matrix* down,
                                 const void* X, int32_t x_type, int32_t T, int64_t ldx, const int32_t* ids,

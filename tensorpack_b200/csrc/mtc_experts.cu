@@ -441,10 +441,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
 }
 
 // ---------------------------------------------------------------------------
-// Y[t] = sum_j weights[t][j] * rows[pos[t][j]], j in order, fp32
+// Y[t] = sum_j weights[t][j] * rows[pos[t][j]], j in order
 // ---------------------------------------------------------------------------
+// Rows and sum are fp32, rounded once to Y's type.
 struct CombineParams {
-  const void* rows;
+  const float* rows;
   long long ldr;
   const int32_t* pos;    // or null: row j, for the ids of one token
   const int32_t* ids;
@@ -456,7 +457,6 @@ struct CombineParams {
   int ydt, vec;
 };
 
-template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
   const int parts = (p.D + 2047) >> 11, t = blockIdx.x / parts;
   __shared__ int at[kMaxTopK];
@@ -479,21 +479,21 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = 0.0f;
   // (rows are padded to 8 values, so the last vector may be read whole)
-  constexpr int kVec = sizeof(T) == 4 ? 2 : 1, kMore = sizeof(T) == 4 ? 4 : 8;
+  constexpr int kMore = 4;
   for (int j0 = 0; j0 < p.k; j0 += kMore) {
-    uint4 raw[kMore][kVec];
+    uint4 raw[kMore][2];
 #pragma unroll
     for (int j = 0; j < kMore; ++j) {
       const int r = j0 + j < kMaxTopK ? at[j0 + j] : -1;
-      const T* row = reinterpret_cast<const T*>(p.rows) + r * p.ldr + d;
+      const float* row = p.rows + r * p.ldr + d;
 #pragma unroll
-      for (int q = 0; q < kVec; ++q) raw[j][q] = load16_if(reinterpret_cast<const uint4*>(row) + q, r >= 0);
+      for (int q = 0; q < 2; ++q) raw[j][q] = load16_if(reinterpret_cast<const uint4*>(row) + q, r >= 0);
     }
 #pragma unroll
     for (int j = 0; j < kMore; ++j)
       if (j0 + j < p.k && at[j0 + j] >= 0) {
         float v[8];
-        unpack8<T>(raw[j], v);
+        unpack8<float>(raw[j], v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = fmaf(w[j0 + j], v[i], a[i]);
       }
@@ -537,7 +537,7 @@ struct ExpertsPlan {
   int plan_ctas;
   size_t order, pos, slots, counts, xq, xs, hq, hs, out, bytes;
 };
-bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
+bool experts_plan(int T, int k, int E, int D, int I, ExpertsPlan* pl) {
   const long long R = (long long)T * k;
   if (R > kMaxRows || (long long)T * ((D + 2047) / 2048) > kMaxRows) return false;
   pl->R = (int)R;
@@ -572,7 +572,7 @@ bool experts_plan(int T, int k, int E, int D, int I, int ydt, ExpertsPlan* pl) {
   }
   pl->hq = take((size_t)R * pl->ldh);
   pl->hs = take((size_t)((I + 127) / 128) * pl->lds * 4);
-  pl->out = take((size_t)R * pl->ldo * (ydt == MTC_F32 ? 4 : 2));
+  pl->out = take((size_t)R * pl->ldo * 4);
   pl->bytes = at;
   return true;
 }
@@ -638,9 +638,9 @@ extern "C" int mtc_route_experts(const void* logits, int32_t type, int32_t T, in
   return launch_route<__half>(p, as_stream(stream));
 }
 
-extern "C" size_t mtc_experts_workspace_bytes(const mtc_fp8_matrix* gate, int32_t T, int32_t k, int32_t y_type) {
+extern "C" size_t mtc_experts_workspace_bytes(const mtc_fp8_matrix* gate, int32_t T, int32_t k, int32_t) {
   ExpertsPlan pl;
-  if (!gate || T < 1 || k < 1 || !experts_plan(T, k, gate->E, gate->K, gate->N, y_type, &pl)) return 0;
+  if (!gate || T < 1 || k < 1 || !experts_plan(T, k, gate->E, gate->K, gate->N, &pl)) return 0;
   return pl.bytes;
 }
 
@@ -665,7 +665,7 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
               "%s: bad shape (T=%d, k=%d, ldx=%lld, ldy=%lld)", who, T, k, (long long)ldx, (long long)ldy);
   const int E = gate->E, D = gate->K, I = gate->N;
   ExpertsPlan pl;
-  MTC_REQUIRE(experts_plan(T, k, E, D, I, y_type, &pl), "%s: too many rows (%d x %d)", who, T, k);
+  MTC_REQUIRE(experts_plan(T, k, E, D, I, &pl), "%s: too many rows (%d x %d)", who, T, k);
   if (ws_bytes < pl.bytes || !ws || (reinterpret_cast<uintptr_t>(ws) & 255)) {
     set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, pl.bytes, ws_bytes);
     return MTC_ERR_WORKSPACE;
@@ -738,12 +738,12 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   b.sx = a.hs;
   b.lds = a.hs_ld;
   b.Y = base + pl.out;
-  b.ydt = y_type;
+  b.ydt = MTC_F32;  // the terms of a sum
   b.ldy = pl.ldo;
   rc = launch_product(b, st, who);
   if (rc != MTC_OK) return rc;
   CombineParams c = {};
-  c.rows = base + pl.out;
+  c.rows = reinterpret_cast<const float*>(base + pl.out);
   c.ldr = pl.ldo;
   c.pos = pl.direct ? nullptr : pos;
   c.ids = ids;
@@ -756,9 +756,6 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   c.ldy = ldy;
   c.ydt = y_type;
   c.vec = (reinterpret_cast<uintptr_t>(Y) & 15) == 0 && ldy % (y_type == MTC_F32 ? 4 : 8) == 0;
-  auto kernel = y_type == MTC_F32    ? combine_kernel<float>
-                : y_type == MTC_BF16 ? combine_kernel<__nv_bfloat16>
-                                     : combine_kernel<__half>;
-  MTC_CHECK_CUDA(launch_chained(kernel, dim3((unsigned)((D + 2047) / 2048) * (unsigned)T), dim3(256), 0, st, 1, c), who);
+  MTC_CHECK_CUDA(launch_chained(combine_kernel, dim3((unsigned)((D + 2047) / 2048) * (unsigned)T), dim3(256), 0, st, 1, c), who);
   return MTC_OK;
 }

@@ -83,9 +83,9 @@ def experts_forward(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, g
     down (E, I, D).  An id outside 0..E-1 is no expert and adds nothing (a
     padded token, or an expert of another rank).  The activations and the
     gated values act(gate) * up (fp32 until then) are quantized as in
-    ``fp8_quantize``; an expert's output is rounded to the result's type, the
-    weighted sum is fp32 in the order of j.  The result is fp32, or
-    ``out_dtype``; ``Y`` takes it if given (it must not overlap an input)."""
+    ``fp8_quantize``; an expert's output and the weighted sum, in the order of
+    j, are fp32.  The result is fp32, or rounded once to ``out_dtype``; ``Y``
+    takes it if given (it must not overlap an input)."""
     X = _rows(X, "experts_forward")
     for m in (gate, up, down):
         if not isinstance(m, FP8Experts) or len(m.shape) != 3:
