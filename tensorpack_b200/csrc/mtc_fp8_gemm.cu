@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kManyStages; ++i) {
-      mbar_init(&full[i], 1 + 32);
+      mbar_init(&full[i], 1 + 32 + 1);  // the codes, the lanes' scales, the tile
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -805,6 +805,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
           if (lane < 2) copy4_async(sc + 128 + lane, sw + kb);
           copy4_arrive(&full[it % kManyStages]);
+          // (that arrival answers for the copies only: the tile, an ordinary
+          // store, is published by one of its own)
+          if (lane == 0) mbar_arrive(&full[it % kManyStages]);
         }
         if (!ok && lane == 0) abort_flag[0] = 1;
         if (__any_sync(0xffffffffu, !ok || abort_flag[0])) break;
