@@ -107,6 +107,7 @@ struct FewParams {
   int early;                          // slots and weights may be read before the predecessor ends
   uint32_t* status;
   unsigned long long timeout_ns;
+  uint32_t withhold;                  // diagnostic: bytes that the first load of a CTA waits for in vain
 };
 
 template <int SRC>
@@ -147,6 +148,11 @@ __device__ __forceinline__ float4 load_cluster4(const float* p, int rank) {
       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
       : "r"(tc::mapa(p, rank))
       : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_cluster1(const volatile uint32_t* p, int rank) {
+  uint32_t v;
+  asm("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(tc::mapa(const_cast<const uint32_t*>(p), rank)) : "memory");
   return v;
 }
 
@@ -218,21 +224,25 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
   const uint32_t tmem = *tmem_slot;
   if (!p.early) griddep_wait();
   const int n_slots = slot_count(p.slots, p.experts, p.M, BN), n_items = n_slots * p.Nb;
-  auto load_weights = [&](int s, const Slot& slot, int f0, int kb) {
-    mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : C::kStage - C::kBTile);
+  // (extra bytes, which never come, under mtc_debug_withhold_bytes only: in
+  // the first stage, of one CTA of a cluster)
+  auto load_weights = [&](int s, const Slot& slot, int f0, int kb, bool first) {
+    mbar_expect_tx(&full[s], (SRC == SRC_CODES ? C::kStage : C::kStage - C::kBTile) +
+                                 (first && rank == 0 ? p.withhold : 0u));
     tc::tma_load_2d(smem + s * C::kStage, &tw0, kb * 128, slot.e * p.N + f0, &full[s]);
     if constexpr (PAIR) tc::tma_load_2d(smem + s * C::kStage + kATile, &tw1, kb * 128, slot.e * p.N + f0, &full[s]);
   };
   if (p.early) {
     if (tid == 128 && cid < n_items) {
       const Slot slot = slot_at(p.slots, p.experts, p.M, BN, cid % n_slots);
-      for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i, slot, cid / n_slots * 128, kb0 + i);
+      for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i, slot, cid / n_slots * 128, kb0 + i, i == 0);
     }
     griddep_wait();
   }
   griddep_launch_dependents();
 
   f32x2 acc[C::kCols / 2];  // sums of two tokens each
+  uint32_t issued = 0;      // thread 128: stages it has loaded
   if (warp == 4) {
     // ------------------------------------------------------------ weights (and codes of the tokens) by TMA
     if (lane == 0) {
@@ -249,17 +259,12 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
             abort_flag[0] = 1;
             break;
           }
-          if (!p.early || it >= C::kStages || w != cid) load_weights(s, slot, f0, kb0 + i);
+          if (!p.early || it >= C::kStages || w != cid) load_weights(s, slot, f0, kb0 + i, it == 0);
           if constexpr (SRC == SRC_CODES)
             tc::tma_load_2d(smem + s * C::kStage + C::kMats * kATile, &tx, (kb0 + i) * 128, slot.row0, &full[s]);
         }
       }
-      if (abort_flag[0]) {
-        // this CTA's copies in flight must land before it leaves
-        for (uint32_t j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
-          (void)mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, 10000000ull);
-        flag(p.status, MTC_STATUS_TIMEOUT);
-      }
+      issued = p.early && cid < n_items ? max(it, (uint32_t)min(n_it, C::kStages)) : it;
     }
   } else if (warp >= 5 && warp < 5 + C::kIssue) {
     // ------------------------------------------------------------ MMA: warp 5 + q issues the iterations q, q + kIssue, ...
@@ -288,11 +293,6 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
                         tc::smem_desc_k_sw128(b0 + 32 * j), idesc, j > 0);
         tc::commit(&acc_full[b]);
         tc::commit(&empty[s]);
-      }
-      if (abort_flag[0]) {
-        // no MMA may read shared memory or write TMEM after this CTA has left
-        tc::commit(&drain[q]);
-        (void)mbar_wait(&drain[q], 0, 100000000ull);
       }
     }
   } else if (warp < 4) {
@@ -527,29 +527,50 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
   }
   __syncwarp();
 
-  if (split > 1) {
-    // ------------------------------------------------------------ sums over the cluster
-    // All stages have been consumed: their memory takes the partial sums,
-    // [matrix][token][feature]; rank r completes the tokens r, r + split, ...,
-    // the partial sums added in rank order.
-    float* part = reinterpret_cast<float*>(smem);
-    const bool on = cid < n_items;
-    const Slot slot = on ? slot_at(p.slots, p.experts, p.M, BN, cid % n_slots) : Slot{};
-    const int ft = on ? cid / n_slots : 0, ntok = on ? min(BN, slot.end - slot.row0) : 0;
-    const int feat = 32 * warp + lane, f0 = 128 * ft;
-    if (warp < 4 && on) {
+  // A cluster's sums: all stages have been consumed, and their memory takes
+  // the partial sums, [matrix][token][feature].
+  float* part = reinterpret_cast<float*>(smem);
+  const bool on = split > 1 && cid < n_items;
+  const Slot slot = on ? slot_at(p.slots, p.experts, p.M, BN, cid % n_slots) : Slot{};
+  const int ft = on ? cid / n_slots : 0, ntok = on ? min(BN, slot.end - slot.row0) : 0;
+  const int feat = 32 * warp + lane, f0 = 128 * ft;
+  if (warp < 4 && on) {
 #pragma unroll
-      for (int j = 0; j < C::kCols; j += 2)
-        if ((j & (BN - 1)) < ntok) {
-          float x, y;
-          unpair(acc[j / 2], x, y);
-          part[j * 128 + feat] = x;
-          part[(j + 1) * 128 + feat] = y;
-        }
+    for (int j = 0; j < C::kCols; j += 2)
+      if ((j & (BN - 1)) < ntok) {
+        float x, y;
+        unpair(acc[j / 2], x, y);
+        part[j * 128 + feat] = x;
+        part[(j + 1) * 128 + feat] = y;
+      }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (abort_flag[0]) {
+    // A wait ran out in one of the warps (all of them see it here).  It is
+    // reported, and nothing of this CTA may be in flight when it leaves:
+    // neither copies into its shared memory nor MMAs that read it or write TMEM.
+    if (tid == 128) {
+      flag(p.status, MTC_STATUS_TIMEOUT);
+      for (uint32_t j = issued > C::kStages ? issued - C::kStages : 0; j < issued; ++j)
+        (void)mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, 10000000ull);
+    } else if (warp >= 5 && warp < 5 + C::kIssue && lane == 0) {
+      tc::commit(&drain[warp - 5]);
+      (void)mbar_wait(&drain[warp - 5], 0, 100000000ull);
     }
     __syncthreads();
+  }
+
+  if (split > 1) {
+    // ------------------------------------------------------------ sums over the cluster
+    // Rank r completes the tokens r, r + split, ..., the partial sums added in
+    // rank order; none if a rank gave up (its sums are not whole).
     tc::cluster_sync();
-    if ((!PAIR || warp < 4) && on && !abort_flag[0]) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q)
+      if (q < split) bad |= load_cluster1(abort_flag, q);
+    if ((!PAIR || warp < 4) && on) {
       // a warp (of all, or of those that quantize) per token, 4 features per
       // lane, all ranks' loads in flight
       const int n_warps = PAIR ? 4 : (int)(blockDim.x >> 5);
@@ -589,7 +610,7 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
           const long long y = (slot.row0 + j) * p.ldy + n4;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (n4 + q < p.N) {
+            if (n4 + q < p.N && !bad) {
               const float o = a[0][q] + bias[q];
               store1(p.Y, p.ydt, y + q, p.act ? epi_act(o, p.act) : o);
             }
@@ -597,13 +618,11 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
       }
       if constexpr (PAIR) {
         few_sync();
-        quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
+        if (!bad) quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
       }
     }
     tc::cluster_sync();  // no CTA leaves while another reads its partial sums
   }
-  tc::fence_before();
-  __syncthreads();
   if (warp == 5) {
     tc::fence_after();
     tc::tmem_dealloc(tmem, C::kAcc * C::kCols);
@@ -661,6 +680,7 @@ struct ManyParams {
   long long hs_ld;
   uint32_t* status;
   unsigned long long timeout_ns;
+  uint32_t withhold;                  // diagnostic: bytes that the first load of a CTA waits for in vain
 };
 
 // Barrier of the two warps that share rows (64 threads), which tells both
@@ -732,6 +752,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
+  uint32_t issued = 0;  // the loading thread: stages it has loaded
 
   if (warp >= kManyWarps) {
     regs_dec<kIssueRegs>();
@@ -760,18 +781,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
             const int s = it % kManyStages;
             uint8_t* st = smem + s * kManyStage;
-            mbar_expect_tx(&full[s], kManyStage);
+            mbar_expect_tx(&full[s], kManyStage + (it == 0 ? p.withhold : 0u));
             tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
             tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
             tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
           }
         }
-        if (abort_flag[0]) {
-          // nothing of this CTA may be in flight when it leaves
-          for (uint32_t j = it > kManyStages ? it - kManyStages : 0; j < it; ++j)
-            (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
-          flag(p.status, MTC_STATUS_TIMEOUT);
-        }
+        issued = it;
       }
     } else if (warp == kManyWarps + 3) {
       // ------------------------------------------------------------ scales and tiles
@@ -834,11 +850,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                       j > 0);
         tc::commit(&acc_full[b]);
         tc::commit(&empty[s]);
-      }
-      if (abort_flag[0]) {
-        // no MMA may read shared memory or write TMEM after this CTA has left
-        tc::commit(&drain[b]);
-        (void)mbar_wait(&drain[b], 0, 100000000ull);
       }
     }
   } else {
@@ -1018,6 +1029,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __syncwarp();
   tc::fence_before();
   __syncthreads();
+  if (abort_flag[0]) {
+    // a wait ran out: reported, and nothing left in flight (see few_kernel)
+    if (tid == 32 * kManyWarps) {
+      flag(p.status, MTC_STATUS_TIMEOUT);
+      for (uint32_t j = issued > kManyStages ? issued - kManyStages : 0; j < issued; ++j)
+        (void)mbar_wait(&full[j % kManyStages], (j / kManyStages) & 1, 10000000ull);
+    } else if ((warp == kManyWarps + 1 || warp == kManyWarps + 2) && lane == 0) {
+      tc::commit(&drain[warp - kManyWarps - 1]);
+      (void)mbar_wait(&drain[warp - kManyWarps - 1], 0, 100000000ull);
+    }
+    __syncthreads();
+  }
   if (warp == kManyWarps + 1) {
     tc::fence_after();
     tc::tmem_dealloc(tmem, 512);
@@ -1184,6 +1207,7 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
     p.hs_ld = a.hs_ld;
     p.status = a.status;
     p.timeout_ns = wait_limit_ns();
+    p.withhold = take_withheld_bytes();
     const long long work = (long long)a.slot_bound * p.n_tiles;
     const int grid = (int)(work < sms ? work : sms);
     if (n_mats == 2) {
@@ -1229,6 +1253,7 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   p.early = a.early;
   p.status = a.status;
   p.timeout_ns = wait_limit_ns();
+  p.withhold = take_withheld_bytes();
   const long long bound = (long long)Nb * a.slot_bound;
   const bool pair = n_mats == 2;
   if (a.xq) {

@@ -68,7 +68,8 @@ inline int read_epilogue(const mtc_epilogue* ep, EpiArg* out, const char* who) {
 
 // Limit of every bounded pipeline wait of the next launches, in ns (2 s
 // unless mtc_set_wait_limit_ns changed it), and the diagnostic hold of
-// mtc_debug_withhold_bytes, taken (and cleared) by the next strip launch.
+// mtc_debug_withhold_bytes, taken (and cleared) by the next launch of a strip
+// decode or an 8-bit product.
 unsigned long long wait_limit_ns();
 uint32_t take_withheld_bytes();
 
