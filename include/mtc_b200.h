@@ -154,13 +154,14 @@ MTC_API int mtc_device_sm_count(int device);
  * pipeline): a diagnostic of this library, also used by its tests. */
 MTC_API int mtc_set_wait_limit_ns(uint64_t ns);
 
-/* Diagnostic for tests of the timeout path: the NEXT mtc_strip_decode call, or
- * 8-bit product (mtc_fp8_gemm, the first one of mtc_experts_forward), of this
- * process, any thread, makes every warp's first batch (a product: every CTA's,
- * or the first CTA's of a cluster, first stage) expect `bytes` (a multiple of
- * 16, at most 4096) more than it copies, so that wait can never complete and
- * runs out at the wait limit; the call after it is unaffected.  0 cancels a
- * pending hold.  No counterpart in the reference. */
+/* Diagnostic for tests of the timeout path: the NEXT mtc_strip_decode call
+ * (this process, any thread) makes every warp's first batch expect `bytes`
+ * (a multiple of 16, at most 4096) more than it copies, so that wait can
+ * never complete and runs out at the wait limit; the call after it is
+ * unaffected.  If an 8-bit product comes first (mtc_fp8_gemm, the first one of
+ * mtc_experts_forward), it takes the hold: the first stage of every CTA (of
+ * the first CTA of a cluster) then never becomes full, whatever `bytes` is.
+ * 0 cancels a pending hold.  No counterpart in the reference. */
 MTC_API int mtc_debug_withhold_bytes(uint32_t bytes);
 
 /* Byte copy by the copy engines (cudaMemcpyAsync, device to device) on

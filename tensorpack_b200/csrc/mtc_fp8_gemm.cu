@@ -107,7 +107,7 @@ struct FewParams {
   int early;                          // slots and weights may be read before the predecessor ends
   uint32_t* status;
   unsigned long long timeout_ns;
-  uint32_t withhold;                  // diagnostic: bytes that the first load of a CTA waits for in vain
+  uint32_t withhold;                  // diagnostic: the first stage of a CTA never becomes full
 };
 
 template <int SRC>
@@ -206,7 +206,9 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
 
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&full[i], SRC == SRC_CODES ? 1 : 2);
+      // (one arrival too many under mtc_debug_withhold_bytes only: in the
+      // first stage, of one CTA of a cluster)
+      mbar_init(&full[i], (SRC == SRC_CODES ? 1 : 2) + (i == 0 && rank == 0 && p.withhold ? 1 : 0));
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < C::kAcc; ++i) {
@@ -224,18 +226,15 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
   const uint32_t tmem = *tmem_slot;
   if (!p.early) griddep_wait();
   const int n_slots = slot_count(p.slots, p.experts, p.M, BN), n_items = n_slots * p.Nb;
-  // (extra bytes, which never come, under mtc_debug_withhold_bytes only: in
-  // the first stage, of one CTA of a cluster)
-  auto load_weights = [&](int s, const Slot& slot, int f0, int kb, bool first) {
-    mbar_expect_tx(&full[s], (SRC == SRC_CODES ? C::kStage : C::kStage - C::kBTile) +
-                                 (first && rank == 0 ? p.withhold : 0u));
+  auto load_weights = [&](int s, const Slot& slot, int f0, int kb) {
+    mbar_expect_tx(&full[s], SRC == SRC_CODES ? C::kStage : C::kStage - C::kBTile);
     tc::tma_load_2d(smem + s * C::kStage, &tw0, kb * 128, slot.e * p.N + f0, &full[s]);
     if constexpr (PAIR) tc::tma_load_2d(smem + s * C::kStage + kATile, &tw1, kb * 128, slot.e * p.N + f0, &full[s]);
   };
   if (p.early) {
     if (tid == 128 && cid < n_items) {
       const Slot slot = slot_at(p.slots, p.experts, p.M, BN, cid % n_slots);
-      for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i, slot, cid / n_slots * 128, kb0 + i, i == 0);
+      for (int i = 0; i < min(n_it, C::kStages); ++i) load_weights(i, slot, cid / n_slots * 128, kb0 + i);
     }
     griddep_wait();
   }
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
             abort_flag[0] = 1;
             break;
           }
-          if (!p.early || it >= C::kStages || w != cid) load_weights(s, slot, f0, kb0 + i, it == 0);
+          if (!p.early || it >= C::kStages || w != cid) load_weights(s, slot, f0, kb0 + i);
           if constexpr (SRC == SRC_CODES)
             tc::tma_load_2d(smem + s * C::kStage + C::kMats * kATile, &tx, (kb0 + i) * 128, slot.row0, &full[s]);
         }
@@ -566,10 +565,8 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
     // Rank r completes the tokens r, r + split, ..., the partial sums added in
     // rank order; none if a rank gave up (its sums are not whole).
     tc::cluster_sync();
-    uint32_t bad = 0;
-#pragma unroll
-    for (int q = 0; q < kMaxCluster; ++q)
-      if (q < split) bad |= load_cluster1(abort_flag, q);
+    // (looked at when the sums are there: in flight with them)
+    const uint32_t gave_up = lane < split ? load_cluster1(abort_flag, lane) : 0u;
     if ((!PAIR || warp < 4) && on) {
       // a warp (of all, or of those that quantize) per token, 4 features per
       // lane, all ranks' loads in flight
@@ -608,6 +605,7 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
           *reinterpret_cast<float4*>(red + i * 128 + f4) = make_float4(h[0], h[1], h[2], h[3]);
         } else {
           const long long y = (slot.row0 + j) * p.ldy + n4;
+          const bool bad = __any_sync(0xffffffffu, gave_up);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (n4 + q < p.N && !bad) {
@@ -618,7 +616,7 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
       }
       if constexpr (PAIR) {
         few_sync();
-        if (!bad) quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
+        if (!__any_sync(0xffffffffu, gave_up)) quantize_staged(p, red, slot.row0, rank, split, count, f0, warp, lane);
       }
     }
     tc::cluster_sync();  // no CTA leaves while another reads its partial sums
@@ -680,7 +678,7 @@ struct ManyParams {
   long long hs_ld;
   uint32_t* status;
   unsigned long long timeout_ns;
-  uint32_t withhold;                  // diagnostic: bytes that the first load of a CTA waits for in vain
+  uint32_t withhold;                  // diagnostic: the first stage of a CTA never becomes full
 };
 
 // Barrier of the two warps that share rows (64 threads), which tells both
@@ -736,7 +734,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kManyStages; ++i) {
-      mbar_init(&full[i], 1 + 32 + 1);  // the codes, the lanes' scales, the tile
+      // the codes, the lanes' scales, the tile (and see few_kernel)
+      mbar_init(&full[i], 1 + 32 + 1 + (i == 0 && p.withhold ? 1 : 0));
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -781,7 +780,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
             const int s = it % kManyStages;
             uint8_t* st = smem + s * kManyStage;
-            mbar_expect_tx(&full[s], kManyStage + (it == 0 ? p.withhold : 0u));
+            mbar_expect_tx(&full[s], kManyStage);
             tc::tma_load_2d(st, &tx, kb * 128, slot.row0, &full[s]);
             tc::tma_load_2d(st + kATile, &tw0, kb * 128, f0, &full[s]);
             tc::tma_load_2d(st + 2 * kATile, GATED ? &tw1 : &tw0, kb * 128, GATED ? f0 : f0 + 128, &full[s]);
