@@ -484,11 +484,14 @@ MTC_API int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_type,
  * sigmoid.  The choice goes by score + bias (bias: E finite floats, or NULL)
  * in 64 bits; without bias and groups by the logits, whose order that is.
  * With groups > 1 (at most 32, dividing E) only the experts of the top_groups
- * groups with the largest sum of their two best choices compete.  ids: the k best, best first, ties to the lowest index; weights:
- * their scores (without bias), divided by their sum if renormalize, times
- * scale.  A logit of -inf or NaN is a masked expert: score 0, chosen only
- * when no other is left; +inf counts as the largest finite number.  A row
- * with masked experts only has weights 0. */
+ * groups with the largest sum of their two best choices compete.  ids: the k
+ * best, best first, ties to the lowest index; weights: their scores (without
+ * bias), divided by their sum if renormalize, times scale.  A logit of -inf or
+ * NaN is a masked expert: score 0, chosen only when no other of the competing
+ * ones is left, and never one of a group's two best: a group's only free
+ * expert counts alone, a group without one comes after all others.  +inf
+ * counts as the largest finite number.  A row with masked experts only has
+ * weights 0. */
 enum { MTC_SCORE_SOFTMAX = 0, MTC_SCORE_SIGMOID = 1 };
 MTC_API int mtc_route_experts(const void* logits, int32_t type, int32_t T, int32_t E, int64_t ld, int32_t k,
                               int32_t score, const float* bias, int32_t groups, int32_t top_groups,

@@ -86,7 +86,9 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteParams& p, const F* c
       g2 = g2 > o1 ? g2 : o1;
     }
   }
-  const F gv = p.gsize > 1 ? g1 + g2 : g1;
+  // (a masked expert, -inf here, adds nothing: a group's only free choice
+  // counts alone, and -inf is a group without any)
+  const F gv = g2 > -INFINITY ? g1 + g2 : g1;
   int rank = 0;
   for (int o = 0; o < p.groups; ++o) {
     const F v = __shfl_sync(0xffffffffu, gv, o * lanes);

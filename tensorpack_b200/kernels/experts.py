@@ -39,7 +39,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     their sum if ``renormalize``, times ``scale``.
 
     A logit of -inf or NaN masks its expert: score 0, chosen only when no
-    other is left; a row of masked experts gets weights 0.  +inf counts as the
+    other of the competing ones is left, and never one of a group's two best
+    (a group's only free expert counts alone, a group without one comes after
+    all others); a row of masked experts gets weights 0.  +inf counts as the
     largest finite number."""
     logits = _rows(logits, "route_experts")
     T, E = logits.shape
