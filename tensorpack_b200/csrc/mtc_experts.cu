@@ -126,20 +126,27 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
 // A warp per token.  The choice is made in 64 bits as defined (without bias
 // and groups by the logits), but reached in 32 where that is certain: the
 // fp32 choices are taken when every decision (between neighbours of the k + 1
-// best, at the groups' border) has a margin above the error, and made again
-// in 64 bits when one has not (about one token in a hundred).
+// best, at the groups' border) has a margin above twice the error of a choice,
+// and made again in 64 bits when one has not (one token in 600 of normal
+// logits, 256 experts in 8 groups).
 //
-// Error of an fp32 choice s + b, with M = max(|s + b| + s): the rounding of
-// the sum is below 2^-24 M.  __expf(x) is off by 2 ulp and |x| 2^-24, the
-// division by 2 ulp.  A sigmoid's error is below ((4 + |z|)(1 - s) + 5) s
-// 2^-24, where |z| s (1 - s) < 0.3; a softmax score's below (20 + 2 d) s 2^-24
-// for a logit d below the largest (the difference, its exponential, the
-// total, the division), where s d < s log(1/s) and so 2 s d < 5 M.  Twice
-// that is below 2^-19 M and 2^-17 M.
+// Error of an fp32 choice c = s + b, in units u = 2^-24 (a rounding is 1, an
+// ulp 2): |c| for the rounding of the sum, and that of s.  CUDA documents
+// 2 + 1.173 |x| ulp for __expf(x), 2 ulp for __fdividef.
+//  * Sigmoid 1 / (1 + exp(-z)): s (1 - s) (4 + 2.35 |z|) for the exponential,
+//    5 s for the sum and the division.  (1 - s) |z| is below 0.28 for z > 0,
+//    and with t = -z > 0 s t falls from t = 1.28 on, so that s t of any expert
+//    is at most that of the largest score, or 1.28 times the largest score:
+//    smax (9.7 + 2.35 max(t, 1.28)), t that of the largest logit.
+//  * Softmax, d the distance to the largest logit, smax = 1 / total: the
+//    difference and its exponential s (4 + 3.35 d), where s d < 0.37 smax; the
+//    total as much on average (s d adds up to log E < 7 at most) and
+//    NPL + 4 additions; division and product 5 s: smax (41.5 + NPL).
+// What is flushed to zero is below 2^-126.
 //
-// 8192 x 256 with groups and bias: 22.3 us (24.7 in 64 bits for all, which
-// also has twice the registers), bound by instruction issue; 24.8 without the
-// limit on registers that lets 48 warps share an SM.
+// 8192 x 256 with groups and bias: 21.6 us, bound by instruction issue.  (2 to
+// 3 us more in 64 bits for all, which also has twice the registers, or without
+// the limit on registers that lets 48 warps share an SM.)
 template <typename T, int NPL>
 __global__ void __launch_bounds__(256, NPL <= 8 ? 6 : 1) route_kernel(const RouteParams p) {
   extern __shared__ double route_smem[];
@@ -174,15 +181,17 @@ __global__ void __launch_bounds__(256, NPL <= 8 ? 6 : 1) route_kernel(const Rout
   float margin;
   bool sure = true;
   {
-    float c[NPL], most = 0.0f;
+    // (the hidden bits: below NPL ulp of each)
+    float c[NPL], most = 0.0f, error;
     if (by_logit) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         c[i] = v[i];
         if (v[i] != -INFINITY) most = fmaxf(most, fabsf(v[i]));
       }
+      error = 2.0f * NPL * most;
     } else {
-      float sum = 0.0f;
+      float sum = 0.0f, smax = 0.0f;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         c[i] = raw_score<float>(v[i], zmax, p.sigmoid);
@@ -200,13 +209,14 @@ __global__ void __launch_bounds__(256, NPL <= 8 ? 6 : 1) route_kernel(const Rout
         const float sc = c[i] * inv;
         c[i] = p.bias && e < p.E ? sc + p.bias[e] : sc;
         if (v[i] == -INFINITY) c[i] = -INFINITY;
-        else most = fmaxf(most, fabsf(c[i]) + sc);
+        else most = fmaxf(most, fabsf(c[i]));
+        smax = fmaxf(smax, sc);
       }
+      // (sigmoid: zmax and smax are the lane's, which bounds its own errors)
+      error = (1.0f + 2.0f * NPL) * most +
+              (p.sigmoid ? smax * (10.0f + 2.4f * fminf(fmaxf(-zmax, 1.3f), 128.0f)) : inv * (42.0f + NPL));
     }
-    most = warp_max(most);
-    // (the hidden bits: below NPL ulp of each)
-    margin = most * ((by_logit ? 0.0f : p.sigmoid ? 1.9073486328125e-6f : 7.62939453125e-6f) +
-                     2.0f * NPL * 1.1920928955078125e-7f);
+    margin = warp_max(error) * 1.1920928955078125e-7f + 4.70197740328915e-38f;  // 2 u, 2^-124
     uint32_t keep = ~0u;
     if (p.groups > 1) {
       float* cs = reinterpret_cast<float*>(route_smem + warp * p.E);
