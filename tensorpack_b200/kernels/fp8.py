@@ -197,12 +197,15 @@ class FP8Experts:
 
 class FP8Matrix(FP8Experts):
     """One K x N weight in e4m3 (``shape`` = (K, N)): codes (N, K), scales
-    (ceil(N/128), ceil(K/128))."""
+    (ceil(N/128), ceil(K/128)).
+
+    The ``scales`` attribute keeps the stack's leading axis,
+    (1, ceil(N/128), ceil(K/128)); ``from_codes`` takes either form."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        if codes.dim() != 2 or scales.dim() != 2:
+        if codes.dim() != 2 or scales.dim() not in (2, 3):
             raise ValueError("FP8Matrix: codes and scales must be matrices")
-        super().__init__(codes[None], scales[None])
+        super().__init__(codes[None], scales if scales.dim() == 3 else scales[None])
         self.shape = self.shape[1:]
 
     @classmethod
