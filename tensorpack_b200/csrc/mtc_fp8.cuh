@@ -135,30 +135,11 @@ __device__ __forceinline__ uint32_t amax_raw(const uint4 (&raw)[NV]) {
 }
 
 // Eight consecutive values at p as fp32; `n` of them exist (the others read
-// as zero).  `vec`: p is 16-byte aligned and n >= 8 may be read as vectors.
+// as zero).  One at a time: for rows that start or end off a vector.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        T lo, hi;
-        *reinterpret_cast<uint16_t*>(&lo) = (uint16_t)(w[i] & 0xffffu);
-        *reinterpret_cast<uint16_t*>(&hi) = (uint16_t)(w[i] >> 16);
-        v[2 * i] = to_f32(lo);
-        v[2 * i + 1] = to_f32(hi);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
-  }
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
 }
 
 // One output value in the output's type (fp32, or rounded once to nearest).

@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(FewCfg<BN, PAIR>::kThreads + (SRC == SRC_CODES
             for (int m = half; m < ((ntok + 1) & ~1); m += 2) {
               const long long row = __shfl_sync(0xffffffffu, at, m);
               float v[8];
-              load8(reinterpret_cast<const T*>(p.X) + row + k, m < ntok ? p.K - k : 0, false, v);
+              load8(reinterpret_cast<const T*>(p.X) + row + k, m < ntok ? p.K - k : 0, v);
               const GroupScale g = group_scale(half_warp_max(amax8(v)));
               put(m, v, g.mul);
               if (l == 0) my_scales[m] = g.scale;

@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
 #pragma unroll
         for (int q = 0; q < kVec; ++q) raw[u][q] = load16_if(reinterpret_cast<const uint4*>(x) + q, n > 0);
       } else {
-        load8(x, n, false, v[u]);
+        load8(x, n, v[u]);
       }
       g += step;
       m += step_m;
