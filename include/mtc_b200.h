@@ -426,7 +426,8 @@ MTC_API int mtc_rd_search(const float* W, int32_t K, int32_t N, int32_t block_si
  * counterpart in the reference.
  * ------------------------------------------------------------------------- */
 
-/* Element types of activations and outputs. */
+/* Element types of activations and outputs.  Every pointer below is aligned to
+ * its elements (others are refused). */
 enum { MTC_F32 = 0, MTC_BF16 = 1, MTC_F16 = 2 };
 
 /* E stacked K x N weights (in_features x out_features) in e4m3: codes as

@@ -528,7 +528,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
   }
 }
 
-bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16; }
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How the experts' products run, from the mean number of rows of an expert:
@@ -618,7 +617,9 @@ extern "C" int mtc_route_experts(const void* logits, int32_t type, int32_t T, in
                                  int32_t renormalize, float scale, int32_t* ids, float* weights, void* stream) {
   clear_error();
   MTC_REQUIRE(logits && ids && weights, "mtc_route_experts: null pointer");
-  MTC_REQUIRE(dtype_ok(type), "mtc_route_experts: unknown element type %d", type);
+  MTC_REQUIRE(type_ok(type), "mtc_route_experts: unknown element type %d", type);
+  MTC_REQUIRE(aligned(logits, type) && aligned(bias) && aligned(ids) && aligned(weights),
+              "mtc_route_experts: pointer not aligned to its elements");
   MTC_REQUIRE(score == MTC_SCORE_SOFTMAX || score == MTC_SCORE_SIGMOID, "mtc_route_experts: unknown score %d", score);
   MTC_REQUIRE(T >= 0 && T <= kMaxRows && E >= 1 && E <= kMaxExperts && ld >= E, "mtc_route_experts: bad shape (T=%d, E=%d, ld=%lld)", T,
               E, (long long)ld);
@@ -671,7 +672,9 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
               who);
   MTC_REQUIRE(gate->E <= kMaxExperts, "%s: %d experts, at most %d", who, gate->E, kMaxExperts);
   MTC_REQUIRE(X && ids && weights && Y, "%s: null pointer", who);
-  MTC_REQUIRE(dtype_ok(x_type) && dtype_ok(y_type), "%s: unknown element type", who);
+  MTC_REQUIRE(type_ok(x_type) && type_ok(y_type), "%s: unknown element type", who);
+  MTC_REQUIRE(aligned(X, x_type) && aligned(ids) && aligned(weights) && aligned(Y, y_type) && aligned(status),
+              "%s: pointer not aligned to its elements", who);
   MTC_REQUIRE(act >= MTC_ACT_NONE && act <= MTC_ACT_GELU_TANH, "%s: unknown activation %d", who, act);
   MTC_REQUIRE(T >= 1 && k >= 1 && k <= kMaxTopK && ldx >= gate->K && ldy >= gate->K,
               "%s: bad shape (T=%d, k=%d, ldx=%lld, ldy=%lld)", who, T, k, (long long)ldx, (long long)ldy);

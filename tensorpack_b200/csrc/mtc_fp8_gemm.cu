@@ -1144,6 +1144,7 @@ int check_matrix(const mtc_fp8_matrix* w, const char* who) {
   MTC_REQUIRE(w->ldk >= w->K && (w->ldk & 15) == 0, "%s: row stride %lld of the codes is not a multiple of 16 >= K",
               who, (long long)w->ldk);
   MTC_REQUIRE((reinterpret_cast<uintptr_t>(w->codes) & 15) == 0, "%s: codes not 16-byte aligned", who);
+  MTC_REQUIRE(aligned(w->scales), "%s: scales not aligned to their elements", who);
   MTC_REQUIRE((long long)w->E * w->N <= 0x7fffff00ll, "%s: more than 2^31 weight rows", who);
   return MTC_OK;
 }

@@ -50,6 +50,12 @@ struct Product {
 constexpr long long kMaxRows = 0x7fff0000ll;
 
 int check_matrix(const mtc_fp8_matrix* w, const char* who);
+
+inline bool type_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16; }
+// Whether p is aligned to elements of that type (fp32, or 4-byte words).
+inline bool aligned(const void* p, int dt = MTC_F32) {
+  return (reinterpret_cast<uintptr_t>(p) & (dt == MTC_F32 ? 3 : 1)) == 0;
+}
 int sm_count();
 
 // Launch with programmatic stream serialization: the kernel may start while

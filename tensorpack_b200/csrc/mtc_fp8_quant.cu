@@ -202,8 +202,6 @@ int launch_quantize(const QuantRows& a, cudaStream_t st, const char* who) {
 }
 
 namespace {
-bool dtype_ok(int dt) { return dt == MTC_F32 || dt == MTC_BF16 || dt == MTC_F16; }
-
 // How a dense product runs.  Times on the device, weights from memory.
 //  * Up to 8 rows the product quantizes the activations itself: 13.7 us at
 //    8 x 4096 x 14336 against 15.1 with the quantizer before it (its codes
@@ -244,6 +242,7 @@ extern "C" int mtc_fp8_pack(const float* W, int32_t K, int32_t N, int64_t ldw, u
                             float* scales, void* stream) {
   clear_error();
   MTC_REQUIRE(W && codes && scales, "mtc_fp8_pack: null pointer");
+  MTC_REQUIRE(aligned(W) && aligned(scales), "mtc_fp8_pack: pointer not aligned to its elements");
   MTC_REQUIRE(K >= 1 && N >= 1 && ldw >= N && ldk >= K && (ldk & 15) == 0, "mtc_fp8_pack: bad shape or strides");
   const dim3 grid((K + 127) / 128, (N + 127) / 128);
   MTC_REQUIRE(grid.y <= 65535, "mtc_fp8_pack: N=%d too large", N);
@@ -257,6 +256,7 @@ extern "C" int mtc_fp8_unpack(const mtc_fp8_matrix* w, int32_t e, float* out, in
   const int rc = check_matrix(w, "mtc_fp8_unpack");
   if (rc != MTC_OK) return rc;
   MTC_REQUIRE(out && ldo >= w->N && e >= 0 && e < w->E, "mtc_fp8_unpack: bad argument");
+  MTC_REQUIRE(aligned(out), "mtc_fp8_unpack: pointer not aligned to its elements");
   const dim3 grid((w->K + 127) / 128, (w->N + 127) / 128);
   MTC_REQUIRE(grid.y <= 65535, "mtc_fp8_unpack: N=%d too large", w->N);
   unpack_kernel<<<grid, 256, 0, as_stream(stream)>>>(w->codes + (long long)e * w->N * w->ldk, w->ldk,
@@ -270,7 +270,8 @@ extern "C" int mtc_fp8_quantize(const void* X, int32_t x_type, int32_t M, int32_
                                 int64_t ldq, float* scales, int64_t lds, void* stream) {
   clear_error();
   MTC_REQUIRE(X && codes && scales, "mtc_fp8_quantize: null pointer");
-  MTC_REQUIRE(dtype_ok(x_type), "mtc_fp8_quantize: unknown element type %d", x_type);
+  MTC_REQUIRE(type_ok(x_type), "mtc_fp8_quantize: unknown element type %d", x_type);
+  MTC_REQUIRE(aligned(X, x_type) && aligned(scales), "mtc_fp8_quantize: pointer not aligned to its elements");
   MTC_REQUIRE(M >= 0 && M <= kMaxRows && K >= 1 && K <= kMaxRows && ldx >= K, "mtc_fp8_quantize: bad shape (M=%d, K=%d, ldx=%lld)", M, K,
               (long long)ldx);
   MTC_REQUIRE(ldq >= K && (ldq & 15) == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && lds >= M,
@@ -301,7 +302,8 @@ extern "C" int mtc_fp8_gemm(const mtc_fp8_matrix* w, const void* X, int32_t x_ty
   if (rc != MTC_OK) return rc;
   MTC_REQUIRE(w->E == 1, "mtc_fp8_gemm: %d stacked matrices", w->E);
   MTC_REQUIRE(X && Y, "mtc_fp8_gemm: null pointer");
-  MTC_REQUIRE(dtype_ok(x_type) && dtype_ok(y_type), "mtc_fp8_gemm: unknown element type");
+  MTC_REQUIRE(type_ok(x_type) && type_ok(y_type), "mtc_fp8_gemm: unknown element type");
+  MTC_REQUIRE(aligned(X, x_type) && aligned(Y, y_type) && aligned(status), "mtc_fp8_gemm: pointer not aligned to its elements");
   MTC_REQUIRE(M >= 1 && M <= kMaxRows && ldx >= w->K && ldy >= w->N, "mtc_fp8_gemm: bad shape (M=%d, ldx=%lld, ldy=%lld)", M,
               (long long)ldx, (long long)ldy);
   EpiArg epa;
