@@ -531,19 +531,21 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How the experts' products run, from the mean number of rows of an expert:
-// up to 12, 16-row tiles whose tokens the first product quantizes itself; up
-// to 20, 32-row tiles of codes; above, the 128-token kernel.  Device times
-// of the three at a mean of m rows:
-//    64 experts, 2048 x 1024:   m = 12  93 / 102 / 119 us   m = 16  107 / 107 / 120
-//                               m = 20 131 / 117 / 125      m = 24  142 / 127 / 125
-//   128 experts, 2048 x 768:    m = 8  121 / 134 / 165      m = 16  161 / 152 / 168
-//     8 experts, 4096 x 14336:  m = 8  264 / 276 / 277      m = 16  334 / 296 / 281
-//   256 experts, 1024 x 512:    m = 8   99 / 106 / 132      m = 24  182 / 151 / 140
+// up to 12, 16-row tiles whose tokens the first product quantizes itself;
+// above, the 128-token kernel on quantized rows.  Device times of the two at a
+// mean of m rows:
+//    64 experts, 2048 x 1024:   m = 10   91 /  96 us   m = 12   93 /  99   m = 14  103 / 100   m = 24  143 / 104
+//   128 experts, 2048 x 768:    m = 8   125 / 133      m = 12  135 / 139   m = 14  144 / 141   m = 16  162 / 138
+//     8 experts, 4096 x 14336:  m = 8   268 / 258      m = 12  267 / 275   m = 14  264 / 258   m = 16  358 / 280
+//   256 experts, 1024 x 512:    m = 8    99 / 144      m = 10  103 / 110   m = 12  113 /  98   m = 24  184 / 105
+//     6 experts, 272 x 264:     m = 14   18 /  20
+// (Tiles of 32 rows, between the two, were ahead of neither: 102, 111 and 126
+// us at m = 12, 16 and 24 of the first.)
 // A single token needs no plan: every row is a slot (20.2 us a call with 8 of
 // 64 experts, 25.7 with a plan).
 struct ExpertsPlan {
   int R, tile, slot_bound;
-  bool direct, raw, many;
+  bool direct, raw;
   long long ldx, ldh, lds, ldo;
   int plan_ctas;
   size_t order, pos, slots, counts, xq, xs, hq, hs, out, bytes;
@@ -555,8 +557,7 @@ bool experts_plan(int T, int k, int E, int D, int I, ExpertsPlan* pl) {
   const double mean = (double)R / E;
   pl->direct = T == 1;
   pl->raw = pl->direct || mean <= 12.0;
-  pl->many = !pl->raw && mean > 20.0;
-  pl->tile = pl->raw ? 16 : pl->many ? 128 : 32;
+  pl->tile = pl->raw ? 16 : 128;
   const long long used = R < E ? R : E;
   long long bound = R / pl->tile + used;
   if (bound > R || pl->direct) bound = R;
@@ -708,7 +709,7 @@ extern "C" int mtc_experts_forward(const mtc_fp8_matrix* gate, const mtc_fp8_mat
   a.slot_bound = pl.slot_bound;
   a.rows = pl.R;
   a.tile = pl.tile;
-  a.many = pl.many;
+  a.many = !pl.raw;
   a.gate_act = act;
   a.status = status;
   Product b = a;

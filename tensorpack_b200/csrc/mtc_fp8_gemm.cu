@@ -1081,7 +1081,7 @@ int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap
   return MTC_OK;
 }
 
-// Tiles that gate / up pairs come in, too.
+// Tiles that gate / up pairs come in, too: activations.
 template <int BN, int SRC>
 int launch_few(const CUtensorMap& tw0, const CUtensorMap& tw1, const CUtensorMap& tx, FewParams& p, long long bound,
                int sms, bool pair, cudaStream_t st, const char* who) {
@@ -1263,11 +1263,10 @@ int launch_product(const Product& a, cudaStream_t st, const char* who) {
   const long long bound = (long long)Nb * a.slot_bound;
   const bool pair = n_mats == 2;
   if (a.xq) {
-    // (pairs in tiles of 16 bring activations, those in tiles of 32 codes)
-    if (a.tile == 32) return launch_few<32, SRC_CODES>(tw[0], tw[1], tx, p, bound, sms, pair, st, who);
-    MTC_REQUIRE(!pair, "%s: a gate / up pair in tiles of %d rows", who, a.tile);
+    MTC_REQUIRE(!pair, "%s: codes of a gate / up pair in tiles of %d rows", who, a.tile);
     switch (a.tile) {
       case 16: return launch_few<16, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
+      case 32: return launch_few<32, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
       case 64: return launch_few<64, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
       default: return launch_few<128, SRC_CODES, false>(tw[0], tw[1], tx, p, bound, sms, st, who);
     }

@@ -209,10 +209,11 @@ namespace {
 //  * The kernel for few rows takes them in tiles that waste at most half of
 //    the MMA.  From 65 rows on the 128 x 256 tiles take over where the few
 //    kernel could not split its inputs any more, that is, where its 128 x 128
-//    tiles fill more than half of the SMs: 26 against 48 us at
-//    129 x 4096 x 14336, 18.0 / 18.7 at 256 x 2048 x 8192 (128 tiles), but
-//    24.4 / 18.4 at 200 x 4096 x 4096 (64), 13.3 / 12.3 at 700 x 1024 x 1536
-//    (72) and 43 / 14.7 at 333 x 4864 x 901 (24).
+//    tiles fill more than half of the SMs: 25 against 48 us at
+//    129 x 4096 x 14336, 17.2 / 18.7 at 256 x 2048 x 8192 (128 tiles), but
+//    23.0 / 18.5 at 200 x 4096 x 4096 (64), 16.6 / 14.9 at 128 x 2048 x 8192
+//    (64), 12.3 / 12.6 at 700 x 1024 x 1536 (72) and 27 / 14.1 at
+//    333 x 4864 x 901 (24).
 struct DensePlan {
   int tile;
   bool many, raw;

@@ -68,7 +68,7 @@ def test_a_product_whose_wait_runs_out(dev, M, K, N, dtype):
 @pytest.mark.parametrize("T,E,k,D,I", [
     (1, 16, 4, 1200, 130), (6, 16, 4, 300, 260),   # activations quantized inside, without and with a plan
     (20, 4, 2, 2048, 128),                         # split
-    (120, 16, 2, 260, 200),                        # tiles of 32 rows
+    (120, 16, 2, 260, 200),                        # a few rows more than those take
     (700, 4, 2, 200, 150), (1000, 8, 2, 1100, 300),  # the kernel for many rows
 ])
 def test_experts_whose_wait_runs_out(dev, T, E, k, D, I):
