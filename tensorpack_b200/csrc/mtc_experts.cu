@@ -144,7 +144,7 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
 //    NPL + 4 additions; division and product 5 s: smax (41.5 + NPL).
 // What is flushed to zero is below 2^-126.
 //
-// 8192 x 256 with groups and bias: 21.6 us, bound by instruction issue.  (2 to
+// 8192 x 256 with groups and bias: 22 us, bound by instruction issue.  (2 to
 // 3 us more in 64 bits for all, which also has twice the registers, or without
 // the limit on registers that lets 48 warps share an SM.)
 template <typename T, int NPL>
@@ -392,7 +392,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const PlanPara
 
 // Each warp owns 32 rows: it counts its experts, the counts of all warps and
 // CTAs become places (experts in order, inside an expert the rows in order),
-// and the rows take them.  The first CTA writes the slot list.
+// and the rows take them.  The first CTA writes the slot list.  Every CTA reads
+// the counts of all, so the time grows with the square of the rows: 6 us for
+// 32768 rows, 0.02 ms for 2^18, 0.2 ms for 2^20 (of some 1 ms for all kernels
+// at 128 x 128), but 10 ms for 2^23 with 64 or 256 experts, 18 ms with 1024.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   extern __shared__ int32_t hist[];  // [32][E]
   __shared__ int warp_sums[33];
@@ -455,7 +458,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
 // ---------------------------------------------------------------------------
 // Y[t] = sum_j weights[t][j] * rows[pos[t][j]], j in order
 // ---------------------------------------------------------------------------
-// Rows and sum are fp32, rounded once to Y's type.
+// Rows and sum are fp32, rounded once to Y's type.  Bound by memory: 32768
+// rows of 2048 take 45 us (6.3 TB/s).
 struct CombineParams {
   const float* rows;
   long long ldr;
@@ -541,8 +545,11 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 //     6 experts, 272 x 264:     m = 14   18 /  20
 // (Tiles of 32 rows, between the two, were ahead of neither: 102, 111 and 126
 // us at m = 12, 16 and 24 of the first.)
-// A single token needs no plan: every row is a slot (20.2 us a call with 8 of
-// 64 experts, 25.7 with a plan).
+// A single token needs no plan: every row is a slot (20.9 us a call with 8 of
+// 64 experts, some 5 more with a plan).
+// (R / E counts every id, also those of no expert here: with few of them the
+// 128-token kernel runs for less than 13 rows of an expert.  The host cannot
+// know.)
 struct ExpertsPlan {
   int R, tile, slot_bound;
   bool direct, raw;

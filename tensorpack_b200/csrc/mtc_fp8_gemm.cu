@@ -10,7 +10,7 @@
 //    costs 16 columns instead of 128 rows, and a warp's stores are
 //    consecutive features.  Bound by the weight bytes: a persistent CTA per
 //    SM streams its features' codes once through a TMA ring (1 x 4096 x 14336
-//    13.4 us, 4.4 TB/s with some 3 us of start-up; 16 x 14336 x 4096 17.1 us
+//    13.9 us, 4.2 TB/s with some 3 us of start-up; 16 x 14336 x 4096 17.5 us
 //    with the quantizer).  When there are few tiles a cluster of up to 8 CTAs
 //    splits the inputs and adds its partial sums through distributed shared
 //    memory in rank order: no workspace, no atomics, the same result every
@@ -19,10 +19,10 @@
 //  * many_kernel<MODE>: 128 tokens x 256 features (TMEM lane = token), one
 //    persistent CTA per SM, two 256-column accumulators that alternate
 //    between the MMA and eight warps that scale and add.  4096 x 4096 x 14336
-//    takes 245 us with the quantizer, 1.96 PFLOP/s: 208 us with the scaling
+//    takes 246 us with the quantizer, 1.96 PFLOP/s: 208 us with the scaling
 //    taken out, 176 us with the MMAs taken out, 150 us with both (loads and
 //    stores alone), so each of them waits for another.  After some 50 ms the
-//    power limit lowers the clock (1965 to 1540 MHz) and it takes 285 us.
+//    power limit lowers the clock (1965 to 1540 MHz) and it takes 289 us.
 //    kGated: the 256 features are 128 of the gate matrix and the same 128 of
 //    the up matrix; the output is act(gate) * up, quantized.
 #include <string.h>
